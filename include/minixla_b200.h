@@ -14,8 +14,9 @@
  * (the result is on the host when the call returns); a GpuCtx is used from
  * one host thread at a time for graph execution (gpu_execute and friends).
  * The device-pointer launches (mxb_fused_gemm, mxb_fused_gemm2, mxb_add,
- * mxb_relu) only touch the context's pool, which is locked, and may come
- * from several threads.
+ * mxb_relu, mxb_layer_norm, mxb_q4_gemm, mxb_grouped_gemm and their backward
+ * forms) only touch the context's pool, which is locked, and may come from
+ * several threads.
  */
 #ifndef MINIXLA_B200_H
 #define MINIXLA_B200_H
@@ -171,7 +172,8 @@ MXB_API int     gpu_ctx_device(const GpuCtx* ctx);
 /* ---- Device-pointer entry points ----------------------------------------
  * For callers that keep operands resident in HBM (benchmarks, frameworks):
  * no host copies.  All pointers are device pointers of the context's device;
- * `stream` is a cudaStream_t (NULL = the context's own stream).  Launches are
+ * `stream` is a cudaStream_t (NULL = the context's own stream; pass
+ * cudaStreamLegacy, 0x1, for the legacy default stream).  Launches are
  * asynchronous on that stream.  Return 0 on success, a negative MXB_E* code
  * on failure (and one stderr line).
  */
@@ -181,7 +183,8 @@ enum {
     MXB_EP_ADD_MOD  = 2,  /* x += operand[(i*N + j) % size]  (eval_fused's rule)       */
     MXB_EP_RELU     = 3,  /* x = x > 0 ? x : 0                                         */
     MXB_EP_SCALE    = 4,  /* x *= scale                                                */
-    MXB_EP_ADD_PRODUCT = 5 /* x += (A2 @ B2)[i,j]  (mxb_fused_gemm2's second product)   */
+    MXB_EP_ADD_PRODUCT = 5, /* x += (A2 @ B2)[i,j]  (mxb_fused_gemm2's second product)  */
+    MXB_EP_RELU_GRAD = 6  /* x = operand[i*ld + j] > 0 ? x : 0  (grouped products only)  */
 };
 #define MXB_MAX_EPILOGUE 16   /* the reference fuses at most 16 steps (optimizer.c:104-107) */
 
@@ -347,6 +350,89 @@ MXB_API int mxb_gemm_plan_batch_for(long long batch, int M, int N, int K, int pr
 MXB_API int mxb_add(GpuCtx* ctx, const float* a, long long n, const float* b, long long b_size,
             float* out, void* stream);
 MXB_API int mxb_relu(GpuCtx* ctx, const float* x, long long n, float* out, void* stream);
+
+/* ---- Layer norm ----------------------------------------------------------
+ * No counterpart in the reference.  For each of `rows` rows of x (row pitch
+ * ldx >= cols), with mean and variance over its `cols` values:
+ *   rstd = 1 / sqrt(var + eps),  y = (x - mean) * rstd * gamma + beta.
+ * gamma and beta ([cols]) may be NULL (ones, zeros).  mean and rstd ([rows])
+ * are written when not NULL; the backward pass reads them.  y may be x itself
+ * (same pointer and pitch).  rows == 0 does nothing.  No alignment is needed;
+ * 16-byte aligned bases and pitches that are multiples of 4 run widest. */
+MXB_API int mxb_layer_norm(GpuCtx* ctx, const float* x, long long ldx, const float* gamma, const float* beta,
+                   float eps, float* y, long long ldy, float* mean, float* rstd, long long rows, int cols,
+                   void* stream);
+
+/* The backward pass.  With v = dy * gamma and xhat = (x - mean) * rstd:
+ *   dx = rstd * (v - mean(v) - xhat * mean(v * xhat))    (means over the row)
+ *   dgamma = sum over rows of dy * xhat,  dbeta = sum over rows of dy.
+ * Each of dx, dgamma, dbeta may be NULL (not wanted; not all three).  dx may
+ * be dy or x itself.  The sums over rows are made in a fixed order: the same
+ * inputs give the same bits.  rows == 0 writes zeros to dgamma and dbeta.
+ * Partial sums use pooled workspace of the context; on a stream that is being
+ * captured the workspace is an allocation of the graph itself, so captured
+ * calls share nothing with other calls or graphs. */
+MXB_API int mxb_layer_norm_backward(GpuCtx* ctx, const float* dy, long long lddy, const float* x, long long ldx,
+                   const float* gamma, const float* mean, const float* rstd, float* dx, long long lddx,
+                   float* dgamma, float* dbeta, long long rows, int cols, void* stream);
+
+/* ---- Products with 4-bit weights -----------------------------------------
+ * No counterpart in the reference.  out[M,N] = epi(A[M,K] @ W), with W held
+ * in 4 bits and a scale for each `group` values along K:
+ *   W[k, n] = (q[n, k] - z[n, k / group]) * scales[n * lds + k / group].
+ * Q: N rows of ldq bytes, two values to a byte, the lower k in the low four
+ * bits (ldq % 16 == 0, 16-byte aligned, ldq >= (K + 1) / 2; what lies behind
+ * column K is not used).  scales: MXB_SCALE_* values, row pitch lds elements;
+ * zeros: one byte (its low four bits) per scale, same pitch, or NULL for 8
+ * everywhere.  group is a multiple of 32.  A needs a 16-byte aligned base and
+ * lda % 4 == 0.  Epilogue steps as mxb_fused_gemm.  Products and sums are
+ * fp32-faithful (the activations enter as exact bf16 parts, every
+ * weight value q - z is exact in bf16, and each group's sum is scaled in
+ * fp32), independent of the context's precision mode.  Workspace as for
+ * mxb_layer_norm_backward. */
+enum {
+    MXB_SCALE_F32 = 0,
+    MXB_SCALE_F16 = 1,
+    MXB_SCALE_BF16 = 2
+};
+MXB_API int mxb_q4_gemm(GpuCtx* ctx, const float* A, long long lda, const unsigned char* Q, long long ldq,
+                   const void* scales, int scale_type, const unsigned char* zeros, long long lds, int group,
+                   float* out, long long ldo, int M, int N, int K, const mxb_ep_step* steps, int n_steps,
+                   void* stream);
+
+/* ---- Products grouped by expert ------------------------------------------
+ * No counterpart in the reference.  Rows offsets[e] .. offsets[e+1] - 1 of A
+ * belong to group e and are multiplied by its own matrix, all groups in one
+ * launch:
+ *   out[r, :] = epi(A[r, :] @ B_e),   B_e = B + e * b_stride  (K x N, pitch ldb).
+ * offsets: groups + 1 non-decreasing values in 0 .. rows, in device memory
+ * (never read on the host).  A group may be empty; rows of A and out that lie
+ * in no group are neither used nor written.  Values outside 0 .. rows, or
+ * decreasing ones, are taken as the nearest allowed value, so that no access
+ * leaves the buffers.  groups <= MXB_MAX_GROUPS; lda, ldb and b_stride are
+ * multiples of 4, A and B 16-byte aligned.  Steps: ADD_FULL, RELU, SCALE and
+ * RELU_GRAD as named above (i: the row of out), and ADD_ROW with
+ * operand[e * ld_or_size + j] (ld_or_size 0: one row for all groups).
+ * precision as mxb_fused_gemm.  rows == 0 does nothing. */
+#define MXB_MAX_GROUPS 1024
+MXB_API int mxb_grouped_gemm(GpuCtx* ctx, const float* A, long long lda, const float* B, long long ldb,
+                   long long b_stride, const int* offsets, int groups, float* out, long long ldo, int rows, int N,
+                   int K, const mxb_ep_step* steps, int n_steps, int precision, void* stream);
+
+/* Gradient of the rows: dA[r, :] = epi(dY[r, :] @ B_e^T), dA [rows, K], dY
+ * [rows, N].  An MXB_EP_RELU_GRAD step with the layer's saved input (the
+ * output of the relu before it) gives the gradient through that relu. */
+MXB_API int mxb_grouped_gemm_grad_a(GpuCtx* ctx, const float* dY, long long lddy, const float* B, long long ldb,
+                   long long b_stride, const int* offsets, int groups, float* dA, long long ldda, int rows, int N,
+                   int K, const mxb_ep_step* steps, int n_steps, int precision, void* stream);
+
+/* Gradient of the weights: dB_e = A_e^T @ dY_e over group e's rows (zeros for
+ * an empty group), dB_e = dB + e * db_stride (K x N, pitch lddb), and, when
+ * dbias is not NULL, dbias[e * N + j] = the sum of dY[r, j] over them.  lda and
+ * lddy are multiples of 4, A and dY 16-byte aligned. */
+MXB_API int mxb_grouped_gemm_grad_b(GpuCtx* ctx, const float* A, long long lda, const float* dY, long long lddy,
+                   const int* offsets, int groups, float* dB, long long lddb, long long db_stride, float* dbias,
+                   int rows, int N, int K, int precision, void* stream);
 
 /* Synchronises the context's device work and reports a device-side error
  * recorded by a kernel (MXB_E_TIMEOUT after a bounded wait ran out), then

@@ -211,6 +211,39 @@ struct GpuCtx {
 
 namespace mxb {
 
+// Workspace of one call: pooled and given back, stream-ordered, when the call
+// has launched its work.  On a stream that is being captured it is an
+// allocation of the graph itself (a memory node, freed by the graph), so a
+// replay never shares it with later calls, with the pool or with other graphs.
+class Scratch {
+  public:
+    Scratch(GpuCtx* ctx, cudaStream_t stream) : ctx_(ctx), stream_(stream) {}
+    Scratch(const Scratch&) = delete;
+    Scratch& operator=(const Scratch&) = delete;
+    ~Scratch() {
+        if (!p_) return;
+        if (in_graph_) {
+            cudaFreeAsync(p_, stream_);
+        } else {
+            ctx_->pool->release(p_, stream_);
+        }
+    }
+    void* alloc(size_t bytes) {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        if (!cuda_ok(cudaStreamIsCapturing(stream_, &status), "capture query")) return nullptr;
+        in_graph_ = status != cudaStreamCaptureStatusNone;
+        if (!in_graph_) return p_ = ctx_->pool->alloc(bytes, stream_);
+        if (!cuda_ok(cudaMallocAsync(&p_, bytes, stream_), "workspace of a captured call")) p_ = nullptr;
+        return p_;
+    }
+
+  private:
+    GpuCtx* ctx_;
+    cudaStream_t stream_;
+    void* p_ = nullptr;
+    bool in_graph_ = false;
+};
+
 struct Info {
     const Node* node = nullptr;
     std::vector<int> dims;        // logical output shape

@@ -17,10 +17,15 @@ LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libminixla_b200.so"
 GPU_PRECISION_TF32 = 1
 GPU_PRECISION_3XTF32 = 3
 
-MXB_EP_ADD_FULL, MXB_EP_ADD_ROW, MXB_EP_ADD_MOD, MXB_EP_RELU, MXB_EP_SCALE, MXB_EP_ADD_PRODUCT = range(6)
+MXB_EP_ADD_FULL, MXB_EP_ADD_ROW, MXB_EP_ADD_MOD, MXB_EP_RELU, MXB_EP_SCALE, MXB_EP_ADD_PRODUCT, MXB_EP_RELU_GRAD = range(7)
+MXB_SCALE_F32, MXB_SCALE_F16, MXB_SCALE_BF16 = range(3)
 MXB_OK, MXB_E_ARG, MXB_E_CUDA, MXB_E_NOMEM, MXB_E_TIMEOUT, MXB_E_UNSUPPORTED = 0, -1, -2, -3, -4, -5
 MXB_MAX_EPILOGUE = 16
 MXB_MAX_PEERS = 7
+MXB_MAX_GROUPS = 1024
+# cudaStreamLegacy: torch's default stream has handle 0, which the library
+# reads as "the context's own stream"; this handle names the default stream.
+CUDA_STREAM_LEGACY = 1
 MXB_IPC_HANDLE_BYTES = 64
 
 # Every symbol the header declares, with (restype, argtypes).
@@ -72,6 +77,36 @@ PROTOTYPES = {
     "mxb_gemm_plan_batch_for": (C.c_int, [C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "mxb_add": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p]),
     "mxb_relu": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p]),
+    "mxb_layer_norm": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_longlong,
+         C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p],
+    ),
+    "mxb_layer_norm_backward": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_void_p,
+         C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_void_p],
+    ),
+    "mxb_q4_gemm": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_void_p,
+         C.c_longlong, C.c_int, C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p],
+    ),
+    "mxb_grouped_gemm": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p, C.c_int,
+         C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p],
+    ),
+    "mxb_grouped_gemm_grad_a": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_longlong, C.c_void_p, C.c_int,
+         C.c_void_p, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p],
+    ),
+    "mxb_grouped_gemm_grad_b": (
+        C.c_int,
+        [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_void_p,
+         C.c_longlong, C.c_longlong, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p],
+    ),
     "mxb_check_device_error": (C.c_int, [C.c_void_p]),
     "mxb_selftest_wait_timeout": (C.c_int, [C.c_void_p, C.c_ulonglong]),
     "mxb_launch_count": (C.c_ulonglong, []),
