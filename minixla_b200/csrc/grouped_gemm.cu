@@ -3,10 +3,35 @@
 //   forward  out[r, n]   = epi(sum over k of A[r, k] * B_e[k, n])
 //   grad_a   dA[r, k]    = epi(sum over n of dY[r, n] * B_e[k, n])
 //   grad_b   dB_e[k, n]  = sum over the group's rows r of A[r, k] * dY[r, n],  dbias[e, n] = sum over r of dY[r, n]
+//
+// All three run on one tcgen05 kernel.  The tile is turned around compared
+// with the dense GEMMs: the dimension along which the result is contiguous
+// (n, or k in grad_a) lies along the tensor core's 128 rows and TMEM lanes,
+// the ragged dimension (the group's rows; k in grad_b) along its columns.
+// A group with few rows then costs an MMA of 16 columns instead of 128 rows,
+// the column count follows each tile's own rows at run time, and a warp
+// stores 32 consecutive floats of one output row at a time whatever the
+// pitch.  A lane-side tile of the weights is read where it lies: MN-major
+// (forward, grad_b) or K-major (grad_a), by the MMA descriptor alone.
+//
+// Which tile belongs to which group is found on the device from `offsets`
+// (a scan at the start of the kernel, a search per tile), so nothing is read
+// back to the host and a captured call follows the offsets of each replay.
+//
+// 3xTF32: x = big + small, three TF32 products.  The tensor core itself cuts
+// an fp32 operand to its upper 19 bits, so the tile that TMA loaded serves as
+// big, and four warps write small = x - big (rounded to the nearest TF32) to a
+// second tile: no pass over the weights beforehand, which would cost two to
+// three times the bytes of the product where a group has few rows.  K is
+// summed in segments of 64, each in a fresh accumulator, because the tensor
+// core cuts its running sums toward zero; the epilogue warps add the segments
+// in fp32 registers.
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <exception>
+
+#include "gemm_common.cuh"
 
 #include "epilogue_cell.cuh"
 #include "runtime_internal.h"
@@ -17,7 +42,7 @@ namespace {
 
 enum GroupedMode : int { kForward, kGradA, kGradB };
 
-struct GroupedParams {
+struct GroupedCall {
     int mode;
     const float* x;      // forward: A; grad_a: dY; grad_b: A          (row matrix)
     long long ldx;
@@ -29,98 +54,595 @@ struct GroupedParams {
     long long ldo, out_stride;
     float* dbias;
     int N, K;
+};
+
+struct GroupedParams {
+    const int* offsets;
+    int groups, rows;
+    float* out;
+    long long ldo, out_stride;  // out_stride: grad_b, between groups
+    int lane_dim;               // columns of the result: N, or K in grad_a
+    int col_dim;                // grad_b: K (else each group's rows)
+    int sum_dim;                // forward: K, grad_a: N (grad_b: each group's rows)
+    int lane_tiles;
+    int split3;                 // 3xTF32
+    unsigned long long timeout_ns;
+    int* err;
     CellEpilogue epi;
 };
 
-// Group e's rows [r0, r1), whatever offsets holds: 0 <= r0 <= r1 <= rows.
-__device__ __forceinline__ void group_rows(const GroupedParams& p, int e, int& r0, int& r1) {
-    r0 = min(max(__ldg(p.offsets + e), 0), p.rows);
-    r1 = min(max(__ldg(p.offsets + e + 1), r0), p.rows);
+// BT: tile columns, the most rows of a group (grad_b: columns of A) that one tile takes.
+template <int BT>
+struct GroupedCfg {
+    static constexpr int kLaneBytes = 128 * kBK * 4;
+    static constexpr int kColBytes = BT * kBK * 4;
+    static constexpr int kStageBytes = kLaneBytes + kColBytes;
+    static constexpr int kStages = BT <= 32 ? 8 : 4;  // tiles as loaded
+    static constexpr int kSmall = 2;                  // their small parts
+    static constexpr int kEpiWarps = BT <= 32 ? 4 : 8;
+    static constexpr int kThreads = 32 * (kEpiWarps + 6);  // epilogue, 4 converter warps, TMA, MMA
+    static constexpr int kTmemCols = 2 * BT;          // two segment buffers
+    static constexpr int kTotals = BT * 4 / kEpiWarps;  // columns of one epilogue thread
+    static constexpr int kSmallOffset = kStages * kStageBytes;
+    static constexpr int kTableOffset = kSmallOffset + kSmall * kStageBytes;
+    static constexpr int kBarOffset = kTableOffset + 3 * MXB_MAX_GROUPS * 4 + 16;
+    static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;
+    static constexpr int kSmemBytes = 1024 + kBarOffset + kNumBars * 8 + 16;
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+    static_assert(kTmemCols >= 32 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns come in powers of two");
+};
+
+// kind::tf32 with fp32 accumulation, operand majorness as given (1: MN-major).
+__host__ __device__ constexpr uint32_t idesc_tf32_major(int m, int n, int a_mn, int b_mn) {
+    return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+           (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// 32 x 32 outputs per block, one group per blockIdx.z; the row tiles of a
-// group are walked by the blocks of blockIdx.y in turn.
-__global__ void __launch_bounds__(1024) grouped_simple_kernel(const __grid_constant__ GroupedParams p) {
-    __shared__ float left[32][33], right[32][33];
-    const int e = blockIdx.z, tx = threadIdx.x, ty = threadIdx.y;
-    int r0, r1;
-    group_rows(p, e, r0, r1);
-    const int out_rows = p.mode == kGradB ? p.K : r1 - r0;
-    const int out_cols = p.mode == kGradA ? p.K : p.N;
-    const int len = p.mode == kForward ? p.K : p.mode == kGradA ? p.N : r1 - r0;
-    const int c = blockIdx.x * 32 + tx;
-    const float* w = p.w + (p.mode == kGradB ? r0 * p.ldw : e * p.w_stride);
-    for (int i0 = blockIdx.y * 32; i0 < out_rows; i0 += gridDim.y * 32) {
-        const int i = i0 + ty;
-        float acc = 0.0f, colsum = 0.0f;
-        for (int l0 = 0; l0 < len; l0 += 32) {
-            // left[i][l], right[l][c]
-            float a = 0.0f, b = 0.0f;
-            if (p.mode == kGradB) {
-                if (i0 + tx < out_rows && l0 + ty < len) a = __ldg(p.x + (r0 + l0 + ty) * p.ldx + i0 + tx);
-                left[tx][ty] = a;
-                if (c < out_cols && l0 + ty < len) b = __ldg(w + (l0 + ty) * p.ldw + c);
-                right[ty][tx] = b;
-            } else {
-                if (i < out_rows && l0 + tx < len) a = __ldg(p.x + (r0 + i) * p.ldx + l0 + tx);
-                left[ty][tx] = a;
-                if (p.mode == kForward) {
-                    if (c < out_cols && l0 + ty < len) b = __ldg(w + (l0 + ty) * p.ldw + c);
-                    right[ty][tx] = b;
-                } else {
-                    const int cc = blockIdx.x * 32 + ty;
-                    if (cc < out_cols && l0 + tx < len) b = __ldg(w + cc * p.ldw + l0 + tx);
-                    right[tx][ty] = b;
-                }
-            }
-            __syncthreads();
-            for (int l = 0; l < 32; ++l) {
-                acc += left[ty][l] * right[l][tx];
-                colsum += right[l][tx];
-            }
-            __syncthreads();
-        }
-        if (i >= out_rows || c >= out_cols) continue;
-        if (p.mode == kGradB) {
-            p.out[e * p.out_stride + i * p.ldo + c] = acc;
-            if (p.dbias && i == 0) p.dbias[static_cast<long long>(e) * p.N + c] = colsum;
+// The part of x below the upper 19 bits that the tensor core reads, rounded
+// to the nearest TF32 (adding half a step; the tensor core cuts the rest).
+// Non-finite x has none.
+__device__ __forceinline__ float small_of(float x) {
+    const float s = x - __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
+    return s == s ? __uint_as_float(__float_as_uint(s) + 0x1000u) : 0.0f;
+}
+
+// One tile of work.
+struct GroupedTile {
+    int group;
+    int lane0;    // first result column
+    int col0;     // first row of the group (grad_b: of dB) in this tile
+    int cols;     // how many
+    int row0;     // the group's first row
+    int sum;      // length of the sum
+};
+
+struct GroupedTable {
+    int first_tile[MXB_MAX_GROUPS];  // exclusive prefix sums of the groups' tiles
+    int row0[MXB_MAX_GROUPS], row1[MXB_MAX_GROUPS];
+    int total;
+};
+static_assert(sizeof(GroupedTable) <= 3 * MXB_MAX_GROUPS * 4 + 16, "table size");
+
+// Tile t: the last group whose first tile is <= t; inside a group the column
+// tiles vary fastest, so CTAs that run together share weights through L2.
+template <int MODE, int BT>
+__device__ __forceinline__ GroupedTile grouped_tile(const GroupedTable& tab, int t, const GroupedParams& p) {
+    int lo = 0, hi = p.groups - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.first_tile[mid] <= t) {
+            lo = mid;
         } else {
-            p.out[(r0 + i) * p.ldo + c] = apply_cell(acc, r0 + i, c, e, p.epi);
+            hi = mid - 1;
         }
     }
+    GroupedTile g;
+    g.group = lo;
+    g.row0 = tab.row0[lo];
+    const int rows = tab.row1[lo] - g.row0;
+    const int dim = MODE == kGradB ? p.col_dim : rows;
+    const int col_tiles = (dim + BT - 1) / BT;
+    const int i = t - tab.first_tile[lo];
+    g.lane0 = i / col_tiles * 128;
+    g.col0 = i % col_tiles * BT;
+    g.cols = min(BT, dim - g.col0);
+    g.sum = MODE == kGradB ? rows : p.sum_dim;
+    return g;
+}
+
+// Fills the table (one warp): group e's rows are clamped to 0 <= row0 <= row1 <= rows.
+template <int MODE, int BT>
+__device__ __forceinline__ void grouped_scan(GroupedTable& tab, const GroupedParams& p, int lane) {
+    int base = 0;
+    for (int e0 = 0; e0 < p.groups; e0 += 32) {
+        const int e = e0 + lane;
+        int tiles = 0;
+        if (e < p.groups) {
+            const int r0 = min(max(__ldg(p.offsets + e), 0), p.rows);
+            const int r1 = min(max(__ldg(p.offsets + e + 1), r0), p.rows);
+            tab.row0[e] = r0;
+            tab.row1[e] = r1;
+            tiles = ((MODE == kGradB ? p.col_dim : r1 - r0) + BT - 1) / BT * p.lane_tiles;
+        }
+        int sum = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (e < p.groups) tab.first_tile[e] = base + sum - tiles;
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) tab.total = base;
+}
+
+// The steps for W outputs of column `col` (rows row .. row + W - 1, the first `n` of them wanted).
+template <int W>
+__device__ __forceinline__ void apply_column(float (&v)[W], long long row, int n, int col, int group,
+                                             const CellEpilogue& e) {
+    for (int s = 0; s < e.n_steps; ++s) {
+        const EpStepDev& st = e.steps[s];
+        if (st.kind == MXB_EP_RELU) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
+        } else if (st.kind == MXB_EP_SCALE) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = v[i] * st.scale;
+        } else if (st.kind == MXB_EP_ADD_ROW) {
+            const float b = __ldg(st.ptr + group * st.ld_or_size + col);
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] += b;
+        } else {  // ADD_FULL, RELU_GRAD
+            const float* src = st.ptr + row * st.ld_or_size + col;
+            float c[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) c[i] = i < n ? __ldg(src + i * st.ld_or_size) : 0.0f;
+            if (st.kind == MXB_EP_ADD_FULL) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] += c[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] = c[i] > 0.0f ? v[i] : 0.0f;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void raise_grouped(const GroupedParams& p, volatile int* abort_flag, int bit) {
+    atomicOr(p.err, bit);
+    *abort_flag = 1;
+}
+
+constexpr int kGroupedSegKb = 2;  // k-blocks (of 32) to an accumulator
+
+template <int MODE, int BT>
+__global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
+    grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_lane, const __grid_constant__ CUtensorMap tm_col,
+                        const __grid_constant__ GroupedParams p) {
+    using C = GroupedCfg<BT>;
+    constexpr bool kLaneMn = MODE != kGradA, kColMn = MODE == kGradB;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    GroupedTable& tab = *reinterpret_cast<GroupedTable*>(smem + C::kTableOffset);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const uint32_t bar0 = smem_addr(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };                         // TMA -> converter, MMA
+    auto empty_bar = [&](int s) { return bar0 + 8u * (C::kStages + s); };         // MMA -> TMA
+    auto conv_bar = [&](int s) { return bar0 + 8u * (2 * C::kStages + s); };      // converter -> MMA
+    auto sfree_bar = [&](int s) { return bar0 + 8u * (2 * C::kStages + C::kSmall + s); };  // MMA -> converter
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + a); };
+    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 2 + a); };
+    const uint32_t drain_bar = bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kConvWarp = C::kEpiWarps, kTmaWarp = C::kEpiWarps + 4, kMmaWarp = C::kEpiWarps + 5;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int s = 0; s < C::kSmall; ++s) {
+            mbar_init(conv_bar(s), 4);
+            mbar_init(sfree_bar(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), C::kEpiWarps);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tm_lane);
+        tma_prefetch_desc(&tm_col);
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
+        tmem_relinquish();
+    } else if (warp == kConvWarp) {
+        grouped_scan<MODE, BT>(tab, p, lane);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = tab.total;
+
+    if (warp == kTmaWarp) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            long long issued = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
+                const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+                const int col_boxes = (g.cols + 31) / 32;
+                const int num_kb = (g.sum + kBK - 1) / kBK;
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
+                        raise_grouped(p, abort_flag, kErrProducer);
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t st = smem_addr(smem + stage * C::kStageBytes);
+                    const uint32_t fb = full_bar(stage);
+                    mbar_arrive_expect_tx(fb, C::kLaneBytes + col_boxes * kBoxBytes);
+                    const int q0 = kb * kBK;
+                    if (MODE == kForward) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, q0, g.group);
+                    } else if (MODE == kGradA) {
+                        tma_load_3d(st, &tm_lane, fb, q0, g.lane0, g.group);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            tma_load_2d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, g.row0 + q0);
+                    }
+                    for (int j = 0; j < col_boxes; ++j) {
+                        const uint32_t dst = st + C::kLaneBytes + j * kBoxBytes;
+                        if (MODE == kGradB) {
+                            tma_load_2d(dst, &tm_col, fb, g.col0 + 32 * j, g.row0 + q0);
+                        } else {
+                            tma_load_2d(dst, &tm_col, fb, q0, g.row0 + g.col0 + 32 * j);
+                        }
+                    }
+                    ++issued;
+                    if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok) {
+                // Copies in flight land in this CTA's shared memory: wait for them before leaving.
+                const long long n = issued < C::kStages ? issued : C::kStages;
+                for (long long i = 1; i <= n; ++i) {
+                    const long long idx = issued - i;
+                    mbar_wait(full_bar(static_cast<int>(idx % C::kStages)),
+                              static_cast<uint32_t>((idx / C::kStages) & 1), p.timeout_ns);
+                }
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        // ------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            int stage = 0, small = 0, acc = 0;
+            uint32_t phase = 0, small_phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
+                const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+                const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, kLaneMn, kColMn);
+                const int num_kb = (g.sum + kBK - 1) / kBK;
+                for (int k_begin = 0; k_begin < num_kb && ok; k_begin += kGroupedSegKb) {
+                    const int k_end = min(num_kb, k_begin + kGroupedSegKb);
+                    if (*abort_flag || !mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns)) {
+                        raise_grouped(p, abort_flag, kErrMma);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
+                    for (int kb = k_begin; kb < k_end; ++kb) {
+                        if (!mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
+                            !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
+                            raise_grouped(p, abort_flag, kErrMma);
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t big_l = smem_addr(smem + stage * C::kStageBytes);
+                        const uint32_t small_l = smem_addr(smem + C::kSmallOffset + small * C::kStageBytes);
+                        auto lane_desc = [&](uint32_t base, int kk) {
+                            return kLaneMn ? smem_desc(base + kk * 1024, kBoxBytes, 512, kLayoutSW128Base32B)
+                                           : smem_desc(base + kk * 32, 16, 1024, kLayoutSW128);
+                        };
+                        auto col_desc = [&](uint32_t base, int kk) {
+                            return kColMn ? smem_desc(base + kk * 1024, kBoxBytes, 512, kLayoutSW128Base32B)
+                                          : smem_desc(base + kk * 32, 16, 1024, kLayoutSW128);
+                        };
+                        // The last k-block ends with its own eighth: nothing past the sum is multiplied.
+                        const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
+                        for (int kk = 0; kk < steps; ++kk) {
+                            const uint32_t accumulate = kb != k_begin || kk != 0 ? 1u : 0u;
+                            const uint64_t bl = lane_desc(big_l, kk), bc = col_desc(big_l + C::kLaneBytes, kk);
+                            if (p.split3) {
+                                // Small cross terms first, the dominant product last.
+                                mma_tf32(d, bl, col_desc(small_l + C::kLaneBytes, kk), idesc, accumulate);
+                                mma_tf32(d, lane_desc(small_l, kk), bc, idesc, 1u);
+                            }
+                            mma_tf32(d, bl, bc, idesc, p.split3 ? 1u : accumulate);
+                        }
+                        mma_commit(empty_bar(stage));
+                        mma_commit(sfree_bar(small));
+                        if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                        if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+                    }
+                    if (!ok) break;
+                    mma_commit(tfull_bar(acc));
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1u;
+                }
+            }
+            mma_commit(drain_bar);
+            if (!mbar_wait(drain_bar, 0, p.timeout_ns)) raise_grouped(p, abort_flag, kErrMma);
+        }
+    } else if (warp >= kConvWarp) {
+        // ------------------------------------------------------------ converter (4 warps)
+        const int t0 = threadIdx.x - 32 * kConvWarp;
+        int stage = 0, small = 0;
+        uint32_t phase = 0, small_phase = 0;
+        bool failed = false;
+        for (int t = blockIdx.x; t < total_tiles && !failed; t += gridDim.x) {
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            const int col_boxes = (g.cols + 31) / 32;
+            const int num_kb = (g.sum + kBK - 1) / kBK;
+            for (int kb = 0; kb < num_kb; ++kb) {
+                const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
+                const bool got = !stop && mbar_wait(full_bar(stage), phase, p.timeout_ns) &&
+                                 mbar_wait(sfree_bar(small), small_phase ^ 1u, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0 && !stop) raise_grouped(p, abort_flag, kErrProducer);
+                    failed = true;
+                    break;
+                }
+                uint8_t* big = smem + stage * C::kStageBytes;
+                uint8_t* low = smem + C::kSmallOffset + small * C::kStageBytes;
+                const int n4 = 1024 + col_boxes * 256;  // float4s of the tile: lane side, then column boxes
+                // grad_b: the rows behind the group's last belong to others (or to none) and may hold
+                // anything; a row is 128 bytes of every box.
+                const int valid = MODE == kGradB ? min(kBK, g.sum - kb * kBK) : kBK;
+                if (MODE == kGradB && valid < kBK) {
+                    for (int i = t0; i < n4; i += 128)
+                        if (((i >> 3) & 31) >= valid)
+                            reinterpret_cast<float4*>(big)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+                if (p.split3) {
+#pragma unroll 4
+                    for (int i = t0; i < n4; i += 128) {
+                        const float4 v = reinterpret_cast<const float4*>(big)[i];
+                        reinterpret_cast<float4*>(low)[i] =
+                            make_float4(small_of(v.x), small_of(v.y), small_of(v.z), small_of(v.w));
+                    }
+                }
+                fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(conv_bar(small));
+                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue
+        constexpr int W = 16;
+        const int quad = warp & 3;
+        const int first_col = (warp >> 2) * C::kTotals;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + first_col;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool failed = false;
+        for (int t = blockIdx.x; t < total_tiles && !failed; t += gridDim.x) {
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            const int num_kb = (g.sum + kBK - 1) / kBK;
+            float total[C::kTotals];
+#pragma unroll
+            for (int i = 0; i < C::kTotals; ++i) total[i] = 0.0f;
+            for (int k_begin = 0; k_begin < num_kb; k_begin += kGroupedSegKb) {
+                const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
+                const bool got = !stop && mbar_wait(tfull_bar(acc), acc_phase, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0 && !stop) raise_grouped(p, abort_flag, kErrEpilogue);
+                    failed = true;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < C::kTotals; c += W) {
+                    if (first_col + c < g.cols) {
+                        uint32_t r[W];
+                        tmem_ld_32x32b_x16(lane_base + static_cast<uint32_t>(acc * BT + c), r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < W; ++i) total[c + i] += __uint_as_float(r[i]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tempty_bar(acc));
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+            if (failed) break;
+            const int col = g.lane0 + quad * 32 + lane;
+            if (col < p.lane_dim) {
+#pragma unroll
+                for (int c = 0; c < C::kTotals; c += W) {
+                    const int n = min(W, g.cols - first_col - c);
+                    if (n <= 0) continue;
+                    float v[W];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) v[i] = total[c + i];
+                    const long long row = g.col0 + first_col + c + (MODE == kGradB ? 0 : g.row0);
+                    if (MODE != kGradB) apply_column<W>(v, row, n, col, g.group, p.epi);
+                    float* dst = p.out + row * p.ldo + col + (MODE == kGradB ? g.group * p.out_stride : 0);
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+                        if (i < n) __stcs(dst + i * p.ldo, v[i]);
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::kTmemCols);
+    }
+}
+
+// dbias[e, n] = the sum of dY[r, n] over group e's rows: 32 columns of one group to a block.
+__global__ void __launch_bounds__(1024) grouped_column_sums(const float* dy, long long ld, const int* offsets, int rows,
+                                                            int N, float* dbias) {
+    __shared__ float part[32][33];
+    const int e = blockIdx.y, c = blockIdx.x * 32 + threadIdx.x;
+    const int r0 = min(max(__ldg(offsets + e), 0), rows);
+    const int r1 = min(max(__ldg(offsets + e + 1), r0), rows);
+    float s = 0.0f;
+    if (c < N)
+        for (int r = r0 + threadIdx.y; r < r1; r += 32) s += __ldg(dy + r * ld + c);
+    part[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    s = part[threadIdx.x][threadIdx.y];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const int cc = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && cc < N) dbias[static_cast<long long>(e) * N + cc] = s;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int grouped_gemm(const char* fn, GpuCtx* ctx, GroupedParams& p, const mxb_ep_step* steps, int n_steps, int precision,
-                 void* stream) {
-    const bool grad_b = p.mode == kGradB;
-    const int x_cols = p.mode == kGradA ? p.N : p.K, out_cols = p.mode == kGradA ? p.K : p.N;
-    const long long w_cols = p.N;
-    if (!ctx || !p.offsets || p.groups < 1 || p.groups > MXB_MAX_GROUPS || p.rows < 0 || p.N < 1 || p.K < 1 ||
-        p.ldx < x_cols || p.ldw < w_cols || p.ldo < out_cols || n_steps < 0 || n_steps > MXB_MAX_EPILOGUE ||
+// Row-major [groups][rows][cols] (groups 0: a plain [rows][cols]) read in boxes of box_rows x 32 floats,
+// rounded to TF32 by the copy or (3xTF32) as it is.
+bool grouped_map(CUtensorMap* map, const float* base, int groups, long long rows, long long cols, long long ld,
+                 long long stride, int box_rows, bool mn_major, bool round) {
+    const unsigned long long dims[3] = {static_cast<unsigned long long>(cols), static_cast<unsigned long long>(rows),
+                                        static_cast<unsigned long long>(groups)};
+    const unsigned long long strides[2] = {static_cast<unsigned long long>(ld) * 4,
+                                           static_cast<unsigned long long>(groups > 1 ? stride : rows * ld) * 4};
+    const unsigned box[3] = {32, static_cast<unsigned>(box_rows), 1};
+    return encode_tensor_map(map, round ? CU_TENSOR_MAP_DATA_TYPE_TFLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                             groups ? 3 : 2, base, dims, strides, box,
+                             mn_major ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+template <int MODE, int BT>
+cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
+    using C = GroupedCfg<BT>;
+    auto kernel = grouped_gemm_kernel<MODE, BT>;
+    static std::mutex mu;
+    static uint64_t configured = 0;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (dev >= 64 || !(configured & (1ull << dev))) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+            if (e != cudaSuccess) return e;
+            if (dev < 64) configured |= 1ull << dev;
+        }
+    }
+    CUtensorMap lane, col;
+    const bool rnd = !split3;
+    bool ok;
+    if (MODE == kGradB) {
+        ok = grouped_map(&lane, g.w, 0, g.rows, g.N, g.ldw, 0, kBK, true, rnd) &&
+             grouped_map(&col, g.x, 0, g.rows, g.K, g.ldx, 0, kBK, true, rnd);
+    } else {
+        ok = grouped_map(&lane, g.w, g.groups, g.K, g.N, g.ldw, g.w_stride, MODE == kForward ? kBK : 128,
+                         MODE == kForward, rnd) &&
+             grouped_map(&col, g.x, 0, g.rows, MODE == kForward ? g.K : g.N, g.ldx, 0, 32, false, rnd);
+    }
+    if (!ok) return cudaErrorInvalidValue;
+    p.lane_tiles = (p.lane_dim + 127) / 128;
+    // At most so many tiles, whatever the offsets are: a part of a tile more for each group that has a row.
+    const long long dim = MODE == kGradB ? static_cast<long long>((g.K + BT - 1) / BT) * g.groups
+                                         : g.rows / BT + std::min(g.groups, g.rows);
+    const int grid = static_cast<int>(std::min<long long>(dim * p.lane_tiles, num_sms));
+    kernel<<<grid, C::kThreads, C::kSmemBytes, stream>>>(lane, col, p);
+    note_launch();
+    return cudaGetLastError();
+}
+
+template <int MODE>
+cudaError_t run_grouped_mode(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
+    const int per_group = MODE == kGradB ? g.K : (g.rows + g.groups - 1) / g.groups;
+    return per_group <= 32 ? run_grouped<MODE, 32>(g, p, split3, num_sms, stream)
+                           : run_grouped<MODE, 128>(g, p, split3, num_sms, stream);
+}
+
+int grouped_gemm(const char* fn, GpuCtx* ctx, const GroupedCall& g, const mxb_ep_step* steps, int n_steps,
+                 int precision, void* stream) {
+    const bool grad_b = g.mode == kGradB;
+    const int x_cols = g.mode == kGradA ? g.N : g.K, out_cols = g.mode == kGradA ? g.K : g.N;
+    if (!ctx || !g.offsets || g.groups < 1 || g.groups > MXB_MAX_GROUPS || g.rows < 0 || g.N < 1 || g.K < 1 ||
+        g.ldx < x_cols || g.ldw < g.N || g.ldo < out_cols || n_steps < 0 || n_steps > MXB_MAX_EPILOGUE ||
         (n_steps > 0 && !steps) || (precision != GPU_PRECISION_TF32 && precision != GPU_PRECISION_3XTF32) ||
-        ((p.rows > 0 || grad_b) && !p.out) || (p.rows > 0 && (!p.x || !p.w))) {
+        ((g.rows > 0 || grad_b) && !g.out) || (g.rows > 0 && (!g.x || !g.w))) {
         set_error("%s: invalid arguments", fn);
         return MXB_E_ARG;
     }
-    if (p.groups > 1 && ((!grad_b && p.w_stride < (p.K - 1) * p.ldw + p.N) ||
-                         (grad_b && p.out_stride < (p.K - 1) * p.ldo + p.N))) {
+    if (g.groups > 1 && ((!grad_b && g.w_stride < (g.K - 1) * g.ldw + g.N) ||
+                         (grad_b && g.out_stride < (g.K - 1) * g.ldo + g.N))) {
         set_error("%s: the groups' matrices overlap", fn);
         return MXB_E_ARG;
     }
-    if (p.ldx % 4 || p.ldw % 4 || (!grad_b && p.groups > 1 && p.w_stride % 4) || !aligned16(p.x) || !aligned16(p.w)) {
+    if (g.ldx % 4 || g.ldw % 4 || (!grad_b && g.groups > 1 && g.w_stride % 4) || !aligned16(g.x) || !aligned16(g.w)) {
         set_error("%s: the operands need 16-byte aligned bases, pitches and group strides (multiples of 4)", fn);
         return MXB_E_ARG;
     }
+    GroupedParams p{};
     if (!take_cell_steps(fn, steps, n_steps, out_cols, true, p.epi)) return MXB_E_ARG;
-    if (p.rows == 0 && !grad_b) return MXB_OK;
+    if (g.rows == 0 && !grad_b) return MXB_OK;
+    p.offsets = g.offsets;
+    p.groups = g.groups;
+    p.rows = g.rows;
+    p.out = g.out;
+    p.ldo = g.ldo;
+    p.out_stride = g.out_stride;
+    p.lane_dim = out_cols;
+    p.col_dim = g.K;
+    p.sum_dim = x_cols;
+    p.split3 = precision == GPU_PRECISION_3XTF32;
+    p.timeout_ns = ctx->timeout_ns;
+    p.err = ctx->d_err;
     DeviceScope scope(ctx->device);
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-    const int tiles = ((grad_b ? p.K : p.rows) + 31) / 32;
-    grouped_simple_kernel<<<dim3((out_cols + 31) / 32, std::min(tiles, 64), p.groups), dim3(32, 32), 0, st>>>(p);
-    note_launch();
-    return cuda_ok(cudaGetLastError(), "grouped product launch") ? MXB_OK : MXB_E_CUDA;
+    if (g.rows == 0) {  // grad_b without a row: every gradient is zero
+        for (int e = 0; e < g.groups; ++e)
+            if (!cuda_ok(cudaMemset2DAsync(g.out + e * g.out_stride, g.ldo * 4, 0, static_cast<size_t>(g.N) * 4, g.K, st),
+                         "gradient clear"))
+                return MXB_E_CUDA;
+        if (g.dbias && !cuda_ok(cudaMemsetAsync(g.dbias, 0, static_cast<size_t>(g.groups) * g.N * 4, st), "gradient clear"))
+            return MXB_E_CUDA;
+        return MXB_OK;
+    }
+    const cudaError_t e = g.mode == kForward ? run_grouped_mode<kForward>(g, p, p.split3, ctx->num_sms, st)
+                          : g.mode == kGradA ? run_grouped_mode<kGradA>(g, p, p.split3, ctx->num_sms, st)
+                                             : run_grouped_mode<kGradB>(g, p, p.split3, ctx->num_sms, st);
+    if (!cuda_ok(e, "grouped product launch")) return MXB_E_CUDA;
+    if (g.dbias) {
+        grouped_column_sums<<<dim3((g.N + 31) / 32, g.groups), dim3(32, 32), 0, st>>>(g.w, g.ldw, g.offsets, g.rows, g.N,
+                                                                                     g.dbias);
+        note_launch();
+        if (!cuda_ok(cudaGetLastError(), "bias gradient launch")) return MXB_E_CUDA;
+    }
+    return MXB_OK;
 }
 
 }  // namespace
@@ -131,22 +653,37 @@ extern "C" {
 int mxb_grouped_gemm(GpuCtx* ctx, const float* A, long long lda, const float* B, long long ldb, long long b_stride,
                      const int* offsets, int groups, float* out, long long ldo, int rows, int N, int K,
                      const mxb_ep_step* steps, int n_steps, int precision, void* stream) {
-    mxb::GroupedParams p{mxb::kForward, A, lda, B, ldb, b_stride, offsets, groups, rows, out, ldo, 0, nullptr, N, K, {}};
-    return mxb::grouped_gemm("mxb_grouped_gemm", ctx, p, steps, n_steps, precision, stream);
+    try {
+        const mxb::GroupedCall g{mxb::kForward, A, lda, B, ldb, b_stride, offsets, groups, rows, out, ldo, 0, nullptr, N, K};
+        return mxb::grouped_gemm("mxb_grouped_gemm", ctx, g, steps, n_steps, precision, stream);
+    } catch (const std::exception& e) {  // host allocations of the tensor-map cache
+        mxb::set_error("mxb_grouped_gemm: %s", e.what());
+        return MXB_E_NOMEM;
+    }
 }
 
 int mxb_grouped_gemm_grad_a(GpuCtx* ctx, const float* dY, long long lddy, const float* B, long long ldb,
                             long long b_stride, const int* offsets, int groups, float* dA, long long ldda, int rows,
                             int N, int K, const mxb_ep_step* steps, int n_steps, int precision, void* stream) {
-    mxb::GroupedParams p{mxb::kGradA, dY, lddy, B, ldb, b_stride, offsets, groups, rows, dA, ldda, 0, nullptr, N, K, {}};
-    return mxb::grouped_gemm("mxb_grouped_gemm_grad_a", ctx, p, steps, n_steps, precision, stream);
+    try {
+        const mxb::GroupedCall g{mxb::kGradA, dY, lddy, B, ldb, b_stride, offsets, groups, rows, dA, ldda, 0, nullptr, N, K};
+        return mxb::grouped_gemm("mxb_grouped_gemm_grad_a", ctx, g, steps, n_steps, precision, stream);
+    } catch (const std::exception& e) {
+        mxb::set_error("mxb_grouped_gemm_grad_a: %s", e.what());
+        return MXB_E_NOMEM;
+    }
 }
 
 int mxb_grouped_gemm_grad_b(GpuCtx* ctx, const float* A, long long lda, const float* dY, long long lddy,
                             const int* offsets, int groups, float* dB, long long lddb, long long db_stride,
                             float* dbias, int rows, int N, int K, int precision, void* stream) {
-    mxb::GroupedParams p{mxb::kGradB, A, lda, dY, lddy, 0, offsets, groups, rows, dB, lddb, db_stride, dbias, N, K, {}};
-    return mxb::grouped_gemm("mxb_grouped_gemm_grad_b", ctx, p, nullptr, 0, precision, stream);
+    try {
+        const mxb::GroupedCall g{mxb::kGradB, A, lda, dY, lddy, 0, offsets, groups, rows, dB, lddb, db_stride, dbias, N, K};
+        return mxb::grouped_gemm("mxb_grouped_gemm_grad_b", ctx, g, nullptr, 0, precision, stream);
+    } catch (const std::exception& e) {
+        mxb::set_error("mxb_grouped_gemm_grad_b: %s", e.what());
+        return MXB_E_NOMEM;
+    }
 }
 
 }  // extern "C"
