@@ -1,5 +1,7 @@
 // Products with 4-bit weights and group scales (mxb_q4_gemm):
 //   out[m, n] = epi(sum over groups g of s[n, g] * sum over k in g of A[m, k] * (q[n, k] - z[n, g])).
+#include "gemm_common.cuh"
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -27,15 +29,10 @@ struct Q4Params {
     float* out;
     long long ldo;
     int M, N, K;
+    unsigned long long timeout_ns;
+    int* err;
     CellEpilogue epi;
 };
-
-__device__ __forceinline__ float load_scale(const Q4Params& p, long long at) {
-    if (p.scale_type == MXB_SCALE_F32) return __ldg(static_cast<const float*>(p.scales) + at);
-    const unsigned short raw = __ldg(static_cast<const unsigned short*>(p.scales) + at);
-    return p.scale_type == MXB_SCALE_F16 ? __half2float(__ushort_as_half(raw))
-                                         : __bfloat162float(__ushort_as_bfloat16(raw));
-}
 
 // ---------------------------------------------------------------- few rows
 //
@@ -55,19 +52,12 @@ __device__ __forceinline__ float load_scale(const Q4Params& p, long long at) {
 //        (column 3 m + part), one MMA instead of three.
 //  RT:   row tiles of eight; their three parts go through three MMAs into
 //        the same accumulators.
-// Weights and activations come through a ring of cp.async units per warp.
+// Each warp has a ring of its own: one lane asks TMA for the next run's
+// weights and activations (zeros past their edges), so that no instruction
+// is spent on addresses and bounds.
 
 constexpr int kFewWarps = 8;
 constexpr int kRun = 128;  // k of one unit
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -79,10 +69,11 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 
 // Two q - z as a bf16 pair, from nibbles 0 and 4 of `w` and the pair (128 + z, 128 + z):
 // 0x4300 | q is the bf16 number 128 + q, and the difference is exact.
-__device__ __forceinline__ uint32_t weight_pair(uint32_t w, __nv_bfloat162 z128) {
+__device__ __forceinline__ uint32_t weight_pair(uint32_t w, uint32_t z128) {
     uint32_t v = (w & 0x000F000Fu) | 0x43004300u;
-    __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), z128);
-    return *reinterpret_cast<uint32_t*>(&h);
+    const __nv_bfloat162 h =
+        __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&z128));
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // The top eight bits of x and y as a bf16 pair; x and y keep the rest.
@@ -96,83 +87,106 @@ __device__ __forceinline__ uint32_t cut_pair(float& x, float& y) {
 template <bool PACK, int RT, int MT>
 struct FewCfg {
     static constexpr int kRows = PACK ? 2 : 8 * RT;
-    static constexpr int kUnit = MT * 1024 + kRows * kRun * 4;
-    static constexpr int kDepth = kUnit * kFewWarps * 4 <= 100 * 1024 ? 4 : kUnit * kFewWarps * 3 <= 110 * 1024 ? 3 : 2;
+    static constexpr int kPieceRows = PACK ? 2 : 8 * RT;            // rows of an activation box (32 k, 128 bytes)
+    static constexpr int kWeightBytes = MT * 1024;
+    static constexpr int kPieceBytes = kPieceRows * 128;
+    static constexpr int kUnit = kWeightBytes + 4 * kPieceBytes;    // a multiple of 1 KiB
+    // As many units as fit in half the shared memory (two CTAs), or in all of it.
+    static constexpr int kHalf = 104 * 1024 / (kUnit * kFewWarps), kAll = 214 * 1024 / (kUnit * kFewWarps);
+    static constexpr int kDepth = kHalf >= 2 ? (kHalf > 4 ? 4 : kHalf) : (kAll > 4 ? 4 : kAll);
     static constexpr int kRing = kUnit * kFewWarps * kDepth;
+    static constexpr int kScaleBytes = 16 * MT * 4 * 8;             // per warp: (scale, zero pair) [row][piece]
+    static constexpr int kScaleOffset = kRing;
+    static constexpr int kBarOffset = kScaleOffset + kFewWarps * kScaleBytes;
     static constexpr int kReduce = kFewWarps * 16 * MT * (8 * RT) * 4;
-    static constexpr int kSmem = kRing > kReduce ? kRing : kReduce;
+    static constexpr int kSmem = 1024 + kBarOffset + kFewWarps * kDepth * 8 + 16;
+    static_assert(kUnit % 1024 == 0 && kDepth >= 2 && kReduce <= kRing && kSmem <= 227 * 1024, "shared memory layout");
 };
 
 template <bool PACK, int RT, int MT>
 __global__ void __launch_bounds__(32 * kFewWarps)
-    q4_few_rows_kernel(const __grid_constant__ Q4Params p) {
+    q4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
+                       const __grid_constant__ Q4Params p) {
     using C = FewCfg<PACK, RT, MT>;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * 16 * MT, m0 = blockIdx.y * C::kRows;
     const int rows = min(C::kRows, p.M - m0);
     const int runs = (p.K + kRun - 1) / kRun;
     uint8_t* ring = smem + warp * C::kDepth * C::kUnit;
+    uint2* scales = reinterpret_cast<uint2*>(smem + C::kScaleOffset + warp * C::kScaleBytes);
+    const uint32_t bar0 = smem_addr(smem + C::kBarOffset) + warp * C::kDepth * 8;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOffset + kFewWarps * C::kDepth * 8);
+    if (lane == 0) {
+        for (int d = 0; d < C::kDepth; ++d) mbar_init(bar0 + 8 * d, 1);
+        fence_barrier_init();
+    }
+    if (threadIdx.x == 0) *abort_flag = 0;
+    __syncthreads();
 
-    // Unit of run r into slot `slot`.  Weights: row i at 64 i, its 16-byte
-    // chunk s (32 k) at position s ^ ((i >> 1) & 3); activations: row m at
-    // 512 m, chunk c at c ^ (m & 1): both conflict-free for the reads below.
+    // Unit of run r into slot `slot`.  Weights: row i's 64 bytes at 64 i, 16-byte chunk s (32 k) at
+    // s ^ ((i >> 1) & 3); activations: a box for each 32 k, row m's 128 bytes at 128 m, chunk c at
+    // c ^ (bits 7..9 of the row's address): the copies' 64- and 128-byte swizzles, conflict-free below.
     auto issue = [&](int r, int slot) {
-        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(ring + slot * C::kUnit));
-        const int k0 = r * kRun;
+        const uint32_t dst = smem_addr(ring + slot * C::kUnit), bar = bar0 + 8 * slot;
+        mbar_arrive_expect_tx(bar, C::kUnit);
+        tma_load_2d(dst, &tm_w, bar, r * (kRun / 2), n0);
 #pragma unroll
-        for (int j = 0; j < 2 * MT; ++j) {
-            const int i = j * 8 + g;
-            const bool in = n0 + i < p.N && k0 / 2 + 16 * t < p.ldq;
-            cp_async16(dst + i * 64 + ((t ^ ((i >> 1) & 3)) << 4),
-                       in ? p.q + (n0 + i) * p.ldq + k0 / 2 + 16 * t : p.q, in ? 16 : 0);
-        }
-        for (int m = 0; m < rows; ++m) {
-            const int left = min(max(p.K - k0 - 4 * lane, 0), 4);
-            cp_async16(dst + MT * 1024 + m * 512 + ((lane ^ (m & 1)) << 4),
-                       left ? p.a + (m0 + m) * p.lda + k0 + 4 * lane : p.a, 4 * left);
-        }
+        for (int c = 0; c < 4; ++c)
+            tma_load_2d(dst + C::kWeightBytes + c * C::kPieceBytes, &tm_a, bar, r * kRun + 32 * c, m0);
     };
-    const bool whole = p.group % kRun == 0;  // one group to a run
-    // Lane t keeps the scale and zero point of 32-value piece t of a run (of the whole run), for its 2 MT weight rows.
-    auto load_group = [&](int r, float (&s)[2 * MT], uint32_t (&z)[2 * MT]) {
-        const int k = r * kRun + (whole ? 0 : 32 * t);
+    // Lane t loads the scale and zero point of 32-value piece t of a run, for its 2 MT weight rows,
+    // a run ahead and unconverted, so that nothing waits for them here.
+    uint32_t s_raw[2 * MT], z_raw[2 * MT];
+    auto load_group = [&](int r) {
+        const int k = r * kRun + 32 * t;
+        const long long at = static_cast<long long>(n0 + g) * p.lds + k / p.group;
 #pragma unroll
         for (int j = 0; j < 2 * MT; ++j) {
-            const int n = n0 + j * 8 + g;
-            const bool in = n < p.N && k < p.K;
-            const long long at = n * p.lds + k / p.group;
-            s[j] = in ? load_scale(p, at) : 0.0f;
-            z[j] = in && p.zeros ? __ldg(p.zeros + at) & 15u : 8u;
+            const bool in = n0 + j * 8 + g < p.N && k < p.K;
+            const long long i = at + j * 8 * p.lds;
+            s_raw[j] = 0;
+            z_raw[j] = 8;
+            if (in) {
+                s_raw[j] = p.scale_type == MXB_SCALE_F32 ? __ldg(static_cast<const uint32_t*>(p.scales) + i)
+                                                         : __ldg(static_cast<const unsigned short*>(p.scales) + i);
+                if (p.zeros) z_raw[j] = __ldg(p.zeros + i);
+            }
         }
     };
 
     // This lane's activation row (PACK: row and part) of the MMA's column g.
     const int part = PACK ? g % 3 : 0;
     float tot[MT][RT][4] = {};
-    float s_next[2 * MT];
-    uint32_t z_next[2 * MT];
     int r = warp;
-    if (r < runs) load_group(r, s_next, z_next);
+    if (lane == 0) {
 #pragma unroll
-    for (int d = 0; d < C::kDepth - 1; ++d) {
-        if (r + d * kFewWarps < runs) issue(r + d * kFewWarps, d);
-        cp_async_commit();
+        for (int d = 0; d < C::kDepth - 1; ++d)
+            if (r + d * kFewWarps < runs) issue(r + d * kFewWarps, d);
     }
+    if (r < runs) load_group(r);
+    const bool whole = p.group % kRun == 0;  // one group to a run
+    uint32_t phase = 0;
+    bool failed = false;
     for (int slot = 0; r < runs; r += kFewWarps) {
-        float s[2 * MT];
-        uint32_t z[2 * MT];
+        __syncwarp();  // the unit and the scales before these are read by every lane
 #pragma unroll
         for (int j = 0; j < 2 * MT; ++j) {
-            s[j] = s_next[j];
-            z[j] = z_next[j];
+            const uint32_t raw = s_raw[j], z = z_raw[j] & 15u;
+            const uint32_t s = p.scale_type == MXB_SCALE_F32   ? raw
+                               : p.scale_type == MXB_SCALE_F16 ? __float_as_uint(__half2float(
+                                                                     __ushort_as_half(static_cast<unsigned short>(raw))))
+                                                               : raw << 16;
+            scales[(j * 8 + g) * 4 + t] = make_uint2(s, 0x43004300u | z | (z << 16));
         }
-        if (r + kFewWarps < runs) load_group(r + kFewWarps, s_next, z_next);
-        cp_async_wait<C::kDepth - 2>();
-        __syncwarp();  // the unit is here for every lane, and the one before it is read by all
+        if (r + kFewWarps < runs) load_group(r + kFewWarps);
         const int ahead = r + (C::kDepth - 1) * kFewWarps;
-        if (ahead < runs) issue(ahead, slot == 0 ? C::kDepth - 1 : slot - 1);
-        cp_async_commit();
+        if (lane == 0 && ahead < runs) issue(ahead, slot == 0 ? C::kDepth - 1 : slot - 1);
+        if (!mbar_wait(bar0 + 8 * slot, phase, p.timeout_ns)) failed = true;
+        failed = __any_sync(0xffffffffu, failed);  // (also makes the scales visible)
+        if (failed) break;
         const uint8_t* unit = ring + slot * C::kUnit;
         float acc[MT][RT][4] = {};
 #pragma unroll
@@ -182,8 +196,10 @@ __global__ void __launch_bounds__(32 * kFewWarps)
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 const int m = PACK ? (g < 6 ? g / 3 : 0) : rt * 8 + g;
-                const float4* x = reinterpret_cast<const float4*>(unit + MT * 1024 + m * 512);
-                float4 lo = x[(c * 8 + 2 * t) ^ (m & 1)], hi = x[(c * 8 + 2 * t + 1) ^ (m & 1)];
+                const uint8_t* x = unit + C::kWeightBytes + c * C::kPieceBytes + m * 128;
+                const int swizzle = (smem_addr(x) >> 7) & 7;
+                float4 lo = *reinterpret_cast<const float4*>(x + (((2 * t) ^ swizzle) << 4));
+                float4 hi = *reinterpret_cast<const float4*>(x + (((2 * t + 1) ^ swizzle) << 4));
                 float u[4] = {lo.x, lo.y, lo.z, lo.w}, v[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -200,25 +216,18 @@ __global__ void __launch_bounds__(32 * kFewWarps)
             }
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                uint32_t w[2], zz[2];
-                float sc[2];
+                uint32_t w[2];
+                uint2 sz[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int i = mt * 16 + h * 8 + g, j = 2 * mt + h;
+                    const int i = mt * 16 + h * 8 + g;
                     w[h] = *reinterpret_cast<const uint32_t*>(unit + i * 64 + ((c ^ ((i >> 1) & 3)) << 4) + 4 * t);
-                    zz[h] = __shfl_sync(0xffffffffu, z[j], (lane & ~3) | c);
-                    sc[h] = __shfl_sync(0xffffffffu, s[j], (lane & ~3) | c);
+                    sz[h] = scales[i * 4 + (whole ? 0 : c)];
                 }
-                __nv_bfloat162 z128[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t pair = 0x43004300u | zz[h] | (zz[h] << 16);
-                    z128[h] = *reinterpret_cast<const __nv_bfloat162*>(&pair);
-                }
-                const uint32_t a1[4] = {weight_pair(w[0], z128[0]), weight_pair(w[1], z128[1]),
-                                        weight_pair(w[0] >> 4, z128[0]), weight_pair(w[1] >> 4, z128[1])};
-                const uint32_t a2[4] = {weight_pair(w[0] >> 8, z128[0]), weight_pair(w[1] >> 8, z128[1]),
-                                        weight_pair(w[0] >> 12, z128[0]), weight_pair(w[1] >> 12, z128[1])};
+                const uint32_t a1[4] = {weight_pair(w[0], sz[0].y), weight_pair(w[1], sz[1].y),
+                                        weight_pair(w[0] >> 4, sz[0].y), weight_pair(w[1] >> 4, sz[1].y)};
+                const uint32_t a2[4] = {weight_pair(w[0] >> 8, sz[0].y), weight_pair(w[1] >> 8, sz[1].y),
+                                        weight_pair(w[0] >> 12, sz[0].y), weight_pair(w[1] >> 12, sz[1].y)};
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -229,17 +238,26 @@ __global__ void __launch_bounds__(32 * kFewWarps)
                     if (!whole || c == 3) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            tot[mt][rt][i] += sc[i >> 1] * acc[mt][rt][i];
+                            tot[mt][rt][i] += __uint_as_float(sz[i >> 1].x) * acc[mt][rt][i];
                             acc[mt][rt][i] = 0.0f;
                         }
                     }
                 }
             }
         }
-        if (++slot == C::kDepth) slot = 0;
+        if (++slot == C::kDepth) { slot = 0; phase ^= 1u; }
     }
-    cp_async_wait<0>();
+    if (failed && lane == 0) {
+        // Record it, and wait (again with a limit) for the copies still on their way to this CTA.
+        atomicOr(p.err, kErrProducer);
+        *abort_flag = 1;
+        for (int d = 0; d < C::kDepth; ++d) {
+            mbar_wait(bar0 + 8 * d, 0, p.timeout_ns);
+            mbar_wait(bar0 + 8 * d, 1, p.timeout_ns);
+        }
+    }
     __syncthreads();  // every warp is done with the ring
+    if (*abort_flag) return;
     // The warps' sums: [warp][MMA column][weight column], added in warp order (PACK: small parts first).
     float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
@@ -280,7 +298,20 @@ cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
             if (dev < 64) configured |= 1ull << dev;
         }
     }
-    kernel<<<dim3((p.N + 16 * MT - 1) / (16 * MT), (p.M + C::kRows - 1) / C::kRows), 32 * kFewWarps, C::kSmem, stream>>>(p);
+    CUtensorMap mw, ma;
+    const unsigned long long w_dims[2] = {static_cast<unsigned long long>(p.ldq), static_cast<unsigned long long>(p.N)};
+    const unsigned long long w_stride[1] = {static_cast<unsigned long long>(p.ldq)};
+    const unsigned w_box[2] = {kRun / 2, 16 * MT};
+    const unsigned long long a_dims[2] = {static_cast<unsigned long long>(p.K), static_cast<unsigned long long>(p.M)};
+    const unsigned long long a_stride[1] = {static_cast<unsigned long long>(p.lda) * 4};
+    const unsigned a_box[2] = {32, C::kPieceRows};
+    if (!encode_tensor_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p.q, w_dims, w_stride, w_box,
+                           CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
+        !encode_tensor_map(&ma, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, p.a, a_dims, a_stride, a_box,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
+        return cudaErrorInvalidValue;
+    kernel<<<dim3((p.N + 16 * MT - 1) / (16 * MT), (p.M + C::kRows - 1) / C::kRows), 32 * kFewWarps, C::kSmem, stream>>>(
+        mw, ma, p);
     note_launch();
     return cudaGetLastError();
 }
@@ -288,6 +319,12 @@ cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
 template <bool PACK, int RT>
 cudaError_t run_few_rows_width(const Q4Params& p, int num_sms, cudaStream_t stream) {
     // Wider warp tiles cut each activation for more weights; narrow ones fill the SMs.
+    static const char* force = getenv("Q4_MT");
+    if (force) {
+        if (force[0] == '4') return run_few_rows<PACK, RT, PACK ? 2 : 4>(p, stream);
+        if (force[0] == '2') return run_few_rows<PACK, RT, 2>(p, stream);
+        return run_few_rows<PACK, RT, 1>(p, stream);
+    }
     if (p.N >= 64 * num_sms && !PACK) return run_few_rows<PACK, RT, PACK ? 2 : 4>(p, stream);
     return p.N >= 32 * num_sms ? run_few_rows<PACK, RT, 2>(p, stream) : run_few_rows<PACK, RT, 1>(p, stream);
 }
@@ -312,6 +349,8 @@ int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, voi
     if (!take_cell_steps("mxb_q4_gemm", steps, n_steps, p.N, false, p.epi)) return MXB_E_ARG;
     DeviceScope scope(ctx->device);
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+    p.timeout_ns = ctx->timeout_ns;
+    p.err = ctx->d_err;
     const cudaError_t e = p.M <= 2   ? run_few_rows_width<true, 1>(p, ctx->num_sms, st)
                           : p.M <= 8 ? run_few_rows_width<false, 1>(p, ctx->num_sms, st)
                                      : run_few_rows_width<false, 2>(p, ctx->num_sms, st);
@@ -326,7 +365,7 @@ extern "C" int mxb_q4_gemm(GpuCtx* ctx, const float* A, long long lda, const uns
                            float* out, long long ldo, int M, int N, int K, const mxb_ep_step* steps, int n_steps,
                            void* stream) {
     try {
-        mxb::Q4Params p{A, lda, Q, ldq, scales, zeros, lds, scale_type, group, out, ldo, M, N, K, {}};
+        mxb::Q4Params p{A, lda, Q, ldq, scales, zeros, lds, scale_type, group, out, ldo, M, N, K, 0, nullptr, {}};
         return mxb::q4_gemm(ctx, p, steps, n_steps, stream);
     } catch (const std::exception& e) {  // host allocations of the pool's lists
         mxb::set_error("mxb_q4_gemm: %s", e.what());
