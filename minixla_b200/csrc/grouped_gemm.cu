@@ -223,8 +223,8 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
     using C = GroupedCfg<BT>;
     constexpr bool kLaneMn = MODE != kGradA, kColMn = MODE == kGradB;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                               ~static_cast<uintptr_t>(1023));
+    // (an offset, not a rounded pointer: the compiler then still knows that these are shared addresses)
+    uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     GroupedTable& tab = *reinterpret_cast<GroupedTable*>(smem + C::kTableOffset);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);

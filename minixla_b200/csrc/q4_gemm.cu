@@ -40,14 +40,13 @@ struct Q4Params {
 // fp32 accumulate) takes 16 weight columns as its rows and activations as
 // its eight columns.  q - z is exact in bf16; an activation is cut into three
 // bf16 parts of eight bits each whose sum is exact, so nothing is rounded
-// before the fp32 sums.  A warp takes every eighth run of 128 k for
+// before the fp32 sums.  A warp takes every eighth run of k for
 // 16 * MT weight columns; lane (g, t) of the warp holds, for each 32 k, the
 // eight values of word t of weight rows g and g + 8 -- the k order inside an
 // MMA is free as long as weights and activations agree on it, so the words
 // are used as they lie -- and the same eight k of activation row g, which it
 // cuts itself.  All 16 k of an MMA lie in one group; the sums of a group (of
-// the whole run, where the group is a multiple of 128) start from zero and
-// are scaled in fp32.
+// at most a run of it) start from zero and are scaled in fp32.
 //  PACK: one or two rows; the eight MMA columns hold the parts side by side
 //        (column 3 m + part), one MMA instead of three.
 //  RT:   row tiles of eight; their three parts go through three MMAs into
@@ -57,7 +56,6 @@ struct Q4Params {
 // is spent on addresses and bounds.
 
 constexpr int kFewWarps = 8;
-constexpr int kRun = 128;  // k of one unit
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -87,17 +85,22 @@ __device__ __forceinline__ uint32_t cut_pair(float& x, float& y) {
 template <bool PACK, int RT, int MT>
 struct FewCfg {
     static constexpr int kRows = PACK ? 2 : 8 * RT;
-    static constexpr int kPieceRows = PACK ? 2 : 8 * RT;            // rows of an activation box (32 k, 128 bytes)
-    static constexpr int kWeightBytes = MT * 1024;
-    static constexpr int kPieceBytes = kPieceRows * 128;
-    static constexpr int kUnit = kWeightBytes + 4 * kPieceBytes;    // a multiple of 1 KiB
+    // k of one unit: 128 bytes of a weight row, or 64 where eight or more rows of activations come with them.
+    static constexpr int kRun = PACK ? 256 : 128;
+    static constexpr int kPieces = kRun / 32;                       // of 32 k
+    static constexpr int kWeightBytes = 16 * MT * kRun / 2;
+    static constexpr int kPieceBytes = kRows * 128;                 // an activation box: 32 k of each row
+    static constexpr int kUnit = kWeightBytes + kPieces * kPieceBytes;  // a multiple of 1 KiB
+    static constexpr int kScaleBytes = 16 * MT * kPieces * 8;       // per warp: (scale, zero pair) [row][piece]
+    static constexpr int kPartBytes = PACK ? kPieces * 6 * 4 * 16 : 0;  // per warp: [piece][MMA column][lane t]
+    static constexpr int kWarpExtra = kScaleBytes + kPartBytes;
     // As many units as fit in half the shared memory (two CTAs), or in all of it.
-    static constexpr int kHalf = 104 * 1024 / (kUnit * kFewWarps), kAll = 214 * 1024 / (kUnit * kFewWarps);
+    static constexpr int kHalf = (108 * 1024 / kFewWarps - kWarpExtra) / kUnit;
+    static constexpr int kAll = (220 * 1024 / kFewWarps - kWarpExtra) / kUnit;
     static constexpr int kDepth = kHalf >= 2 ? (kHalf > 4 ? 4 : kHalf) : (kAll > 4 ? 4 : kAll);
     static constexpr int kRing = kUnit * kFewWarps * kDepth;
-    static constexpr int kScaleBytes = 16 * MT * 4 * 8;             // per warp: (scale, zero pair) [row][piece]
-    static constexpr int kScaleOffset = kRing;
-    static constexpr int kBarOffset = kScaleOffset + kFewWarps * kScaleBytes;
+    static constexpr int kExtraOffset = kRing;
+    static constexpr int kBarOffset = kExtraOffset + kFewWarps * kWarpExtra;
     static constexpr int kReduce = kFewWarps * 16 * MT * (8 * RT) * 4;
     static constexpr int kSmem = 1024 + kBarOffset + kFewWarps * kDepth * 8 + 16;
     static_assert(kUnit % 1024 == 0 && kDepth >= 2 && kReduce <= kRing && kSmem <= 227 * 1024, "shared memory layout");
@@ -108,15 +111,16 @@ __global__ void __launch_bounds__(32 * kFewWarps)
     q4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
                        const __grid_constant__ Q4Params p) {
     using C = FewCfg<PACK, RT, MT>;
+    constexpr int kRun = C::kRun, kPieces = C::kPieces;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                               ~static_cast<uintptr_t>(1023));
+    // (an offset, not a rounded pointer: the compiler then still knows that these are shared addresses)
+    uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * 16 * MT, m0 = blockIdx.y * C::kRows;
     const int rows = min(C::kRows, p.M - m0);
     const int runs = (p.K + kRun - 1) / kRun;
     uint8_t* ring = smem + warp * C::kDepth * C::kUnit;
-    uint2* scales = reinterpret_cast<uint2*>(smem + C::kScaleOffset + warp * C::kScaleBytes);
+    uint8_t* extra = smem + C::kExtraOffset + warp * C::kWarpExtra;
     const uint32_t bar0 = smem_addr(smem + C::kBarOffset) + warp * C::kDepth * 8;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOffset + kFewWarps * C::kDepth * 8);
     if (lane == 0) {
@@ -126,39 +130,61 @@ __global__ void __launch_bounds__(32 * kFewWarps)
     if (threadIdx.x == 0) *abort_flag = 0;
     __syncthreads();
 
-    // Unit of run r into slot `slot`.  Weights: row i's 64 bytes at 64 i, 16-byte chunk s (32 k) at
-    // s ^ ((i >> 1) & 3); activations: a box for each 32 k, row m's 128 bytes at 128 m, chunk c at
-    // c ^ (bits 7..9 of the row's address): the copies' 64- and 128-byte swizzles, conflict-free below.
+    // Unit of run r into slot `slot`.  Weights: row i's 16-byte chunk c (piece c, 32 k) at c ^ (i & 7), or at
+    // c ^ ((i >> 1) & 3) in a row of 64 bytes; activations: a box for each piece, row m's 128 bytes at 128 m,
+    // chunk c at c ^ (bits 7..9 of the row's address): the copies' swizzles, conflict-free for the reads below.
     auto issue = [&](int r, int slot) {
         const uint32_t dst = smem_addr(ring + slot * C::kUnit), bar = bar0 + 8 * slot;
         mbar_arrive_expect_tx(bar, C::kUnit);
         tma_load_2d(dst, &tm_w, bar, r * (kRun / 2), n0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < kPieces; ++c)
             tma_load_2d(dst + C::kWeightBytes + c * C::kPieceBytes, &tm_a, bar, r * kRun + 32 * c, m0);
     };
-    // Lane t loads the scale and zero point of 32-value piece t of a run, for its 2 MT weight rows,
-    // a run ahead and unconverted, so that nothing waits for them here.
-    uint32_t s_raw[2 * MT], z_raw[2 * MT];
+    // Pieces between two scalings: all of a run's, or the largest power of two of them that divides a group.
+    const int span = p.group % 256 == 0 && kPieces == 8 ? 8 : p.group % 128 == 0 ? 4 : p.group % 64 == 0 ? 2 : 1;
+    // Lane t loads the scales and zero points of its kOwn pieces of a run for its 2 MT weight rows, a run
+    // ahead and unconverted, so that nothing waits for them here.  One load serves two pieces unless a
+    // group ends between them.
+    constexpr int kOwn = kPieces / 4;
+    uint32_t s_raw[kOwn][2 * MT], z_raw[kOwn][2 * MT];
     auto load_group = [&](int r) {
-        const int k = r * kRun + 32 * t;
-        const long long at = static_cast<long long>(n0 + g) * p.lds + k / p.group;
 #pragma unroll
-        for (int j = 0; j < 2 * MT; ++j) {
-            const bool in = n0 + j * 8 + g < p.N && k < p.K;
-            const long long i = at + j * 8 * p.lds;
-            s_raw[j] = 0;
-            z_raw[j] = 8;
-            if (in) {
-                s_raw[j] = p.scale_type == MXB_SCALE_F32 ? __ldg(static_cast<const uint32_t*>(p.scales) + i)
-                                                         : __ldg(static_cast<const unsigned short*>(p.scales) + i);
-                if (p.zeros) z_raw[j] = __ldg(p.zeros + i);
+        for (int h = 0; h < kOwn; ++h) {
+            if (h == 1 && span > 1) break;
+            // (the span's first piece: its last may lie behind K)
+            const int k = r * kRun + 32 * ((kOwn * t + h) & ~(span - 1));
+            const long long at = static_cast<long long>(n0 + g) * p.lds + k / p.group;
+#pragma unroll
+            for (int j = 0; j < 2 * MT; ++j) {
+                const bool in = n0 + j * 8 + g < p.N && k < p.K;
+                const long long i = at + j * 8 * p.lds;
+                s_raw[h][j] = 0;
+                z_raw[h][j] = 8;
+                if (in) {
+                    s_raw[h][j] = p.scale_type == MXB_SCALE_F32 ? __ldg(static_cast<const uint32_t*>(p.scales) + i)
+                                                                : __ldg(static_cast<const unsigned short*>(p.scales) + i);
+                    if (p.zeros) z_raw[h][j] = __ldg(p.zeros + i);
+                }
             }
         }
     };
+    auto scale_entry = [&](uint32_t raw, uint32_t z) {
+        const uint32_t s = p.scale_type == MXB_SCALE_F32   ? raw
+                           : p.scale_type == MXB_SCALE_F16 ? __float_as_uint(__half2float(
+                                                                 __ushort_as_half(static_cast<unsigned short>(raw))))
+                                                           : raw << 16;
+        z &= 15u;
+        return make_uint2(s, 0x43004300u | z | (z << 16));
+    };
 
-    // This lane's activation row (PACK: row and part) of the MMA's column g.
-    const int part = PACK ? g % 3 : 0;
+    // What this lane reads, as offsets into a unit, the scales and the parts.
+    int w_at[kPieces];
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c)
+        w_at[c] = g * (kRun / 2) + ((c ^ (kPieces == 8 ? g : g >> 1)) << 4) + 4 * t;
+    const uint2* scale_at = reinterpret_cast<const uint2*>(extra) + g * kPieces;
+
     float tot[MT][RT][4] = {};
     int r = warp;
     if (lane == 0) {
@@ -167,62 +193,82 @@ __global__ void __launch_bounds__(32 * kFewWarps)
             if (r + d * kFewWarps < runs) issue(r + d * kFewWarps, d);
     }
     if (r < runs) load_group(r);
-    const bool whole = p.group % kRun == 0;  // one group to a run
     uint32_t phase = 0;
     bool failed = false;
     for (int slot = 0; r < runs; r += kFewWarps) {
-        __syncwarp();  // the unit and the scales before these are read by every lane
+        __syncwarp();  // the unit, scales and parts before these are read by every lane
 #pragma unroll
         for (int j = 0; j < 2 * MT; ++j) {
-            const uint32_t raw = s_raw[j], z = z_raw[j] & 15u;
-            const uint32_t s = p.scale_type == MXB_SCALE_F32   ? raw
-                               : p.scale_type == MXB_SCALE_F16 ? __float_as_uint(__half2float(
-                                                                     __ushort_as_half(static_cast<unsigned short>(raw))))
-                                                               : raw << 16;
-            scales[(j * 8 + g) * 4 + t] = make_uint2(s, 0x43004300u | z | (z << 16));
+            const uint2 lo = scale_entry(s_raw[0][j], z_raw[0][j]);
+            uint2* entry = reinterpret_cast<uint2*>(extra) + (j * 8 + g) * kPieces + kOwn * t;
+            if constexpr (kOwn == 1) {
+                *entry = lo;
+            } else {
+                const uint2 hi = span > 1 ? lo : scale_entry(s_raw[1][j], z_raw[1][j]);
+                *reinterpret_cast<uint4*>(entry) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
         }
         if (r + kFewWarps < runs) load_group(r + kFewWarps);
         const int ahead = r + (C::kDepth - 1) * kFewWarps;
         if (lane == 0 && ahead < runs) issue(ahead, slot == 0 ? C::kDepth - 1 : slot - 1);
         if (!mbar_wait(bar0 + 8 * slot, phase, p.timeout_ns)) failed = true;
-        failed = __any_sync(0xffffffffu, failed);  // (also makes the scales visible)
-        if (failed) break;
+        if (__any_sync(0xffffffffu, failed)) {
+            failed = true;
+            break;
+        }
         const uint8_t* unit = ring + slot * C::kUnit;
-        float acc[MT][RT][4] = {};
+        if constexpr (PACK) {
+            // Each lane cuts eight of a row's values, once for the run: piece lane / 4, word t = lane % 4.
+            const int c = g;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            // Parts of this lane's eight activations: pairs (k, k + 4) as the nibbles of a word pair up.
-            uint32_t b[RT][PACK ? 1 : 3][4];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const int m = PACK ? (g < 6 ? g / 3 : 0) : rt * 8 + g;
+            for (int m = 0; m < 2; ++m) {
+                if (m >= rows) break;
                 const uint8_t* x = unit + C::kWeightBytes + c * C::kPieceBytes + m * 128;
                 const int swizzle = (smem_addr(x) >> 7) & 7;
-                float4 lo = *reinterpret_cast<const float4*>(x + (((2 * t) ^ swizzle) << 4));
-                float4 hi = *reinterpret_cast<const float4*>(x + (((2 * t + 1) ^ swizzle) << 4));
+                const float4 lo = *reinterpret_cast<const float4*>(x + (((2 * t) ^ swizzle) << 4));
+                const float4 hi = *reinterpret_cast<const float4*>(x + (((2 * t + 1) ^ swizzle) << 4));
                 float u[4] = {lo.x, lo.y, lo.z, lo.w}, v[4] = {hi.x, hi.y, hi.z, hi.w};
+                uint4* parts = reinterpret_cast<uint4*>(extra + C::kScaleBytes) + (c * 6 + 3 * m) * 4 + t;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t p0 = cut_pair(u[i], v[i]), p1 = cut_pair(u[i], v[i]);
-                    const uint32_t p2 = __byte_perm(__float_as_uint(u[i]), __float_as_uint(v[i]), 0x7632);
-                    if (PACK) {
-                        b[rt][0][i] = part == 0 ? p0 : part == 1 ? p1 : p2;
-                    } else {
-                        b[rt][0][i] = p2;  // small parts first
-                        b[rt][PACK ? 0 : 1][i] = p1;
-                        b[rt][PACK ? 0 : 2][i] = p0;
-                    }
+                for (int q = 0; q < 3; ++q)
+                    parts[q * 4] = make_uint4(cut_pair(u[0], v[0]), cut_pair(u[1], v[1]), cut_pair(u[2], v[2]),
+                                              cut_pair(u[3], v[3]));
+            }
+            __syncwarp();
+        }
+        float acc[MT][RT][4] = {};
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+            // Parts of this lane's eight activations: pairs (k, k + 4) as the nibbles of a word pair up.
+            uint32_t b[RT][PACK ? 1 : 3][4];
+            if (PACK) {
+                const uint4 v = reinterpret_cast<const uint4*>(extra + C::kScaleBytes)[(c * 6 + min(g, 3 * rows - 1)) * 4 + t];
+                b[0][0][0] = v.x;
+                b[0][0][1] = v.y;
+                b[0][0][2] = v.z;
+                b[0][0][3] = v.w;
+            } else {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const uint8_t* x = unit + C::kWeightBytes + c * C::kPieceBytes + (rt * 8 + g) * 128;
+                    const float4 lo = *reinterpret_cast<const float4*>(x + (((2 * t) ^ g) << 4));
+                    const float4 hi = *reinterpret_cast<const float4*>(x + (((2 * t + 1) ^ g) << 4));
+                    float u[4] = {lo.x, lo.y, lo.z, lo.w}, v[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int q = 2; q >= 0; --q)  // (small parts first below)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) b[rt][PACK ? 0 : q][i] = cut_pair(u[i], v[i]);
                 }
             }
+            const bool flush = (c & (span - 1)) == span - 1;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 uint32_t w[2];
                 uint2 sz[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int i = mt * 16 + h * 8 + g;
-                    w[h] = *reinterpret_cast<const uint32_t*>(unit + i * 64 + ((c ^ ((i >> 1) & 3)) << 4) + 4 * t);
-                    sz[h] = scales[i * 4 + (whole ? 0 : c)];
+                    w[h] = *reinterpret_cast<const uint32_t*>(unit + w_at[c] + (mt * 16 + h * 8) * (kRun / 2));
+                    sz[h] = scale_at[(mt * 16 + h * 8) * kPieces + c];
                 }
                 const uint32_t a1[4] = {weight_pair(w[0], sz[0].y), weight_pair(w[1], sz[1].y),
                                         weight_pair(w[0] >> 4, sz[0].y), weight_pair(w[1] >> 4, sz[1].y)};
@@ -235,7 +281,7 @@ __global__ void __launch_bounds__(32 * kFewWarps)
                         mma_bf16(acc[mt][rt], a1, b[rt][q][0], b[rt][q][1]);
                         mma_bf16(acc[mt][rt], a2, b[rt][q][2], b[rt][q][3]);
                     }
-                    if (!whole || c == 3) {
+                    if (flush) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             tot[mt][rt][i] += __uint_as_float(sz[i >> 1].x) * acc[mt][rt][i];
@@ -301,12 +347,13 @@ cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
     CUtensorMap mw, ma;
     const unsigned long long w_dims[2] = {static_cast<unsigned long long>(p.ldq), static_cast<unsigned long long>(p.N)};
     const unsigned long long w_stride[1] = {static_cast<unsigned long long>(p.ldq)};
-    const unsigned w_box[2] = {kRun / 2, 16 * MT};
+    const unsigned w_box[2] = {C::kRun / 2, 16 * MT};
     const unsigned long long a_dims[2] = {static_cast<unsigned long long>(p.K), static_cast<unsigned long long>(p.M)};
     const unsigned long long a_stride[1] = {static_cast<unsigned long long>(p.lda) * 4};
-    const unsigned a_box[2] = {32, C::kPieceRows};
+    const unsigned a_box[2] = {32, C::kRows};
     if (!encode_tensor_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p.q, w_dims, w_stride, w_box,
-                           CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
+                           C::kRun == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
         !encode_tensor_map(&ma, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, p.a, a_dims, a_stride, a_box,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
         return cudaErrorInvalidValue;
@@ -321,11 +368,11 @@ cudaError_t run_few_rows_width(const Q4Params& p, int num_sms, cudaStream_t stre
     // Wider warp tiles cut each activation for more weights; narrow ones fill the SMs.
     static const char* force = getenv("Q4_MT");
     if (force) {
-        if (force[0] == '4') return run_few_rows<PACK, RT, PACK ? 2 : 4>(p, stream);
+        if (force[0] == '4') return run_few_rows<PACK, RT, 4>(p, stream);
         if (force[0] == '2') return run_few_rows<PACK, RT, 2>(p, stream);
         return run_few_rows<PACK, RT, 1>(p, stream);
     }
-    if (p.N >= 64 * num_sms && !PACK) return run_few_rows<PACK, RT, PACK ? 2 : 4>(p, stream);
+    if (p.N >= 64 * num_sms && !PACK) return run_few_rows<PACK, RT, 4>(p, stream);
     return p.N >= 32 * num_sms ? run_few_rows<PACK, RT, 2>(p, stream) : run_few_rows<PACK, RT, 1>(p, stream);
 }
 
