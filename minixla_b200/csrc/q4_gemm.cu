@@ -47,8 +47,9 @@ struct Q4Params {
 // are used as they lie -- and the same eight k of activation row g, which it
 // cuts itself.  All 16 k of an MMA lie in one group; the sums of a group (of
 // at most a run of it) start from zero and are scaled in fp32.
-//  PACK: one or two rows; the eight MMA columns hold the parts side by side
-//        (column 3 m + part), one MMA instead of three.
+//  PACK: one or two rows (that many); the eight MMA columns hold the parts
+//        side by side (column 3 m + part), one MMA instead of three, and the
+//        warp cuts its run once instead of every lane its own eight values.
 //  RT:   row tiles of eight; their three parts go through three MMAs into
 //        the same accumulators.
 // Each warp has a ring of its own: one lane asks TMA for the next run's
@@ -68,7 +69,8 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 // Two q - z as a bf16 pair, from nibbles 0 and 4 of `w` and the pair (128 + z, 128 + z):
 // 0x4300 | q is the bf16 number 128 + q, and the difference is exact.
 __device__ __forceinline__ uint32_t weight_pair(uint32_t w, uint32_t z128) {
-    uint32_t v = (w & 0x000F000Fu) | 0x43004300u;
+    uint32_t v;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(v) : "r"(w), "r"(0x43004300u));  // (w & mask) | magic
     const __nv_bfloat162 h =
         __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&z128));
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -82,20 +84,21 @@ __device__ __forceinline__ uint32_t cut_pair(float& x, float& y) {
     return __byte_perm(ux, uy, 0x7632);
 }
 
-template <bool PACK, int RT, int MT>
+template <int PACK, int RT, int MT, int SHIFT>
 struct FewCfg {
-    static constexpr int kRows = PACK ? 2 : 8 * RT;
+    static constexpr int kRows = PACK ? PACK : 8 * RT;
     // k of one unit: 128 bytes of a weight row, or 64 where eight or more rows of activations come with them.
     static constexpr int kRun = PACK ? 256 : 128;
     static constexpr int kPieces = kRun / 32;                       // of 32 k
     static constexpr int kWeightBytes = 16 * MT * kRun / 2;
-    static constexpr int kPieceBytes = kRows * 128;                 // an activation box: 32 k of each row
+    static constexpr int kPieceBytes = kRows * 128;                 // 32 k of each row
     static constexpr int kUnit = kWeightBytes + kPieces * kPieceBytes;  // a multiple of 1 KiB
-    static constexpr int kScaleBytes = 16 * MT * kPieces * 8;       // per warp: (scale, zero pair) [row][piece]
-    static constexpr int kPartBytes = PACK ? kPieces * 6 * 4 * 16 : 0;  // per warp: [piece][MMA column][lane t]
+    static constexpr int kStretches = kPieces >> SHIFT;             // of a run, each in one group
+    static constexpr int kScaleBytes = (16 * MT + 8) * kStretches * 8;  // per warp: (scale, zero pair) [stretch][row]
+    static constexpr int kPartBytes = PACK * kPieces * 3 * 4 * 16;  // per warp: [piece][MMA column][lane t]
     static constexpr int kWarpExtra = kScaleBytes + kPartBytes;
     // As many units as fit in half the shared memory (two CTAs), or in all of it.
-    static constexpr int kHalf = (108 * 1024 / kFewWarps - kWarpExtra) / kUnit;
+    static constexpr int kHalf = (111 * 1024 / kFewWarps - kWarpExtra) / kUnit;
     static constexpr int kAll = (220 * 1024 / kFewWarps - kWarpExtra) / kUnit;
     static constexpr int kDepth = kHalf >= 2 ? (kHalf > 4 ? 4 : kHalf) : (kAll > 4 ? 4 : kAll);
     static constexpr int kRing = kUnit * kFewWarps * kDepth;
@@ -106,11 +109,11 @@ struct FewCfg {
     static_assert(kUnit % 1024 == 0 && kDepth >= 2 && kReduce <= kRing && kSmem <= 227 * 1024, "shared memory layout");
 };
 
-template <bool PACK, int RT, int MT>
+template <int PACK, int RT, int MT, int SHIFT>
 __global__ void __launch_bounds__(32 * kFewWarps)
     q4_few_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a,
                        const __grid_constant__ Q4Params p) {
-    using C = FewCfg<PACK, RT, MT>;
+    using C = FewCfg<PACK, RT, MT, SHIFT>;
     constexpr int kRun = C::kRun, kPieces = C::kPieces;
     extern __shared__ uint8_t smem_raw[];
     // (an offset, not a rounded pointer: the compiler then still knows that these are shared addresses)
@@ -132,50 +135,35 @@ __global__ void __launch_bounds__(32 * kFewWarps)
 
     // Unit of run r into slot `slot`.  Weights: row i's 16-byte chunk c (piece c, 32 k) at c ^ (i & 7), or at
     // c ^ ((i >> 1) & 3) in a row of 64 bytes; activations: a box for each piece, row m's 128 bytes at 128 m,
-    // chunk c at c ^ (bits 7..9 of the row's address): the copies' swizzles, conflict-free for the reads below.
+    // chunk c at c ^ (m & 7) (the copies' swizzles, conflict-free for the reads below), or (PACK) row by row.
     auto issue = [&](int r, int slot) {
         const uint32_t dst = smem_addr(ring + slot * C::kUnit), bar = bar0 + 8 * slot;
         mbar_arrive_expect_tx(bar, C::kUnit);
         tma_load_2d(dst, &tm_w, bar, r * (kRun / 2), n0);
 #pragma unroll
-        for (int c = 0; c < kPieces; ++c)
+        for (int c = 0; c < (PACK ? 1 : kPieces); ++c)
             tma_load_2d(dst + C::kWeightBytes + c * C::kPieceBytes, &tm_a, bar, r * kRun + 32 * c, m0);
     };
-    // Pieces between two scalings: all of a run's, or the largest power of two of them that divides a group.
-    const int span = p.group % 256 == 0 && kPieces == 8 ? 8 : p.group % 128 == 0 ? 4 : p.group % 64 == 0 ? 2 : 1;
-    // Lane t loads the scales and zero points of its kOwn pieces of a run for its 2 MT weight rows, a run
-    // ahead and unconverted, so that nothing waits for them here.  One load serves two pieces unless a
-    // group ends between them.
-    constexpr int kOwn = kPieces / 4;
-    uint32_t s_raw[kOwn][2 * MT], z_raw[kOwn][2 * MT];
+    // The run's scales and zero points, one for each weight row and stretch, spread over the lanes
+    // (neighbouring lanes take neighbouring stretches of a row) and loaded a run ahead, unconverted, so that
+    // nothing waits for them here.
+    constexpr int kEntries = 16 * MT * C::kStretches, kOwn = (kEntries + 31) / 32;
+    uint32_t s_raw[kOwn], z_raw[kOwn];
     auto load_group = [&](int r) {
+        const int k = r * kRun + (lane % C::kStretches << SHIFT) * 32;
+        const long long piece = k / p.group;
 #pragma unroll
-        for (int h = 0; h < kOwn; ++h) {
-            if (h == 1 && span > 1) break;
-            // (the span's first piece: its last may lie behind K)
-            const int k = r * kRun + 32 * ((kOwn * t + h) & ~(span - 1));
-            const long long at = static_cast<long long>(n0 + g) * p.lds + k / p.group;
-#pragma unroll
-            for (int j = 0; j < 2 * MT; ++j) {
-                const bool in = n0 + j * 8 + g < p.N && k < p.K;
-                const long long i = at + j * 8 * p.lds;
-                s_raw[h][j] = 0;
-                z_raw[h][j] = 8;
-                if (in) {
-                    s_raw[h][j] = p.scale_type == MXB_SCALE_F32 ? __ldg(static_cast<const uint32_t*>(p.scales) + i)
-                                                                : __ldg(static_cast<const unsigned short*>(p.scales) + i);
-                    if (p.zeros) z_raw[h][j] = __ldg(p.zeros + i);
-                }
+        for (int i = 0; i < kOwn; ++i) {
+            const int row = (32 * i + lane) / C::kStretches, n = n0 + row;
+            s_raw[i] = 0;
+            z_raw[i] = 8;
+            if (row < 16 * MT && n < p.N && k < p.K) {
+                const long long at = n * p.lds + piece;
+                s_raw[i] = p.scale_type == MXB_SCALE_F32 ? __ldg(static_cast<const uint32_t*>(p.scales) + at)
+                                                         : __ldg(static_cast<const unsigned short*>(p.scales) + at);
+                if (p.zeros) z_raw[i] = __ldg(p.zeros + at);
             }
         }
-    };
-    auto scale_entry = [&](uint32_t raw, uint32_t z) {
-        const uint32_t s = p.scale_type == MXB_SCALE_F32   ? raw
-                           : p.scale_type == MXB_SCALE_F16 ? __float_as_uint(__half2float(
-                                                                 __ushort_as_half(static_cast<unsigned short>(raw))))
-                                                           : raw << 16;
-        z &= 15u;
-        return make_uint2(s, 0x43004300u | z | (z << 16));
     };
 
     // What this lane reads, as offsets into a unit, the scales and the parts.
@@ -183,8 +171,9 @@ __global__ void __launch_bounds__(32 * kFewWarps)
 #pragma unroll
     for (int c = 0; c < kPieces; ++c)
         w_at[c] = g * (kRun / 2) + ((c ^ (kPieces == 8 ? g : g >> 1)) << 4) + 4 * t;
-    const uint2* scale_at = reinterpret_cast<const uint2*>(extra) + g * kPieces;
+    const uint2* scale_at = reinterpret_cast<const uint2*>(extra) + g;
 
+    const int part_at = min(g, 3 * PACK - 1) * 4 + t;  // (columns without a part repeat the last: not stored)
     float tot[MT][RT][4] = {};
     int r = warp;
     if (lane == 0) {
@@ -198,15 +187,16 @@ __global__ void __launch_bounds__(32 * kFewWarps)
     for (int slot = 0; r < runs; r += kFewWarps) {
         __syncwarp();  // the unit, scales and parts before these are read by every lane
 #pragma unroll
-        for (int j = 0; j < 2 * MT; ++j) {
-            const uint2 lo = scale_entry(s_raw[0][j], z_raw[0][j]);
-            uint2* entry = reinterpret_cast<uint2*>(extra) + (j * 8 + g) * kPieces + kOwn * t;
-            if constexpr (kOwn == 1) {
-                *entry = lo;
-            } else {
-                const uint2 hi = span > 1 ? lo : scale_entry(s_raw[1][j], z_raw[1][j]);
-                *reinterpret_cast<uint4*>(entry) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-            }
+        for (int i = 0; i < kOwn; ++i) {
+            const int e = 32 * i + lane;
+            const uint32_t raw = s_raw[i], z = z_raw[i] & 15u;
+            const uint32_t sc = p.scale_type == MXB_SCALE_F32   ? raw
+                                : p.scale_type == MXB_SCALE_F16 ? __float_as_uint(__half2float(
+                                                                      __ushort_as_half(static_cast<unsigned short>(raw))))
+                                                                : raw << 16;
+            if (e < kEntries)
+                reinterpret_cast<uint2*>(extra)[e % C::kStretches * (16 * MT + 8) + e / C::kStretches] =
+                    make_uint2(sc, 0x43004300u | z | (z << 16));
         }
         if (r + kFewWarps < runs) load_group(r + kFewWarps);
         const int ahead = r + (C::kDepth - 1) * kFewWarps;
@@ -219,16 +209,12 @@ __global__ void __launch_bounds__(32 * kFewWarps)
         const uint8_t* unit = ring + slot * C::kUnit;
         if constexpr (PACK) {
             // Each lane cuts eight of a row's values, once for the run: piece lane / 4, word t = lane % 4.
-            const int c = g;
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                if (m >= rows) break;
-                const uint8_t* x = unit + C::kWeightBytes + c * C::kPieceBytes + m * 128;
-                const int swizzle = (smem_addr(x) >> 7) & 7;
-                const float4 lo = *reinterpret_cast<const float4*>(x + (((2 * t) ^ swizzle) << 4));
-                const float4 hi = *reinterpret_cast<const float4*>(x + (((2 * t + 1) ^ swizzle) << 4));
+            for (int m = 0; m < PACK; ++m) {
+                const float4* x = reinterpret_cast<const float4*>(unit + C::kWeightBytes + m * kRun * 4) + 2 * lane;
+                const float4 lo = x[0], hi = x[1];
                 float u[4] = {lo.x, lo.y, lo.z, lo.w}, v[4] = {hi.x, hi.y, hi.z, hi.w};
-                uint4* parts = reinterpret_cast<uint4*>(extra + C::kScaleBytes) + (c * 6 + 3 * m) * 4 + t;
+                uint4* parts = reinterpret_cast<uint4*>(extra + C::kScaleBytes) + (g * 3 * PACK + 3 * m) * 4 + t;
 #pragma unroll
                 for (int q = 0; q < 3; ++q)
                     parts[q * 4] = make_uint4(cut_pair(u[0], v[0]), cut_pair(u[1], v[1]), cut_pair(u[2], v[2]),
@@ -242,7 +228,7 @@ __global__ void __launch_bounds__(32 * kFewWarps)
             // Parts of this lane's eight activations: pairs (k, k + 4) as the nibbles of a word pair up.
             uint32_t b[RT][PACK ? 1 : 3][4];
             if (PACK) {
-                const uint4 v = reinterpret_cast<const uint4*>(extra + C::kScaleBytes)[(c * 6 + min(g, 3 * rows - 1)) * 4 + t];
+                const uint4 v = reinterpret_cast<const uint4*>(extra + C::kScaleBytes)[part_at + c * 3 * PACK * 4];
                 b[0][0][0] = v.x;
                 b[0][0][1] = v.y;
                 b[0][0][2] = v.z;
@@ -260,7 +246,8 @@ __global__ void __launch_bounds__(32 * kFewWarps)
                         for (int i = 0; i < 4; ++i) b[rt][PACK ? 0 : q][i] = cut_pair(u[i], v[i]);
                 }
             }
-            const bool flush = (c & (span - 1)) == span - 1;
+            const int stretch = c >> SHIFT;
+            const bool flush = ((c + 1) >> SHIFT) != stretch;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
                 uint32_t w[2];
@@ -268,7 +255,7 @@ __global__ void __launch_bounds__(32 * kFewWarps)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     w[h] = *reinterpret_cast<const uint32_t*>(unit + w_at[c] + (mt * 16 + h * 8) * (kRun / 2));
-                    sz[h] = scale_at[(mt * 16 + h * 8) * kPieces + c];
+                    sz[h] = scale_at[stretch * (16 * MT + 8) + mt * 16 + h * 8];
                 }
                 const uint32_t a1[4] = {weight_pair(w[0], sz[0].y), weight_pair(w[1], sz[1].y),
                                         weight_pair(w[0] >> 4, sz[0].y), weight_pair(w[1] >> 4, sz[1].y)};
@@ -327,10 +314,10 @@ __global__ void __launch_bounds__(32 * kFewWarps)
     }
 }
 
-template <bool PACK, int RT, int MT>
+template <int PACK, int RT, int MT, int SHIFT>
 cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
-    using C = FewCfg<PACK, RT, MT>;
-    auto kernel = q4_few_rows_kernel<PACK, RT, MT>;
+    using C = FewCfg<PACK, RT, MT, SHIFT>;
+    auto kernel = q4_few_rows_kernel<PACK, RT, MT, SHIFT>;
     static std::mutex mu;
     static uint64_t configured = 0;
     int dev = 0;
@@ -350,12 +337,13 @@ cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
     const unsigned w_box[2] = {C::kRun / 2, 16 * MT};
     const unsigned long long a_dims[2] = {static_cast<unsigned long long>(p.K), static_cast<unsigned long long>(p.M)};
     const unsigned long long a_stride[1] = {static_cast<unsigned long long>(p.lda) * 4};
-    const unsigned a_box[2] = {32, C::kRows};
+    const unsigned a_box[2] = {PACK ? C::kRun : 32, C::kRows};
     if (!encode_tensor_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p.q, w_dims, w_stride, w_box,
                            C::kRun == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
         !encode_tensor_map(&ma, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, p.a, a_dims, a_stride, a_box,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
+                           PACK ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
         return cudaErrorInvalidValue;
     kernel<<<dim3((p.N + 16 * MT - 1) / (16 * MT), (p.M + C::kRows - 1) / C::kRows), 32 * kFewWarps, C::kSmem, stream>>>(
         mw, ma, p);
@@ -363,17 +351,23 @@ cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
     return cudaGetLastError();
 }
 
-template <bool PACK, int RT>
+template <int PACK, int RT, int MT>
+cudaError_t run_few_rows_groups(const Q4Params& p, cudaStream_t stream) {
+    // A scaling for every 128 k where the groups allow it, else for every 32.
+    return p.group % 128 == 0 ? run_few_rows<PACK, RT, MT, 2>(p, stream) : run_few_rows<PACK, RT, MT, 0>(p, stream);
+}
+
+template <int PACK, int RT>
 cudaError_t run_few_rows_width(const Q4Params& p, int num_sms, cudaStream_t stream) {
     // Wider warp tiles cut each activation for more weights; narrow ones fill the SMs.
     static const char* force = getenv("Q4_MT");
     if (force) {
-        if (force[0] == '4') return run_few_rows<PACK, RT, 4>(p, stream);
-        if (force[0] == '2') return run_few_rows<PACK, RT, 2>(p, stream);
-        return run_few_rows<PACK, RT, 1>(p, stream);
+        if (force[0] == '4') return run_few_rows_groups<PACK, RT, 4>(p, stream);
+        if (force[0] == '2') return run_few_rows_groups<PACK, RT, 2>(p, stream);
+        return run_few_rows_groups<PACK, RT, 1>(p, stream);
     }
-    if (p.N >= 64 * num_sms && !PACK) return run_few_rows<PACK, RT, 4>(p, stream);
-    return p.N >= 32 * num_sms ? run_few_rows<PACK, RT, 2>(p, stream) : run_few_rows<PACK, RT, 1>(p, stream);
+    if (p.N >= 64 * num_sms && !PACK) return run_few_rows_groups<PACK, RT, 4>(p, stream);
+    return p.N >= 32 * num_sms ? run_few_rows_groups<PACK, RT, 2>(p, stream) : run_few_rows_groups<PACK, RT, 1>(p, stream);
 }
 
 int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, void* stream) {
@@ -398,9 +392,10 @@ int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, voi
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     p.timeout_ns = ctx->timeout_ns;
     p.err = ctx->d_err;
-    const cudaError_t e = p.M <= 2   ? run_few_rows_width<true, 1>(p, ctx->num_sms, st)
-                          : p.M <= 8 ? run_few_rows_width<false, 1>(p, ctx->num_sms, st)
-                                     : run_few_rows_width<false, 2>(p, ctx->num_sms, st);
+    const cudaError_t e = p.M == 1   ? run_few_rows_width<1, 1>(p, ctx->num_sms, st)
+                          : p.M == 2 ? run_few_rows_width<2, 1>(p, ctx->num_sms, st)
+                          : p.M <= 8 ? run_few_rows_width<0, 1>(p, ctx->num_sms, st)
+                                     : run_few_rows_width<0, 2>(p, ctx->num_sms, st);
     return cuda_ok(e, "4-bit product launch") ? MXB_OK : MXB_E_CUDA;
 }
 
