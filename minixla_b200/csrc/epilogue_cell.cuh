@@ -39,6 +39,43 @@ __device__ __forceinline__ float apply_cell(float v, long long row, int col, int
     return v;
 }
 
+// The steps for W outputs of column `col` (rows row .. row + W - 1, the first `n` of them wanted).
+template <int W>
+__device__ __forceinline__ void apply_column(float (&v)[W], long long row, int n, int col, int group,
+                                             const CellEpilogue& e) {
+    for (int s = 0; s < e.n_steps; ++s) {
+        const EpStepDev& st = e.steps[s];
+        if (st.kind == MXB_EP_RELU) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
+        } else if (st.kind == MXB_EP_SCALE) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = v[i] * st.scale;
+        } else if (st.kind == MXB_EP_ADD_ROW) {
+            const float b = __ldg(st.ptr + group * st.ld_or_size + col);
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] += b;
+        } else if (st.kind == MXB_EP_ADD_MOD) {
+            const unsigned long long size = static_cast<unsigned long long>(st.ld_or_size);
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (i < n) v[i] += __ldg(st.ptr + (static_cast<unsigned long long>(row + i) * e.n_cols + col) % size);
+        } else {  // ADD_FULL, RELU_GRAD
+            const float* src = st.ptr + row * st.ld_or_size + col;
+            float c[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) c[i] = i < n ? __ldg(src + i * st.ld_or_size) : 0.0f;
+            if (st.kind == MXB_EP_ADD_FULL) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] += c[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] = c[i] > 0.0f ? v[i] : 0.0f;
+            }
+        }
+    }
+}
+
 // Checks `steps` for an output of n_cols columns and copies them.  `grouped`:
 // the steps of the grouped products (RELU_GRAD, ADD_ROW with a pitch between
 // groups, no modulo rule); else those of mxb_fused_gemm.

@@ -177,38 +177,6 @@ __device__ __forceinline__ void grouped_scan(GroupedTable& tab, const GroupedPar
     if (lane == 0) tab.total = base;
 }
 
-// The steps for W outputs of column `col` (rows row .. row + W - 1, the first `n` of them wanted).
-template <int W>
-__device__ __forceinline__ void apply_column(float (&v)[W], long long row, int n, int col, int group,
-                                             const CellEpilogue& e) {
-    for (int s = 0; s < e.n_steps; ++s) {
-        const EpStepDev& st = e.steps[s];
-        if (st.kind == MXB_EP_RELU) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
-        } else if (st.kind == MXB_EP_SCALE) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = v[i] * st.scale;
-        } else if (st.kind == MXB_EP_ADD_ROW) {
-            const float b = __ldg(st.ptr + group * st.ld_or_size + col);
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[i] += b;
-        } else {  // ADD_FULL, RELU_GRAD
-            const float* src = st.ptr + row * st.ld_or_size + col;
-            float c[W];
-#pragma unroll
-            for (int i = 0; i < W; ++i) c[i] = i < n ? __ldg(src + i * st.ld_or_size) : 0.0f;
-            if (st.kind == MXB_EP_ADD_FULL) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) v[i] += c[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < W; ++i) v[i] = c[i] > 0.0f ? v[i] : 0.0f;
-            }
-        }
-    }
-}
-
 __device__ __forceinline__ void raise_grouped(const GroupedParams& p, volatile int* abort_flag, int bit) {
     atomicOr(p.err, bit);
     *abort_flag = 1;

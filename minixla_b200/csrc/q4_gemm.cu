@@ -359,15 +359,429 @@ cudaError_t run_few_rows_groups(const Q4Params& p, cudaStream_t stream) {
 
 template <int PACK, int RT>
 cudaError_t run_few_rows_width(const Q4Params& p, int num_sms, cudaStream_t stream) {
-    // Wider warp tiles cut each activation for more weights; narrow ones fill the SMs.
-    static const char* force = getenv("Q4_MT");
-    if (force) {
-        if (force[0] == '4') return run_few_rows_groups<PACK, RT, 4>(p, stream);
-        if (force[0] == '2') return run_few_rows_groups<PACK, RT, 2>(p, stream);
-        return run_few_rows_groups<PACK, RT, 1>(p, stream);
+    // Wider warp tiles cut each activation for more weights; narrow ones fill the SMs.  8192 x 8192, groups
+    // of 128, cold L2: one row 25.4 / 19.5 us at 16 / 32 columns a warp, eight rows 37.9 / 29.6 / 27.6 us at
+    // 16 / 32 / 64 (groups of 32: 42.0 / 31.7 / 33.8), sixteen rows 68.6 / 46.0 / 35.8 us.
+    if (RT == 2 && p.N >= 32 * num_sms) return run_few_rows_groups<PACK, RT, RT == 2 ? 4 : 2>(p, stream);
+    return p.N >= 24 * num_sms ? run_few_rows_groups<PACK, RT, 2>(p, stream) : run_few_rows_groups<PACK, RT, 1>(p, stream);
+}
+
+// ---------------------------------------------------------------- many rows
+//
+// More than 16 rows: bound by the tensor cores.  A tile is 128 weight columns
+// (TMEM lanes) by up to 128 rows (TMEM columns).  Eight warps turn the 4-bit
+// values of 64 k into a K-major bf16 tile of q - z (exact); the activations'
+// three bf16 parts, cut beforehand into workspace by q4_cut_kernel, arrive by
+// TMA; per 16 k the three parts are multiplied into the same accumulator.
+// That is 3 bf16 products, half the tensor time of the 3xTF32 product that
+// fp32 weights need, and exact up to the fp32 sums.  An accumulator takes the
+// k of one group (at most 128); the epilogue warps, whose lanes each hold one
+// weight column, add it times that column's scale to fp32 totals.
+// The eight k of a word keep the order in which its nibbles pair up (k, k + 4):
+// the cut kernel writes the activations in the same order.
+
+constexpr int kManyCols = 128;  // rows of A per tile
+constexpr int kManyK = 64;      // k per stage: 128 bytes of bf16
+
+struct ManyCfg {
+    static constexpr int kXBytes = 3 * kManyCols * kManyK * 2;  // the parts of a stage
+    static constexpr int kXStages = 3;
+    static constexpr int kRawBytes = 128 * 64;                  // 128 k of 128 weight rows
+    static constexpr int kRawStages = 4;
+    static constexpr int kDeqBytes = 128 * kManyK * 2;
+    static constexpr int kDeqStages = 2;
+    static constexpr int kEpiWarps = 8, kConvWarps = 8;
+    static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 2);
+    static constexpr int kRawOffset = kXStages * kXBytes;
+    static constexpr int kDeqOffset = kRawOffset + kRawStages * kRawBytes;
+    static constexpr int kBarOffset = kDeqOffset + kDeqStages * kDeqBytes;
+    static constexpr int kNumBars = 2 * kXStages + 2 * kRawStages + 2 * kDeqStages + 4 + 1;
+    static constexpr int kTmemCols = 2 * kManyCols;
+    static constexpr int kSmem = 1024 + kBarOffset + kNumBars * 8 + 16;
+    static_assert(kSmem <= 227 * 1024, "shared memory budget");
+};
+
+// kind::f16 with bf16 operands, both K-major, fp32 accumulation.
+__host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// parts[q][m][k'] = part q of A[m][k], k' the pair order within each eight k; zeros from K to kp.
+__global__ void __launch_bounds__(256) q4_cut_kernel(const float* a, long long lda, int M, int K, long long kp,
+                                                     uint4* parts) {
+    const long long eights = kp / 8, total = M * eights;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+        const long long m = i / eights;
+        const int k = static_cast<int>(i - m * eights) * 8;
+        const float* src = a + m * lda + k;
+        float u[4], v[4];
+        if (k + 8 <= K) {
+            const float4 lo = __ldg(reinterpret_cast<const float4*>(src));
+            const float4 hi = __ldg(reinterpret_cast<const float4*>(src) + 1);
+            u[0] = lo.x, u[1] = lo.y, u[2] = lo.z, u[3] = lo.w;
+            v[0] = hi.x, v[1] = hi.y, v[2] = hi.z, v[3] = hi.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] = k + j < K ? __ldg(src + j) : 0.0f;
+                v[j] = k + 4 + j < K ? __ldg(src + 4 + j) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+            parts[q * total + i] = make_uint4(cut_pair(u[0], v[0]), cut_pair(u[1], v[1]), cut_pair(u[2], v[2]),
+                                              cut_pair(u[3], v[3]));
     }
-    if (p.N >= 64 * num_sms && !PACK) return run_few_rows_groups<PACK, RT, 4>(p, stream);
-    return p.N >= 32 * num_sms ? run_few_rows_groups<PACK, RT, 2>(p, stream) : run_few_rows_groups<PACK, RT, 1>(p, stream);
+}
+
+struct ManyParams {
+    Q4Params q;
+    int col_tiles, tiles;
+};
+
+__device__ __forceinline__ void raise_q4(const Q4Params& p, volatile int* abort_flag, int bit) {
+    atomicOr(p.err, bit);
+    *abort_flag = 1;
+}
+
+__device__ __forceinline__ float scale_value(const Q4Params& p, long long at) {
+    if (p.scale_type == MXB_SCALE_F32) return __ldg(static_cast<const float*>(p.scales) + at);
+    const unsigned short raw = __ldg(static_cast<const unsigned short*>(p.scales) + at);
+    return p.scale_type == MXB_SCALE_F16 ? __half2float(__ushort_as_half(raw)) : __uint_as_float(raw << 16);
+}
+
+__global__ void __launch_bounds__(ManyCfg::kThreads, 1)
+    q4_many_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                        const __grid_constant__ ManyParams mp) {
+    using C = ManyCfg;
+    const Q4Params& p = mp.q;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const uint32_t bar0 = smem_addr(bars);
+    constexpr int kX = C::kXStages, kR = C::kRawStages, kD = C::kDeqStages;
+    auto xfull = [&](int s) { return bar0 + 8u * s; };
+    auto xempty = [&](int s) { return bar0 + 8u * (kX + s); };
+    auto rfull = [&](int s) { return bar0 + 8u * (2 * kX + s); };
+    auto rempty = [&](int s) { return bar0 + 8u * (2 * kX + kR + s); };
+    auto dfull = [&](int s) { return bar0 + 8u * (2 * kX + 2 * kR + s); };
+    auto dempty = [&](int s) { return bar0 + 8u * (2 * kX + 2 * kR + kD + s); };
+    auto tfull = [&](int a) { return bar0 + 8u * (2 * kX + 2 * kR + 2 * kD + a); };
+    auto tempty = [&](int a) { return bar0 + 8u * (2 * kX + 2 * kR + 2 * kD + 2 + a); };
+    const uint32_t drain = bar0 + 8u * (2 * kX + 2 * kR + 2 * kD + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kConvWarp = C::kEpiWarps, kTmaWarp = kConvWarp + C::kConvWarps, kMmaWarp = kTmaWarp + 1;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kX; ++s) {
+            mbar_init(xfull(s), 1);
+            mbar_init(xempty(s), 1);
+        }
+        for (int s = 0; s < kR; ++s) {
+            mbar_init(rfull(s), 1);
+            mbar_init(rempty(s), C::kConvWarps);
+        }
+        for (int s = 0; s < kD; ++s) {
+            mbar_init(dfull(s), C::kConvWarps);
+            mbar_init(dempty(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull(a), 1);
+            mbar_init(tempty(a), C::kEpiWarps);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tm_w);
+        tma_prefetch_desc(&tm_x);
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int stages = (p.K + kManyK - 1) / kManyK;
+    const int halves = (p.K + 31) / 32;                                     // of 32 k
+    const int seg = p.group % 128 == 0 ? 4 : p.group % 64 == 0 ? 2 : 1;     // halves to an accumulator
+
+    if (warp == kTmaWarp) {
+        if (lane == 0) {
+            int xs = 0, rs = 0;
+            uint32_t xph = 0, rph = 0;
+            long long xn = 0, rn = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < mp.tiles && ok; t += gridDim.x) {
+                const int n0 = t / mp.col_tiles * 128, m0 = t % mp.col_tiles * kManyCols;
+                const int boxes = (min(kManyCols, p.M - m0) + 31) / 32;
+                for (int kb = 0; kb < stages; ++kb) {
+                    if ((kb & 1) == 0) {
+                        if (*abort_flag || !mbar_wait(rempty(rs), rph ^ 1u, p.timeout_ns)) {
+                            ok = false;
+                            break;
+                        }
+                        mbar_arrive_expect_tx(rfull(rs), C::kRawBytes);
+                        tma_load_2d(smem_addr(smem + C::kRawOffset + rs * C::kRawBytes), &tm_w, rfull(rs), kb * 32, n0);
+                        ++rn;
+                        if (++rs == kR) { rs = 0; rph ^= 1u; }
+                    }
+                    if (*abort_flag || !mbar_wait(xempty(xs), xph ^ 1u, p.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_expect_tx(xfull(xs), 3 * boxes * 4096);
+                    const uint32_t dst = smem_addr(smem + xs * C::kXBytes);
+                    for (int q = 0; q < 3; ++q)
+                        for (int j = 0; j < boxes; ++j)
+                            tma_load_3d(dst + (q * 4 + j) * 4096, &tm_x, xfull(xs), kb * kManyK, m0 + 32 * j, q);
+                    ++xn;
+                    if (++xs == kX) { xs = 0; xph ^= 1u; }
+                }
+            }
+            if (!ok) {
+                raise_q4(p, abort_flag, kErrProducer);
+                // Copies in flight land in this CTA's shared memory: wait for them before leaving.
+                for (long long i = xn > kX ? xn - kX : 0; i < xn; ++i)
+                    mbar_wait(xfull(static_cast<int>(i % kX)), static_cast<uint32_t>((i / kX) & 1), p.timeout_ns);
+                for (long long i = rn > kR ? rn - kR : 0; i < rn; ++i)
+                    mbar_wait(rfull(static_cast<int>(i % kR)), static_cast<uint32_t>((i / kR) & 1), p.timeout_ns);
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        if (lane == 0) {
+            int xs = 0, ds = 0, acc = 0;
+            uint32_t xph = 0, dph = 0, aph = 0;
+            bool ok = true;
+            for (int t = blockIdx.x; t < mp.tiles && ok; t += gridDim.x) {
+                const int m0 = t % mp.col_tiles * kManyCols;
+                const uint32_t idesc = idesc_bf16(128, (min(kManyCols, p.M - m0) + 15) & ~15);
+                for (int kb = 0; kb < stages && ok; ++kb) {
+                    if (*abort_flag || !mbar_wait(xfull(xs), xph, p.timeout_ns) ||
+                        !mbar_wait(dfull(ds), dph, p.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t w = smem_addr(smem + C::kDeqOffset + ds * C::kDeqBytes);
+                    const uint32_t x = smem_addr(smem + xs * C::kXBytes);
+                    for (int h = 2 * kb; h < min(2 * kb + 2, halves); ++h) {
+                        const bool first = h % seg == 0;
+                        if (first) {
+                            if (!mbar_wait(tempty(acc), aph ^ 1u, p.timeout_ns)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                        }
+                        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kManyCols);
+#pragma unroll
+                        for (int kk = 0; kk < 2; ++kk) {
+                            const uint32_t at = (2 * (h & 1) + kk) * 32;
+                            const uint64_t wd = smem_desc(w + at, 16, 1024, kLayoutSW128);
+#pragma unroll
+                            for (int q = 2; q >= 0; --q)  // small parts first
+                                mma_f16(d, wd, smem_desc(x + q * 4 * 4096 + at, 16, 1024, kLayoutSW128), idesc,
+                                        first && kk == 0 && q == 2 ? 0u : 1u);
+                        }
+                        if (h % seg == seg - 1 || h == halves - 1) {
+                            mma_commit(tfull(acc));
+                            acc ^= 1;
+                            if (acc == 0) aph ^= 1u;
+                        }
+                    }
+                    mma_commit(xempty(xs));
+                    mma_commit(dempty(ds));
+                    if (++xs == kX) { xs = 0; xph ^= 1u; }
+                    if (++ds == kD) { ds = 0; dph ^= 1u; }
+                }
+            }
+            if (!ok) raise_q4(p, abort_flag, kErrMma);
+            mma_commit(drain);
+            if (!mbar_wait(drain, 0, p.timeout_ns)) raise_q4(p, abort_flag, kErrMma);
+        }
+    } else if (warp >= kConvWarp) {
+        // ------------------------------------------------------------ 4 bits to bf16: a row and 32 k a thread
+        const int tid = threadIdx.x - 32 * kConvWarp, row = tid & 127, half = tid >> 7;
+        int rs = 0, ds = 0;
+        uint32_t rph = 0, dph = 0;
+        bool failed = false;
+        for (int t = blockIdx.x; t < mp.tiles && !failed; t += gridDim.x) {
+            const int n = min(t / mp.col_tiles * 128 + row, p.N - 1);
+            auto zero_of = [&](int kb) -> uint32_t {
+                const int k = kb * kManyK + 32 * half;
+                return p.zeros && k < p.K ? __ldg(p.zeros + n * p.lds + k / p.group) : 8u;
+            };
+            uint32_t z_next = zero_of(0);
+            for (int kb = 0; kb < stages; ++kb) {
+                const uint32_t z = z_next & 15u;
+                if (kb + 1 < stages) z_next = zero_of(kb + 1);
+                const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
+                const bool got = !stop && mbar_wait(rfull(rs), rph, p.timeout_ns) &&
+                                 mbar_wait(dempty(ds), dph ^ 1u, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0 && !stop) raise_q4(p, abort_flag, kErrProducer);
+                    failed = true;
+                    break;
+                }
+                const int chunk = (kb & 1) * 2 + half;  // 16 bytes of the row's 64
+                const uint4 w4 = *reinterpret_cast<const uint4*>(smem + C::kRawOffset + rs * C::kRawBytes + row * 64 +
+                                                                 ((chunk ^ ((row >> 1) & 3)) << 4));
+                const uint32_t z128 = 0x43004300u | z | (z << 16);
+                uint8_t* dst = smem + C::kDeqOffset + ds * C::kDeqBytes + row * 128;
+                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<uint4*>(dst + (((4 * half + j) ^ (row & 7)) << 4)) =
+                        make_uint4(weight_pair(w[j], z128), weight_pair(w[j] >> 4, z128), weight_pair(w[j] >> 8, z128),
+                                   weight_pair(w[j] >> 12, z128));
+                fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(dfull(ds));
+                    if ((kb & 1) || kb == stages - 1) mbar_arrive(rempty(rs));
+                }
+                if (++ds == kD) { ds = 0; dph ^= 1u; }
+                if ((kb & 1) || kb == stages - 1) {
+                    if (++rs == kR) { rs = 0; rph ^= 1u; }
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue: a weight column and 64 rows a thread
+        constexpr int W = 16, kTotals = kManyCols / 2;
+        const int quad = warp & 3, first_col = (warp >> 2) * kTotals;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + first_col;
+        int acc = 0;
+        uint32_t aph = 0;
+        bool failed = false;
+        for (int t = blockIdx.x; t < mp.tiles && !failed; t += gridDim.x) {
+            const int col = t / mp.col_tiles * 128 + quad * 32 + lane, m0 = t % mp.col_tiles * kManyCols;
+            const int cols = min(kManyCols, p.M - m0);
+            const long long scale_row = min(col, p.N - 1) * p.lds;
+            float total[kTotals];
+#pragma unroll
+            for (int i = 0; i < kTotals; ++i) total[i] = 0.0f;
+            float s_next = scale_value(p, scale_row);
+            for (int h = 0; h < halves; h += seg) {
+                const float s = s_next;
+                if (h + seg < halves) s_next = scale_value(p, scale_row + (h + seg) * 32 / p.group);
+                const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
+                const bool got = !stop && mbar_wait(tfull(acc), aph, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0 && !stop) raise_q4(p, abort_flag, kErrEpilogue);
+                    failed = true;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < kTotals; c += W) {
+                    if (first_col + c < cols) {
+                        uint32_t r[W];
+                        tmem_ld_32x32b_x16(lane_base + static_cast<uint32_t>(acc * kManyCols + c), r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < W; ++i) total[c + i] += s * __uint_as_float(r[i]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tempty(acc));
+                acc ^= 1;
+                if (acc == 0) aph ^= 1u;
+            }
+            if (failed) break;
+            if (col < p.N) {
+#pragma unroll
+                for (int c = 0; c < kTotals; c += W) {
+                    const int n = min(W, cols - first_col - c);
+                    if (n <= 0) continue;
+                    float v[W];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) v[i] = total[c + i];
+                    const long long row = m0 + first_col + c;
+                    apply_column<W>(v, row, n, col, 0, p.epi);
+                    float* dst = p.out + row * p.ldo + col;
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+                        if (i < n) __stcs(dst + i * p.ldo, v[i]);
+                }
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::kTmemCols);
+    }
+}
+
+int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
+    using C = ManyCfg;
+    static std::mutex mu;
+    static uint64_t configured = 0;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (ctx->device >= 64 || !(configured & (1ull << ctx->device))) {
+            if (!cuda_ok(cudaFuncSetAttribute(q4_many_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
+                         "4-bit product set-up"))
+                return MXB_E_CUDA;
+            if (ctx->device < 64) configured |= 1ull << ctx->device;
+        }
+    }
+    const long long kp = (static_cast<long long>(p.K) + kManyK - 1) / kManyK * kManyK;
+    Scratch scratch(ctx, stream);
+    void* parts = scratch.alloc(static_cast<size_t>(3) * p.M * kp * 2);
+    if (!parts) return MXB_E_NOMEM;
+    const long long blocks = (p.M * (kp / 8) + 255) / 256;
+    q4_cut_kernel<<<static_cast<int>(std::min<long long>(blocks, 8ll * ctx->num_sms)), 256, 0, stream>>>(
+        p.a, p.lda, p.M, p.K, kp, static_cast<uint4*>(parts));
+    note_launch();
+    if (!cuda_ok(cudaGetLastError(), "4-bit product: cutting the rows")) return MXB_E_CUDA;
+
+    CUtensorMap mw, mx;
+    const unsigned long long w_dims[2] = {static_cast<unsigned long long>(p.ldq), static_cast<unsigned long long>(p.N)};
+    const unsigned long long w_stride[1] = {static_cast<unsigned long long>(p.ldq)};
+    const unsigned w_box[2] = {64, 128};
+    const unsigned long long x_dims[3] = {static_cast<unsigned long long>(kp), static_cast<unsigned long long>(p.M), 3};
+    const unsigned long long x_strides[2] = {static_cast<unsigned long long>(kp) * 2,
+                                             static_cast<unsigned long long>(kp) * 2 * p.M};
+    const unsigned x_box[3] = {kManyK, 32, 1};
+    if (!encode_tensor_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p.q, w_dims, w_stride, w_box,
+                           CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
+        !encode_tensor_map(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, parts, x_dims, x_strides, x_box,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B)) {
+        set_error("mxb_q4_gemm: the tensor maps could not be made");
+        return MXB_E_CUDA;
+    }
+    ManyParams mp{p, (p.M + kManyCols - 1) / kManyCols, 0};
+    const long long tiles = static_cast<long long>(mp.col_tiles) * ((p.N + 127) / 128);
+    if (tiles >= (1ll << 31)) {
+        set_error("mxb_q4_gemm: too many tiles");
+        return MXB_E_UNSUPPORTED;
+    }
+    mp.tiles = static_cast<int>(tiles);
+    q4_many_rows_kernel<<<static_cast<int>(std::min<long long>(tiles, ctx->num_sms)), C::kThreads, C::kSmem, stream>>>(
+        mw, mx, mp);
+    note_launch();
+    return cuda_ok(cudaGetLastError(), "4-bit product launch") ? MXB_OK : MXB_E_CUDA;
 }
 
 int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, void* stream) {
@@ -392,6 +806,7 @@ int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, voi
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     p.timeout_ns = ctx->timeout_ns;
     p.err = ctx->d_err;
+    if (p.M > 16) return run_many_rows(ctx, p, st);
     const cudaError_t e = p.M == 1   ? run_few_rows_width<1, 1>(p, ctx->num_sms, st)
                           : p.M == 2 ? run_few_rows_width<2, 1>(p, ctx->num_sms, st)
                           : p.M <= 8 ? run_few_rows_width<0, 1>(p, ctx->num_sms, st)
