@@ -297,67 +297,73 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         }
     } else if (warp == kMmaWarp) {
         // ------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            int stage = 0, small = 0, acc = 0;
-            uint32_t phase = 0, small_phase = 0, acc_phase = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
-                const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
-                const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, kLaneMn, kColMn);
-                const int num_kb = (g.sum + kBK - 1) / kBK;
-                for (int k_begin = 0; k_begin < num_kb && ok; k_begin += kGroupedSegKb) {
-                    const int k_end = min(num_kb, k_begin + kGroupedSegKb);
-                    if (*abort_flag || !mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns)) {
-                        raise_grouped(p, abort_flag, kErrMma);
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
+        // K-major operand: 32 bytes of a 128-byte row for each 8 of the sum; MN-major: 8 rows of 128 bytes.
+        constexpr uint32_t kHiMn = smem_desc_hi(512, kLayoutSW128Base32B), kHiK = smem_desc_hi(1024, kLayoutSW128);
+        constexpr uint32_t kLaneHi = kLaneMn ? kHiMn : kHiK, kColHi = kColMn ? kHiMn : kHiK;
+        constexpr uint32_t kLaneStep = kLaneMn ? 64 : 2, kColStep = kColMn ? 64 : 2;
+        const bool leader = elect_one();
+        int stage = 0, small = 0, acc = 0;
+        uint32_t phase = 0, small_phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, kLaneMn, kColMn);
+            const int num_kb = (g.sum + kBK - 1) / kBK;
+            int in_seg = 0;
+            for (int kb = 0; kb < num_kb; ++kb) {
+                bool ready = *abort_flag == 0;
+                if (ready && in_seg == 0) ready = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
+                if (!ready || !mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
+                    !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const bool end_seg = ++in_seg == kGroupedSegKb || kb == num_kb - 1;
+                if (leader) {
                     const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
-                    for (int kb = k_begin; kb < k_end; ++kb) {
-                        if (!mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
-                            !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
-                            raise_grouped(p, abort_flag, kErrMma);
-                            ok = false;
-                            break;
+                    const uint32_t big = smem_addr(smem + stage * C::kStageBytes);
+                    const uint32_t low = smem_addr(smem + C::kSmallOffset + small * C::kStageBytes);
+                    const uint32_t bl = smem_desc_lo(big, kLaneMn ? kBoxBytes : 16);
+                    const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, kColMn ? kBoxBytes : 16);
+                    const uint32_t sl = smem_desc_lo(low, kLaneMn ? kBoxBytes : 16);
+                    const uint32_t sc = smem_desc_lo(low + C::kLaneBytes, kColMn ? kBoxBytes : 16);
+                    // The last k-block ends with its own eighth: nothing past the sum is multiplied.
+                    const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
+                    const uint32_t begun = in_seg > 1 ? 1u : 0u;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        if (kk >= steps) break;
+                        const uint64_t da = smem_desc_of(kLaneHi, bl + kk * kLaneStep);
+                        const uint64_t db = smem_desc_of(kColHi, bc + kk * kColStep);
+                        if (p.split3) {
+                            // Small cross terms first, the dominant product last.
+                            mma_tf32(d, da, smem_desc_of(kColHi, sc + kk * kColStep), idesc, kk ? 1u : begun);
+                            mma_tf32(d, smem_desc_of(kLaneHi, sl + kk * kLaneStep), db, idesc, 1u);
+                            mma_tf32(d, da, db, idesc, 1u);
+                        } else {
+                            mma_tf32(d, da, db, idesc, kk ? 1u : begun);
                         }
-                        tc_fence_after();
-                        const uint32_t big_l = smem_addr(smem + stage * C::kStageBytes);
-                        const uint32_t small_l = smem_addr(smem + C::kSmallOffset + small * C::kStageBytes);
-                        auto lane_desc = [&](uint32_t base, int kk) {
-                            return kLaneMn ? smem_desc(base + kk * 1024, kBoxBytes, 512, kLayoutSW128Base32B)
-                                           : smem_desc(base + kk * 32, 16, 1024, kLayoutSW128);
-                        };
-                        auto col_desc = [&](uint32_t base, int kk) {
-                            return kColMn ? smem_desc(base + kk * 1024, kBoxBytes, 512, kLayoutSW128Base32B)
-                                          : smem_desc(base + kk * 32, 16, 1024, kLayoutSW128);
-                        };
-                        // The last k-block ends with its own eighth: nothing past the sum is multiplied.
-                        const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
-                        for (int kk = 0; kk < steps; ++kk) {
-                            const uint32_t accumulate = kb != k_begin || kk != 0 ? 1u : 0u;
-                            const uint64_t bl = lane_desc(big_l, kk), bc = col_desc(big_l + C::kLaneBytes, kk);
-                            if (p.split3) {
-                                // Small cross terms first, the dominant product last.
-                                mma_tf32(d, bl, col_desc(small_l + C::kLaneBytes, kk), idesc, accumulate);
-                                mma_tf32(d, lane_desc(small_l, kk), bc, idesc, 1u);
-                            }
-                            mma_tf32(d, bl, bc, idesc, p.split3 ? 1u : accumulate);
-                        }
-                        mma_commit(empty_bar(stage));
-                        mma_commit(sfree_bar(small));
-                        if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
-                        if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
                     }
-                    if (!ok) break;
-                    mma_commit(tfull_bar(acc));
+                    mma_commit(empty_bar(stage));
+                    mma_commit(sfree_bar(small));
+                    if (end_seg) mma_commit(tfull_bar(acc));
+                }
+                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+                if (end_seg) {
+                    in_seg = 0;
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1u;
                 }
             }
+        }
+        if (leader) {
+            if (!ok) raise_grouped(p, abort_flag, kErrMma);
             mma_commit(drain_bar);
             if (!mbar_wait(drain_bar, 0, p.timeout_ns)) raise_grouped(p, abort_flag, kErrMma);
         }
+        __syncwarp();
     } else if (warp >= kConvWarp) {
         // ------------------------------------------------------------ converter (4 warps)
         const int t0 = threadIdx.x - 32 * kConvWarp;

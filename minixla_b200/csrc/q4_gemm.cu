@@ -455,11 +455,24 @@ __device__ __forceinline__ void raise_q4(const Q4Params& p, volatile int* abort_
     *abort_flag = 1;
 }
 
-__device__ __forceinline__ float scale_value(const Q4Params& p, long long at) {
-    if (p.scale_type == MXB_SCALE_F32) return __ldg(static_cast<const float*>(p.scales) + at);
-    const unsigned short raw = __ldg(static_cast<const unsigned short*>(p.scales) + at);
-    return p.scale_type == MXB_SCALE_F16 ? __half2float(__ushort_as_half(raw)) : __uint_as_float(raw << 16);
+// A scale as it lies in memory, and as a number: apart, so that a load can be under way while others are used.
+__device__ __forceinline__ uint32_t scale_raw(const Q4Params& p, long long at) {
+    return p.scale_type == MXB_SCALE_F32 ? __ldg(static_cast<const uint32_t*>(p.scales) + at)
+                                         : __ldg(static_cast<const unsigned short*>(p.scales) + at);
 }
+__device__ __forceinline__ float scale_value(const Q4Params& p, uint32_t raw) {
+    return p.scale_type == MXB_SCALE_F32   ? __uint_as_float(raw)
+           : p.scale_type == MXB_SCALE_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(raw)))
+                                           : __uint_as_float(raw << 16);
+}
+
+// The group of successive k, without a division for each.
+struct GroupWalk {
+    int group, index, pos;  // pos: k - index * group
+    __device__ __forceinline__ void step(int k) {
+        for (pos += k; pos >= group; pos -= group) ++index;
+    }
+};
 
 __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
     q4_many_rows_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
@@ -564,57 +577,66 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
             }
         }
     } else if (warp == kMmaWarp) {
-        if (lane == 0) {
-            int xs = 0, ds = 0, acc = 0;
-            uint32_t xph = 0, dph = 0, aph = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; t < mp.tiles && ok; t += gridDim.x) {
-                const int m0 = t % mp.col_tiles * kManyCols;
-                const uint32_t idesc = idesc_bf16(128, (min(kManyCols, p.M - m0) + 15) & ~15);
-                for (int kb = 0; kb < stages && ok; ++kb) {
-                    if (*abort_flag || !mbar_wait(xfull(xs), xph, p.timeout_ns) ||
-                        !mbar_wait(dfull(ds), dph, p.timeout_ns)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t w = smem_addr(smem + C::kDeqOffset + ds * C::kDeqBytes);
-                    const uint32_t x = smem_addr(smem + xs * C::kXBytes);
-                    for (int h = 2 * kb; h < min(2 * kb + 2, halves); ++h) {
-                        const bool first = h % seg == 0;
-                        if (first) {
-                            if (!mbar_wait(tempty(acc), aph ^ 1u, p.timeout_ns)) {
-                                ok = false;
-                                break;
-                            }
-                            tc_fence_after();
-                        }
-                        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kManyCols);
+        // ------------------------------------------------------------ MMA issuer
+        constexpr uint32_t kHi = smem_desc_hi(1024, kLayoutSW128);
+        const bool leader = elect_one();
+        int xs = 0, ds = 0, acc = 0;
+        uint32_t xph = 0, dph = 0, aph = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; t < mp.tiles && ok; t += gridDim.x) {
+            const int m0 = t % mp.col_tiles * kManyCols;
+            const uint32_t idesc = idesc_bf16(128, (min(kManyCols, p.M - m0) + 15) & ~15);
+            int in_seg = 0;
+            for (int kb = 0; kb < stages && ok; ++kb) {
+                if (*abort_flag || !mbar_wait(xfull(xs), xph, p.timeout_ns) ||
+                    !mbar_wait(dfull(ds), dph, p.timeout_ns)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t w = smem_desc_lo(smem_addr(smem + C::kDeqOffset + ds * C::kDeqBytes), 16);
+                const uint32_t x = smem_desc_lo(smem_addr(smem + xs * C::kXBytes), 16);
 #pragma unroll
-                        for (int kk = 0; kk < 2; ++kk) {
-                            const uint32_t at = (2 * (h & 1) + kk) * 32;
-                            const uint64_t wd = smem_desc(w + at, 16, 1024, kLayoutSW128);
+                for (int h = 0; h < 2; ++h) {
+                    if (2 * kb + h >= halves) break;
+                    if (in_seg == 0) {
+                        if (!mbar_wait(tempty(acc), aph ^ 1u, p.timeout_ns)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                    }
+                    const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kManyCols);
+                    if (leader) {
+#pragma unroll
+                        for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                             for (int q = 2; q >= 0; --q)  // small parts first
-                                mma_f16(d, wd, smem_desc(x + q * 4 * 4096 + at, 16, 1024, kLayoutSW128), idesc,
-                                        first && kk == 0 && q == 2 ? 0u : 1u);
-                        }
-                        if (h % seg == seg - 1 || h == halves - 1) {
-                            mma_commit(tfull(acc));
-                            acc ^= 1;
-                            if (acc == 0) aph ^= 1u;
-                        }
+                                mma_f16(d, smem_desc_of(kHi, w + 2 * (2 * h + kk)),
+                                        smem_desc_of(kHi, x + q * 1024 + 2 * (2 * h + kk)), idesc,
+                                        kk == 0 && q == 2 ? (in_seg != 0 ? 1u : 0u) : 1u);
                     }
+                    if (++in_seg == seg || 2 * kb + h == halves - 1) {
+                        if (leader) mma_commit(tfull(acc));
+                        in_seg = 0;
+                        acc ^= 1;
+                        if (acc == 0) aph ^= 1u;
+                    }
+                }
+                if (leader) {
                     mma_commit(xempty(xs));
                     mma_commit(dempty(ds));
-                    if (++xs == kX) { xs = 0; xph ^= 1u; }
-                    if (++ds == kD) { ds = 0; dph ^= 1u; }
                 }
+                if (++xs == kX) { xs = 0; xph ^= 1u; }
+                if (++ds == kD) { ds = 0; dph ^= 1u; }
             }
+        }
+        if (leader) {
             if (!ok) raise_q4(p, abort_flag, kErrMma);
             mma_commit(drain);
             if (!mbar_wait(drain, 0, p.timeout_ns)) raise_q4(p, abort_flag, kErrMma);
         }
+        __syncwarp();
     } else if (warp >= kConvWarp) {
         // ------------------------------------------------------------ 4 bits to bf16: a row and 32 k a thread
         const int tid = threadIdx.x - 32 * kConvWarp, row = tid & 127, half = tid >> 7;
@@ -623,13 +645,15 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
         bool failed = false;
         for (int t = blockIdx.x; t < mp.tiles && !failed; t += gridDim.x) {
             const int n = min(t / mp.col_tiles * 128 + row, p.N - 1);
+            GroupWalk at{p.group, 0, 0};
+            at.step(32 * half);
             auto zero_of = [&](int kb) -> uint32_t {
-                const int k = kb * kManyK + 32 * half;
-                return p.zeros && k < p.K ? __ldg(p.zeros + n * p.lds + k / p.group) : 8u;
+                return p.zeros && kb * kManyK + 32 * half < p.K ? __ldg(p.zeros + n * p.lds + at.index) : 8u;
             };
             uint32_t z_next = zero_of(0);
             for (int kb = 0; kb < stages; ++kb) {
                 const uint32_t z = z_next & 15u;
+                at.step(kManyK);
                 if (kb + 1 < stages) z_next = zero_of(kb + 1);
                 const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
                 const bool got = !stop && mbar_wait(rfull(rs), rph, p.timeout_ns) &&
@@ -677,10 +701,12 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
             float total[kTotals];
 #pragma unroll
             for (int i = 0; i < kTotals; ++i) total[i] = 0.0f;
-            float s_next = scale_value(p, scale_row);
+            uint32_t s_next = scale_raw(p, scale_row);
+            GroupWalk at{p.group, 0, 0};
             for (int h = 0; h < halves; h += seg) {
-                const float s = s_next;
-                if (h + seg < halves) s_next = scale_value(p, scale_row + (h + seg) * 32 / p.group);
+                const float s = scale_value(p, s_next);
+                at.step(32 * seg);
+                if (h + seg < halves) s_next = scale_raw(p, scale_row + at.index);
                 const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
                 const bool got = !stop && mbar_wait(tfull(acc), aph, p.timeout_ns);
                 if (!__all_sync(0xffffffffu, got)) {

@@ -437,6 +437,34 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo_bytes
     return d;
 }
 
+// The two words of the same descriptor apart: the upper one is a constant of
+// the operand's layout, the lower one moves with the address, 1 per 16 bytes
+// (shared memory ends below 256 KB, so a step never carries past bit 13).
+__host__ __device__ constexpr uint32_t smem_desc_hi(uint32_t sbo_bytes, uint32_t layout) {
+    return ((sbo_bytes >> 4) & 0x3FFFu) | (1u << 14) | ((layout & 7u) << 29);
+}
+
+__device__ __forceinline__ uint32_t smem_desc_lo(uint32_t saddr, uint32_t lbo_bytes) {
+    return ((saddr >> 4) & 0x3FFFu) | ((lbo_bytes >> 4) << 16);
+}
+
+__device__ __forceinline__ uint64_t smem_desc_of(uint32_t hi, uint32_t lo) {
+    return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+// One thread of a converged warp, always the same one.  Loops that the whole
+// warp runs, with only the issue under this predicate, keep their state in
+// uniform registers, which the tcgen05 and TMA instructions read.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t yes;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(yes));
+    return yes != 0;
+}
+
 // Instruction descriptor for kind::tf32 with fp32 accumulation:
 // D format F32 (bits 4-5 = 1), A/B format TF32 (bits 7-9, 10-12 = 2),
 // A K-major (bit 15 = 0), B MN-major (bit 16 = 1), N>>3 at bits 17-22,
