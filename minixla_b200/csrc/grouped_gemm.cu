@@ -107,6 +107,28 @@ __device__ __forceinline__ float small_of(float x) {
     return s == s ? __uint_as_float(__float_as_uint(s) + 0x1000u) : 0.0f;
 }
 
+// The small parts of a staged k-block of n4 float4s (lane side, then column
+// boxes), thread t0 of THREADS; the layout does not matter, both tiles have the
+// same.  grad_b: of the 32 rows of every box (128 bytes each) only the first
+// `valid` belong to the group; the others may hold anything and become zeros.
+template <int MODE, int THREADS>
+__device__ __forceinline__ void convert_tile(uint8_t* big, uint8_t* low, int t0, int n4, int valid, int split3) {
+    float4* src = reinterpret_cast<float4*>(big);
+    float4* dst = reinterpret_cast<float4*>(low);
+    if (MODE == kGradB && valid < kBK) {
+        for (int i = t0; i < n4; i += THREADS)
+            if (((i >> 3) & 31) >= valid) src[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    if (!split3) return;
+    // n4 is a multiple of 2 * THREADS: two float4s a step at least.
+#pragma unroll 4
+    for (int i = t0; i < n4; i += 2 * THREADS) {
+        const float4 v = src[i], w = src[i + THREADS];
+        dst[i] = make_float4(small_of(v.x), small_of(v.y), small_of(v.z), small_of(v.w));
+        dst[i + THREADS] = make_float4(small_of(w.x), small_of(w.y), small_of(w.z), small_of(w.w));
+    }
+}
+
 // One tile of work.
 struct GroupedTile {
     int group;
@@ -126,7 +148,7 @@ static_assert(sizeof(GroupedTable) <= 3 * MXB_MAX_GROUPS * 4 + 16, "table size")
 
 // Tile t: the last group whose first tile is <= t; inside a group the column
 // tiles vary fastest, so CTAs that run together share weights through L2.
-template <int MODE, int BT>
+template <int MODE, int BT, int LANES = 128>
 __device__ __forceinline__ GroupedTile grouped_tile(const GroupedTable& tab, int t, const GroupedParams& p) {
     int lo = 0, hi = p.groups - 1;
     while (lo < hi) {
@@ -144,7 +166,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedTable& tab, int
     const int dim = MODE == kGradB ? p.col_dim : rows;
     const int col_tiles = (dim + BT - 1) / BT;
     const int i = t - tab.first_tile[lo];
-    g.lane0 = i / col_tiles * 128;
+    g.lane0 = i / col_tiles * LANES;
     g.col0 = i % col_tiles * BT;
     g.cols = min(BT, dim - g.col0);
     g.sum = MODE == kGradB ? rows : p.sum_dim;
@@ -383,25 +405,8 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                     failed = true;
                     break;
                 }
-                uint8_t* big = smem + stage * C::kStageBytes;
-                uint8_t* low = smem + C::kSmallOffset + small * C::kStageBytes;
-                const int n4 = 1024 + col_boxes * 256;  // float4s of the tile: lane side, then column boxes
-                // grad_b: the rows behind the group's last belong to others (or to none) and may hold
-                // anything; a row is 128 bytes of every box.
-                const int valid = MODE == kGradB ? min(kBK, g.sum - kb * kBK) : kBK;
-                if (MODE == kGradB && valid < kBK) {
-                    for (int i = t0; i < n4; i += 128)
-                        if (((i >> 3) & 31) >= valid)
-                            reinterpret_cast<float4*>(big)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-                if (p.split3) {
-#pragma unroll 4
-                    for (int i = t0; i < n4; i += 128) {
-                        const float4 v = reinterpret_cast<const float4*>(big)[i];
-                        reinterpret_cast<float4*>(low)[i] =
-                            make_float4(small_of(v.x), small_of(v.y), small_of(v.z), small_of(v.w));
-                    }
-                }
+                convert_tile<MODE, 128>(smem + stage * C::kStageBytes, smem + C::kSmallOffset + small * C::kStageBytes, t0,
+                                        1024 + col_boxes * 256, g.sum - kb * kBK, p.split3);
                 fence_proxy_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(conv_bar(small));
@@ -478,6 +483,334 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
     }
 }
 
+// ------------------------------------------------------------------ CTA pairs
+//
+// Groups with many rows: bound by the tensor cores, and on one SM by shared
+// memory, whose 128 bytes a clock the MMA (24 bytes per operand element and
+// product triple, with the copies and the converter) would need 1.5 times.  Two
+// CTAs share a tile of 256 lanes x 256 columns (cta_group::2): each stages
+// 128 lanes and half the columns, converts them itself, and holds its
+// lanes' accumulators; per byte staged the pair multiplies twice as much.
+// The epilogue's 128 totals a thread need more registers than an even
+// split gives: the other warps hand some over (setmaxnreg; the shares add up
+// to the launch's 512 x 128).
+
+struct GroupedPairCfg {
+    static constexpr int kCols = 256;
+    static constexpr int kLaneBytes = 128 * kBK * 4;
+    static constexpr int kColBytes = (kCols / 2) * kBK * 4;
+    static constexpr int kStageBytes = kLaneBytes + kColBytes;
+    static constexpr int kStages = 4, kSmall = 2;
+    static constexpr int kEpiWarps = 8, kConvWarps = 4;
+    static constexpr int kThreads = 512;              // epilogue, converter, and a warpgroup with TMA and MMA
+    static constexpr int kTmemCols = 512;
+    static constexpr int kTotals = 128;
+    static constexpr int kSmallOffset = kStages * kStageBytes;
+    static constexpr int kTableOffset = kSmallOffset + kSmall * kStageBytes;
+    static constexpr int kBarOffset = kTableOffset + 3 * MXB_MAX_GROUPS * 4 + 16;
+    static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;
+    static constexpr int kSmemBytes = 1024 + kBarOffset + kNumBars * 8 + 16;
+    static constexpr int kEpiRegs = 192, kConvRegs = 72, kIssueRegs = 56;
+    static_assert(2 * kEpiRegs + kConvRegs + kIssueRegs <= 512, "more registers than the launch has");
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+};
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThreads, 1)
+    grouped_pair_kernel(const __grid_constant__ CUtensorMap tm_lane, const __grid_constant__ CUtensorMap tm_col,
+                        const __grid_constant__ GroupedParams p) {
+    using C = GroupedPairCfg;
+    constexpr int BT = C::kCols;
+    constexpr bool kLaneMn = MODE != kGradA, kColMn = MODE == kGradB;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    GroupedTable& tab = *reinterpret_cast<GroupedTable*>(smem + C::kTableOffset);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const uint32_t bar0 = smem_addr(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };                         // TMA -> converter (own CTA)
+    auto empty_bar = [&](int s) { return bar0 + 8u * (C::kStages + s); };         // MMA -> TMA (both CTAs)
+    auto conv_bar = [&](int s) { return bar0 + 8u * (2 * C::kStages + s); };      // both converters -> MMA (leader)
+    auto sfree_bar = [&](int s) { return bar0 + 8u * (2 * C::kStages + C::kSmall + s); };  // MMA -> converter (both)
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + a); };
+    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 2 + a); };
+    const uint32_t drain_bar = bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    constexpr int kConvWarp = C::kEpiWarps, kTmaWarp = kConvWarp + C::kConvWarps, kMmaWarp = kTmaWarp + 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int s = 0; s < C::kSmall; ++s) {
+            mbar_init(conv_bar(s), 2 * C::kConvWarps);
+            mbar_init(sfree_bar(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), 2 * C::kEpiWarps);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tm_lane);
+        tma_prefetch_desc(&tm_col);
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc_pair(smem_addr(tmem_slot), C::kTmemCols);
+        tmem_relinquish_pair();
+    } else if (warp == kConvWarp) {
+        grouped_scan<MODE, BT>(tab, p, lane);
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // barriers initialised, TMEM allocated and the tables written in both CTAs
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = tab.total;
+    // The pair's columns are rounded up to 32: each CTA stages half of them.
+    auto half_cols = [](int cols) { return ((cols + 31) & ~31) / 2; };
+
+    if (warp >= kTmaWarp) {
+        fewer_registers<C::kIssueRegs>();
+        if (warp == kTmaWarp) {
+            // -------------------------------------------------------- TMA producer (both CTAs)
+            const bool leader = elect_one();
+            int stage = 0;
+            uint32_t phase = 0;
+            long long issued = 0;
+            bool ok = true;
+            for (int t = pair; t < total_tiles && ok; t += num_pairs) {
+                const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
+                const int half = half_cols(g.cols), col_boxes = (half + 31) / 32;
+                const int lane0 = g.lane0 + static_cast<int>(rank) * 128, col0 = g.col0 + static_cast<int>(rank) * half;
+                const int num_kb = (g.sum + kBK - 1) / kBK;
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    if (*abort_flag || !mbar_wait_cluster(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    if (leader) {
+                        const uint32_t st = smem_addr(smem + stage * C::kStageBytes), fb = full_bar(stage);
+                        mbar_arrive_expect_tx(fb, C::kLaneBytes + col_boxes * kBoxBytes);
+                        const int q0 = kb * kBK;
+                        if (MODE == kForward) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, lane0 + 32 * j, q0, g.group);
+                        } else if (MODE == kGradA) {
+                            tma_load_3d(st, &tm_lane, fb, q0, lane0, g.group);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                tma_load_2d(st + j * kBoxBytes, &tm_lane, fb, lane0 + 32 * j, g.row0 + q0);
+                        }
+                        for (int j = 0; j < col_boxes; ++j) {
+                            const uint32_t dst = st + C::kLaneBytes + j * kBoxBytes;
+                            if (MODE == kGradB) {
+                                tma_load_2d(dst, &tm_col, fb, col0 + 32 * j, g.row0 + q0);
+                            } else {
+                                tma_load_2d(dst, &tm_col, fb, q0, g.row0 + col0 + 32 * j);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                    ++issued;
+                    if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok && leader) {
+                raise_grouped(p, abort_flag, kErrProducer);
+                // Copies in flight land in this CTA's shared memory: wait for them before leaving.
+                for (long long i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
+                    mbar_wait(full_bar(static_cast<int>(i % C::kStages)), static_cast<uint32_t>((i / C::kStages) & 1),
+                              p.timeout_ns);
+            }
+            __syncwarp();
+        } else if (warp == kMmaWarp && rank == 0) {
+            // -------------------------------------------------------- MMA issuer (leader only)
+            constexpr uint32_t kHiMn = smem_desc_hi(512, kLayoutSW128Base32B), kHiK = smem_desc_hi(1024, kLayoutSW128);
+            constexpr uint32_t kLaneHi = kLaneMn ? kHiMn : kHiK, kColHi = kColMn ? kHiMn : kHiK;
+            constexpr uint32_t kLaneStep = kLaneMn ? 64 : 2, kColStep = kColMn ? 64 : 2;
+            const bool leader = elect_one();
+            int stage = 0, small = 0, acc = 0;
+            uint32_t small_phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int t = pair; t < total_tiles && ok; t += num_pairs) {
+                const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
+                const uint32_t idesc = idesc_tf32_major(256, 2 * half_cols(g.cols), kLaneMn, kColMn);
+                const int num_kb = (g.sum + kBK - 1) / kBK;
+                int in_seg = 0;
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    bool ready = *abort_flag == 0;
+                    if (ready && in_seg == 0) ready = mbar_wait_cluster(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
+                    if (!ready || !mbar_wait_cluster(conv_bar(small), small_phase, p.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const bool end_seg = ++in_seg == kGroupedSegKb || kb == num_kb - 1;
+                    if (leader) {
+                        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
+                        const uint32_t big = smem_addr(smem + stage * C::kStageBytes);
+                        const uint32_t low = smem_addr(smem + C::kSmallOffset + small * C::kStageBytes);
+                        const uint32_t bl = smem_desc_lo(big, kLaneMn ? kBoxBytes : 16);
+                        const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, kColMn ? kBoxBytes : 16);
+                        const uint32_t sl = smem_desc_lo(low, kLaneMn ? kBoxBytes : 16);
+                        const uint32_t sc = smem_desc_lo(low + C::kLaneBytes, kColMn ? kBoxBytes : 16);
+                        const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
+                        const uint32_t begun = in_seg > 1 ? 1u : 0u;
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            if (kk >= steps) break;
+                            const uint64_t da = smem_desc_of(kLaneHi, bl + kk * kLaneStep);
+                            const uint64_t db = smem_desc_of(kColHi, bc + kk * kColStep);
+                            if (p.split3) {
+                                // Small cross terms first, the dominant product last.
+                                mma_tf32_pair(d, da, smem_desc_of(kColHi, sc + kk * kColStep), idesc, kk ? 1u : begun);
+                                mma_tf32_pair(d, smem_desc_of(kLaneHi, sl + kk * kLaneStep), db, idesc, 1u);
+                                mma_tf32_pair(d, da, db, idesc, 1u);
+                            } else {
+                                mma_tf32_pair(d, da, db, idesc, kk ? 1u : begun);
+                            }
+                        }
+                        mma_commit_pair(empty_bar(stage), 0x3);
+                        mma_commit_pair(sfree_bar(small), 0x3);
+                        if (end_seg) mma_commit_pair(tfull_bar(acc), 0x3);
+                    }
+                    __syncwarp();
+                    if (++stage == C::kStages) stage = 0;
+                    if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+                    if (end_seg) {
+                        in_seg = 0;
+                        acc ^= 1;
+                        if (acc == 0) acc_phase ^= 1u;
+                    }
+                }
+            }
+            if (leader) {
+                if (!ok) raise_grouped(p, abort_flag, kErrMma);
+                mma_commit_pair(drain_bar, 0x1);
+                if (!mbar_wait_cluster(drain_bar, 0, p.timeout_ns)) raise_grouped(p, abort_flag, kErrMma);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= kConvWarp) {
+        // ------------------------------------------------------------ converter (each CTA its own half)
+        fewer_registers<C::kConvRegs>();
+        const int t0 = threadIdx.x - 32 * kConvWarp;
+        const uint32_t conv_leader = mapa_shared(conv_bar(0), 0);
+        int stage = 0, small = 0;
+        uint32_t phase = 0, small_phase = 0;
+        bool failed = false;
+        for (int t = pair; t < total_tiles && !failed; t += num_pairs) {
+            const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
+            const int col_boxes = (half_cols(g.cols) + 31) / 32;
+            const int num_kb = (g.sum + kBK - 1) / kBK;
+            for (int kb = 0; kb < num_kb; ++kb) {
+                const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
+                const bool got = !stop && mbar_wait(full_bar(stage), phase, p.timeout_ns) &&
+                                 mbar_wait_cluster(sfree_bar(small), small_phase ^ 1u, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0 && !stop) raise_grouped(p, abort_flag, kErrProducer);
+                    failed = true;
+                    break;
+                }
+                convert_tile<MODE, 128>(smem + stage * C::kStageBytes, smem + C::kSmallOffset + small * C::kStageBytes, t0,
+                                        1024 + col_boxes * 256, g.sum - kb * kBK, p.split3);
+                fence_proxy_async_shared();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(conv_leader + 8u * small);
+                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue (both CTAs, their own lanes)
+        more_registers<C::kEpiRegs>();
+        constexpr int W = 16;
+        const int quad = warp & 3, first_col = (warp >> 2) * C::kTotals;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + first_col;
+        const uint32_t tempty_leader = mapa_shared(tempty_bar(0), 0);
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool failed = false;
+        for (int t = pair; t < total_tiles && !failed; t += num_pairs) {
+            const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
+            const int num_kb = (g.sum + kBK - 1) / kBK;
+            float total[C::kTotals];
+#pragma unroll
+            for (int i = 0; i < C::kTotals; ++i) total[i] = 0.0f;
+            for (int k_begin = 0; k_begin < num_kb; k_begin += kGroupedSegKb) {
+                const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
+                const bool got = !stop && mbar_wait_cluster(tfull_bar(acc), acc_phase, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0 && !stop) raise_grouped(p, abort_flag, kErrEpilogue);
+                    failed = true;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < C::kTotals; c += W) {
+                    if (first_col + c < g.cols) {
+                        uint32_t r[W];
+                        tmem_ld_32x32b_x16(lane_base + static_cast<uint32_t>(acc * BT + c), r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < W; ++i) total[c + i] += __uint_as_float(r[i]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(tempty_leader + 8u * acc);
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+            if (failed) break;
+            const int col = g.lane0 + static_cast<int>(rank) * 128 + quad * 32 + lane;
+            if (col < p.lane_dim) {
+#pragma unroll
+                for (int c = 0; c < C::kTotals; c += W) {
+                    const int n = min(W, g.cols - first_col - c);
+                    if (n <= 0) continue;
+                    float v[W];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) v[i] = total[c + i];
+                    const long long row = g.col0 + first_col + c + (MODE == kGradB ? 0 : g.row0);
+                    if (MODE != kGradB) apply_column<W>(v, row, n, col, g.group, p.epi);
+                    float* dst = p.out + row * p.ldo + col + (MODE == kGradB ? g.group * p.out_stride : 0);
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+                        if (i < n) __stcs(dst + i * p.ldo, v[i]);
+                }
+            }
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();  // no CTA leaves while its peer may still signal its barriers
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, C::kTmemCols);
+    }
+}
+
 // dbias[e, n] = the sum of dY[r, n] over group e's rows: 32 columns of one group to a block.
 __global__ void __launch_bounds__(1024) grouped_column_sums(const float* dy, long long ld, const int* offsets, int rows,
                                                             int N, float* dbias) {
@@ -514,6 +847,24 @@ bool grouped_map(CUtensorMap* map, const float* base, int groups, long long rows
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
+// The two tensor maps of a call; the lane side's box is 32 x 32 floats, or 128 rows of 32 in grad_a.
+template <int MODE>
+bool grouped_maps(const GroupedCall& g, bool round, CUtensorMap* lane, CUtensorMap* col) {
+    if (MODE == kGradB)
+        return grouped_map(lane, g.w, 0, g.rows, g.N, g.ldw, 0, kBK, true, round) &&
+               grouped_map(col, g.x, 0, g.rows, g.K, g.ldx, 0, kBK, true, round);
+    return grouped_map(lane, g.w, g.groups, g.K, g.N, g.ldw, g.w_stride, MODE == kForward ? kBK : 128, MODE == kForward,
+                       round) &&
+           grouped_map(col, g.x, 0, g.rows, MODE == kForward ? g.K : g.N, g.ldx, 0, 32, false, round);
+}
+
+// At most so many column tiles, whatever the offsets are: a part of a tile more for each group that has a row.
+template <int MODE>
+long long most_col_tiles(const GroupedCall& g, int cols) {
+    return MODE == kGradB ? static_cast<long long>((g.K + cols - 1) / cols) * g.groups
+                          : g.rows / cols + std::min(g.groups, g.rows);
+}
+
 template <int MODE, int BT>
 cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
     using C = GroupedCfg<BT>;
@@ -532,23 +883,61 @@ cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int
         }
     }
     CUtensorMap lane, col;
-    const bool rnd = !split3;
-    bool ok;
-    if (MODE == kGradB) {
-        ok = grouped_map(&lane, g.w, 0, g.rows, g.N, g.ldw, 0, kBK, true, rnd) &&
-             grouped_map(&col, g.x, 0, g.rows, g.K, g.ldx, 0, kBK, true, rnd);
-    } else {
-        ok = grouped_map(&lane, g.w, g.groups, g.K, g.N, g.ldw, g.w_stride, MODE == kForward ? kBK : 128,
-                         MODE == kForward, rnd) &&
-             grouped_map(&col, g.x, 0, g.rows, MODE == kForward ? g.K : g.N, g.ldx, 0, 32, false, rnd);
-    }
-    if (!ok) return cudaErrorInvalidValue;
+    if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
     p.lane_tiles = (p.lane_dim + 127) / 128;
-    // At most so many tiles, whatever the offsets are: a part of a tile more for each group that has a row.
-    const long long dim = MODE == kGradB ? static_cast<long long>((g.K + BT - 1) / BT) * g.groups
-                                         : g.rows / BT + std::min(g.groups, g.rows);
-    const int grid = static_cast<int>(std::min<long long>(dim * p.lane_tiles, num_sms));
+    const int grid = static_cast<int>(std::min<long long>(most_col_tiles<MODE>(g, BT) * p.lane_tiles, num_sms));
     kernel<<<grid, C::kThreads, C::kSmemBytes, stream>>>(lane, col, p);
+    note_launch();
+    return cudaGetLastError();
+}
+
+template <int MODE>
+cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
+    using C = GroupedPairCfg;
+    auto kernel = grouped_pair_kernel<MODE>;
+    static std::mutex mu;
+    static uint64_t configured = 0;
+    static int max_clusters[64] = {0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    int clusters = num_sms / 2;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (dev >= 64 || !(configured & (1ull << dev))) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+            if (e != cudaSuccess) return e;
+            cudaLaunchConfig_t cfg = {};
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = 2;
+            attr.val.clusterDim.y = 1;
+            attr.val.clusterDim.z = 1;
+            cfg.gridDim = dim3(2 * clusters, 1, 1);
+            cfg.blockDim = dim3(C::kThreads, 1, 1);
+            cfg.dynamicSmemBytes = C::kSmemBytes;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            int n = 0;
+            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+                cudaGetLastError();
+                n = clusters;
+            }
+            clusters = n;
+            if (dev < 64) {
+                max_clusters[dev] = n;
+                configured |= 1ull << dev;
+            }
+        } else {
+            clusters = max_clusters[dev];
+        }
+    }
+    CUtensorMap lane, col;
+    if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
+    p.lane_tiles = (p.lane_dim + 255) / 256;
+    const int pairs =
+        static_cast<int>(std::min<long long>(most_col_tiles<MODE>(g, C::kCols) * p.lane_tiles, clusters));
+    kernel<<<2 * pairs, C::kThreads, C::kSmemBytes, stream>>>(lane, col, p);
     note_launch();
     return cudaGetLastError();
 }
@@ -556,6 +945,8 @@ cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int
 template <int MODE>
 cudaError_t run_grouped_mode(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
     const int per_group = MODE == kGradB ? g.K : (g.rows + g.groups - 1) / g.groups;
+    static const char* force = getenv("GR_PAIR");
+    if (force ? force[0] == '1' : per_group > 160) return run_grouped_pair<MODE>(g, p, split3, num_sms, stream);
     return per_group <= 32 ? run_grouped<MODE, 32>(g, p, split3, num_sms, stream)
                            : run_grouped<MODE, 128>(g, p, split3, num_sms, stream);
 }
