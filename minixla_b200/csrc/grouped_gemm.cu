@@ -71,6 +71,8 @@ struct GroupedParams {
     CellEpilogue epi;
 };
 
+constexpr int kGroupedTableBytes = 20 * MXB_MAX_GROUPS + 128 * 4 + 16;
+
 // BT: tile columns, the most rows of a group (grad_b: columns of A) that one tile takes.
 template <int BT>
 struct GroupedCfg {
@@ -80,12 +82,17 @@ struct GroupedCfg {
     static constexpr int kStages = BT <= 32 ? 8 : 4;  // tiles as loaded
     static constexpr int kSmall = 2;                  // their small parts
     static constexpr int kEpiWarps = BT <= 32 ? 4 : 8;
-    static constexpr int kThreads = 32 * (kEpiWarps + 6);  // epilogue, 4 converter warps, TMA, MMA
+    static constexpr int kConvWarps = 8;
+    static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 4);  // and a warpgroup with TMA and MMA
+    // Registers a thread: what the launch gets, in shares of 128 threads (BT 128: 5 x 96, BT 32: 4 x 128).
+    static constexpr int kEpiRegs = BT <= 32 ? 128 : 144, kConvRegs = BT <= 32 ? 128 : 64, kIssueRegs = BT <= 32 ? 128 : 64;
+    static_assert(kEpiWarps / 4 * kEpiRegs + kConvWarps / 4 * kConvRegs + kIssueRegs <= (BT <= 32 ? 512 : 480),
+                  "more registers than the launch has");
     static constexpr int kTmemCols = 2 * BT;          // two segment buffers
     static constexpr int kTotals = BT * 4 / kEpiWarps;  // columns of one epilogue thread
     static constexpr int kSmallOffset = kStages * kStageBytes;
     static constexpr int kTableOffset = kSmallOffset + kSmall * kStageBytes;
-    static constexpr int kBarOffset = kTableOffset + 3 * MXB_MAX_GROUPS * 4 + 16;
+    static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
     static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;
     static constexpr int kSmemBytes = 1024 + kBarOffset + kNumBars * 8 + 16;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
@@ -120,12 +127,11 @@ __device__ __forceinline__ void convert_tile(uint8_t* big, uint8_t* low, int t0,
             if (((i >> 3) & 31) >= valid) src[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
     if (!split3) return;
-    // n4 is a multiple of 2 * THREADS: two float4s a step at least.
+    // n4 is a multiple of THREADS (256).
 #pragma unroll 4
-    for (int i = t0; i < n4; i += 2 * THREADS) {
-        const float4 v = src[i], w = src[i + THREADS];
+    for (int i = t0; i < n4; i += THREADS) {
+        const float4 v = src[i];
         dst[i] = make_float4(small_of(v.x), small_of(v.y), small_of(v.z), small_of(v.w));
-        dst[i + THREADS] = make_float4(small_of(w.x), small_of(w.y), small_of(w.z), small_of(w.w));
     }
 }
 
@@ -139,18 +145,25 @@ struct GroupedTile {
     int sum;      // length of the sum
 };
 
+// Which tile is which, written by each CTA from `offsets` at its start (every
+// CTA the same: the order below depends on nothing else).  A group's column
+// tiles are two entries, the whole tiles and the narrower last one; the entries
+// are ordered by the cost of a tile, dearest first, in quarter octaves.  The
+// CTAs (pairs) take tiles by their index, every other round backwards, so that
+// the cheap tiles at the end even out what the dear ones left.
 struct GroupedTable {
-    int first_tile[MXB_MAX_GROUPS];  // exclusive prefix sums of the groups' tiles
+    int first_tile[2 * MXB_MAX_GROUPS];             // of each entry: the tiles before it
+    unsigned short entry[2 * MXB_MAX_GROUPS];       // group * 2 + (0: whole tiles, 1: the last one)
     int row0[MXB_MAX_GROUPS], row1[MXB_MAX_GROUPS];
-    int total;
+    int classes[128];
+    int entries, total;
 };
-static_assert(sizeof(GroupedTable) <= 3 * MXB_MAX_GROUPS * 4 + 16, "table size");
+static_assert(sizeof(GroupedTable) <= kGroupedTableBytes && kGroupedTableBytes % 16 == 0, "table size");
 
-// Tile t: the last group whose first tile is <= t; inside a group the column
-// tiles vary fastest, so CTAs that run together share weights through L2.
+// Tile t: inside an entry the column tiles vary fastest, so CTAs that run together share weights through L2.
 template <int MODE, int BT, int LANES = 128>
 __device__ __forceinline__ GroupedTile grouped_tile(const GroupedTable& tab, int t, const GroupedParams& p) {
-    int lo = 0, hi = p.groups - 1;
+    int lo = 0, hi = tab.entries - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (tab.first_tile[mid] <= t) {
@@ -160,48 +173,120 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedTable& tab, int
         }
     }
     GroupedTile g;
-    g.group = lo;
-    g.row0 = tab.row0[lo];
-    const int rows = tab.row1[lo] - g.row0;
+    const int last = tab.entry[lo] & 1;
+    g.group = tab.entry[lo] >> 1;
+    g.row0 = tab.row0[g.group];
+    const int rows = tab.row1[g.group] - g.row0;
     const int dim = MODE == kGradB ? p.col_dim : rows;
-    const int col_tiles = (dim + BT - 1) / BT;
-    const int i = t - tab.first_tile[lo];
+    const int i = t - tab.first_tile[lo], whole = dim / BT, col_tiles = last ? 1 : whole;
     g.lane0 = i / col_tiles * LANES;
-    g.col0 = i % col_tiles * BT;
-    g.cols = min(BT, dim - g.col0);
+    g.col0 = (last ? whole : i % col_tiles) * BT;
+    g.cols = last ? dim - g.col0 : BT;
     g.sum = MODE == kGradB ? rows : p.sum_dim;
     return g;
+}
+
+// Tile of worker `me` of `n` in round `round`, or -1; -2 once no worker has one.
+__device__ __forceinline__ int grouped_turn(int round, int me, int n, int total) {
+    const long long first = static_cast<long long>(round) * n;
+    if (first >= total) return -2;
+    const long long t = first + (round & 1 ? n - 1 - me : me);
+    return t < total ? static_cast<int>(t) : -1;
 }
 
 // Fills the table (one warp): group e's rows are clamped to 0 <= row0 <= row1 <= rows.
 template <int MODE, int BT>
 __device__ __forceinline__ void grouped_scan(GroupedTable& tab, const GroupedParams& p, int lane) {
-    int base = 0;
-    for (int e0 = 0; e0 < p.groups; e0 += 32) {
-        const int e = e0 + lane;
-        int tiles = 0;
-        if (e < p.groups) {
-            const int r0 = min(max(__ldg(p.offsets + e), 0), p.rows);
-            const int r1 = min(max(__ldg(p.offsets + e + 1), r0), p.rows);
+    for (int c = lane; c < 128; c += 32) tab.classes[c] = 0;
+    __syncwarp();
+    // Entry i = 2 e + part: how many column tiles it has, and its class (127 - 4 log2(cost) or so; -1: no tile).
+    auto look = [&](int i, int& tiles) -> int {
+        tiles = 0;
+        const int e = i >> 1;
+        if (e >= p.groups) return -1;
+        const int r0 = min(max(__ldg(p.offsets + e), 0), p.rows);
+        const int r1 = min(max(__ldg(p.offsets + e + 1), r0), p.rows);
+        if ((i & 1) == 0) {
             tab.row0[e] = r0;
             tab.row1[e] = r1;
-            tiles = ((MODE == kGradB ? p.col_dim : r1 - r0) + BT - 1) / BT * p.lane_tiles;
         }
-        int sum = tiles;
+        const int dim = MODE == kGradB ? p.col_dim : r1 - r0;
+        const int cols = i & 1 ? dim % BT : BT;
+        tiles = i & 1 ? (cols ? 1 : 0) : dim / BT;
+        if (!tiles) return -1;
+        const unsigned cost = static_cast<unsigned>((cols + 15) / 16) *
+                              static_cast<unsigned>(MODE == kGradB ? (r1 - r0) / kBK + 1 : 1);
+        const int octave = 31 - __clz(cost);
+        return 127 - (octave * 4 + static_cast<int>(octave >= 2 ? (cost >> (octave - 2)) & 3 : (cost << (2 - octave)) & 3));
+    };
+    const int n = 2 * p.groups;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        int tiles;
+        const int c = look(i0 + lane, tiles);
+        const unsigned same = __match_any_sync(0xffffffffu, c);
+        if (c >= 0 && lane == __ffs(same) - 1) tab.classes[c] += __popc(same);
+        __syncwarp();
+    }
+    // Classes' first places, by an exclusive scan of four counts a lane.
+    int count[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        count[j] = sum;
+        sum += tab.classes[4 * lane + j];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) tab.classes[4 * lane + j] = upto - sum + count[j];
+    const int entries = __shfl_sync(0xffffffffu, upto, 31);
+    __syncwarp();
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        int tiles;
+        const int c = look(i0 + lane, tiles);
+        const unsigned same = __match_any_sync(0xffffffffu, c);
+        const int place = c >= 0 ? tab.classes[c] + __popc(same & ((1u << lane) - 1)) : 0;
+        __syncwarp();
+        if (c >= 0) {
+            tab.entry[place] = static_cast<unsigned short>(i0 + lane);
+            tab.first_tile[place] = tiles * p.lane_tiles;
+            if (lane == __ffs(same) - 1) tab.classes[c] += __popc(same);
+        }
+        __syncwarp();
+    }
+    int base = 0;
+    for (int i0 = 0; i0 < entries; i0 += 32) {
+        const int tiles = i0 + lane < entries ? tab.first_tile[i0 + lane] : 0;
+        int inclusive = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
+            const int v = __shfl_up_sync(0xffffffffu, inclusive, o);
+            if (lane >= o) inclusive += v;
         }
-        if (e < p.groups) tab.first_tile[e] = base + sum - tiles;
-        base += __shfl_sync(0xffffffffu, sum, 31);
+        if (i0 + lane < entries) tab.first_tile[i0 + lane] = base + inclusive - tiles;
+        base += __shfl_sync(0xffffffffu, inclusive, 31);
     }
-    if (lane == 0) tab.total = base;
+    if (lane == 0) {
+        tab.entries = entries;
+        tab.total = base;
+    }
 }
 
 __device__ __forceinline__ void raise_grouped(const GroupedParams& p, volatile int* abort_flag, int bit) {
     atomicOr(p.err, bit);
     *abort_flag = 1;
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 constexpr int kGroupedSegKb = 2;  // k-blocks (of 32) to an accumulator
@@ -230,7 +315,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
     const uint32_t drain_bar = bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 4);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int kConvWarp = C::kEpiWarps, kTmaWarp = C::kEpiWarps + 4, kMmaWarp = C::kEpiWarps + 5;
+    constexpr int kConvWarp = C::kEpiWarps, kTmaWarp = kConvWarp + C::kConvWarps, kMmaWarp = kTmaWarp + 1;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::kStages; ++s) {
@@ -238,7 +323,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
             mbar_init(empty_bar(s), 1);
         }
         for (int s = 0; s < C::kSmall; ++s) {
-            mbar_init(conv_bar(s), 4);
+            mbar_init(conv_bar(s), C::kConvWarps);
             mbar_init(sfree_bar(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -263,136 +348,149 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = tab.total;
 
-    if (warp == kTmaWarp) {
-        // ------------------------------------------------------------ TMA producer
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            long long issued = 0;
+    if (warp >= kTmaWarp) {
+        if constexpr (BT > 32) fewer_registers<C::kIssueRegs>();
+        if (warp == kTmaWarp) {
+            // ------------------------------------------------------------ TMA producer
+            if (lane == 0) {
+                int stage = 0;
+                uint32_t phase = 0;
+                long long issued = 0;
+                bool ok = true;
+                for (int round = 0; ok; ++round) {
+                    const int t = grouped_turn(round, blockIdx.x, gridDim.x, total_tiles);
+                    if (t == -2) break;
+                    if (t < 0) continue;
+                    const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+                    const int col_boxes = (g.cols + 31) / 32;
+                    const int num_kb = (g.sum + kBK - 1) / kBK;
+                    for (int kb = 0; kb < num_kb; ++kb) {
+                        if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
+                            raise_grouped(p, abort_flag, kErrProducer);
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t st = smem_addr(smem + stage * C::kStageBytes);
+                        const uint32_t fb = full_bar(stage);
+                        mbar_arrive_expect_tx(fb, C::kLaneBytes + col_boxes * kBoxBytes);
+                        const int q0 = kb * kBK;
+                        if (MODE == kForward) {
+    #pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, q0, g.group);
+                        } else if (MODE == kGradA) {
+                            tma_load_3d(st, &tm_lane, fb, q0, g.lane0, g.group);
+                        } else {
+    #pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                tma_load_2d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, g.row0 + q0);
+                        }
+                        for (int j = 0; j < col_boxes; ++j) {
+                            const uint32_t dst = st + C::kLaneBytes + j * kBoxBytes;
+                            if (MODE == kGradB) {
+                                tma_load_2d(dst, &tm_col, fb, g.col0 + 32 * j, g.row0 + q0);
+                            } else {
+                                tma_load_2d(dst, &tm_col, fb, q0, g.row0 + g.col0 + 32 * j);
+                            }
+                        }
+                        ++issued;
+                        if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                    }
+                }
+                if (!ok) {
+                    // Copies in flight land in this CTA's shared memory: wait for them before leaving.
+                    const long long n = issued < C::kStages ? issued : C::kStages;
+                    for (long long i = 1; i <= n; ++i) {
+                        const long long idx = issued - i;
+                        mbar_wait(full_bar(static_cast<int>(idx % C::kStages)),
+                                  static_cast<uint32_t>((idx / C::kStages) & 1), p.timeout_ns);
+                    }
+                }
+            }
+        } else if (warp == kMmaWarp) {
+            // ------------------------------------------------------------ MMA issuer
+            // K-major operand: 32 bytes of a 128-byte row for each 8 of the sum; MN-major: 8 rows of 128 bytes.
+            constexpr uint32_t kHiMn = smem_desc_hi(512, kLayoutSW128Base32B), kHiK = smem_desc_hi(1024, kLayoutSW128);
+            constexpr uint32_t kLaneHi = kLaneMn ? kHiMn : kHiK, kColHi = kColMn ? kHiMn : kHiK;
+            constexpr uint32_t kLaneStep = kLaneMn ? 64 : 2, kColStep = kColMn ? 64 : 2;
+            const bool leader = elect_one();
+            int stage = 0, small = 0, acc = 0;
+            uint32_t phase = 0, small_phase = 0, acc_phase = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
+            for (int round = 0; ok; ++round) {
+                    const int t = grouped_turn(round, blockIdx.x, gridDim.x, total_tiles);
+                    if (t == -2) break;
+                    if (t < 0) continue;
                 const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
-                const int col_boxes = (g.cols + 31) / 32;
+                const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, kLaneMn, kColMn);
                 const int num_kb = (g.sum + kBK - 1) / kBK;
+                int in_seg = 0;
                 for (int kb = 0; kb < num_kb; ++kb) {
-                    if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
-                        raise_grouped(p, abort_flag, kErrProducer);
+                    bool ready = *abort_flag == 0;
+                    if (ready && in_seg == 0) ready = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
+                    if (!ready || !mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
+                        !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t st = smem_addr(smem + stage * C::kStageBytes);
-                    const uint32_t fb = full_bar(stage);
-                    mbar_arrive_expect_tx(fb, C::kLaneBytes + col_boxes * kBoxBytes);
-                    const int q0 = kb * kBK;
-                    if (MODE == kForward) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, q0, g.group);
-                    } else if (MODE == kGradA) {
-                        tma_load_3d(st, &tm_lane, fb, q0, g.lane0, g.group);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            tma_load_2d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, g.row0 + q0);
-                    }
-                    for (int j = 0; j < col_boxes; ++j) {
-                        const uint32_t dst = st + C::kLaneBytes + j * kBoxBytes;
-                        if (MODE == kGradB) {
-                            tma_load_2d(dst, &tm_col, fb, g.col0 + 32 * j, g.row0 + q0);
-                        } else {
-                            tma_load_2d(dst, &tm_col, fb, q0, g.row0 + g.col0 + 32 * j);
+                    tc_fence_after();
+                    const bool end_seg = ++in_seg == kGroupedSegKb || kb == num_kb - 1;
+                    if (leader) {
+                        const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
+                        const uint32_t big = smem_addr(smem + stage * C::kStageBytes);
+                        const uint32_t low = smem_addr(smem + C::kSmallOffset + small * C::kStageBytes);
+                        const uint32_t bl = smem_desc_lo(big, kLaneMn ? kBoxBytes : 16);
+                        const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, kColMn ? kBoxBytes : 16);
+                        const uint32_t sl = smem_desc_lo(low, kLaneMn ? kBoxBytes : 16);
+                        const uint32_t sc = smem_desc_lo(low + C::kLaneBytes, kColMn ? kBoxBytes : 16);
+                        // The last k-block ends with its own eighth: nothing past the sum is multiplied.
+                        const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
+                        const uint32_t begun = in_seg > 1 ? 1u : 0u;
+    #pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            if (kk >= steps) break;
+                            const uint64_t da = smem_desc_of(kLaneHi, bl + kk * kLaneStep);
+                            const uint64_t db = smem_desc_of(kColHi, bc + kk * kColStep);
+                            if (p.split3) {
+                                // Small cross terms first, the dominant product last.
+                                mma_tf32(d, da, smem_desc_of(kColHi, sc + kk * kColStep), idesc, kk ? 1u : begun);
+                                mma_tf32(d, smem_desc_of(kLaneHi, sl + kk * kLaneStep), db, idesc, 1u);
+                                mma_tf32(d, da, db, idesc, 1u);
+                            } else {
+                                mma_tf32(d, da, db, idesc, kk ? 1u : begun);
+                            }
                         }
+                        mma_commit(empty_bar(stage));
+                        mma_commit(sfree_bar(small));
+                        if (end_seg) mma_commit(tfull_bar(acc));
                     }
-                    ++issued;
                     if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
-                }
-            }
-            if (!ok) {
-                // Copies in flight land in this CTA's shared memory: wait for them before leaving.
-                const long long n = issued < C::kStages ? issued : C::kStages;
-                for (long long i = 1; i <= n; ++i) {
-                    const long long idx = issued - i;
-                    mbar_wait(full_bar(static_cast<int>(idx % C::kStages)),
-                              static_cast<uint32_t>((idx / C::kStages) & 1), p.timeout_ns);
-                }
-            }
-        }
-    } else if (warp == kMmaWarp) {
-        // ------------------------------------------------------------ MMA issuer
-        // K-major operand: 32 bytes of a 128-byte row for each 8 of the sum; MN-major: 8 rows of 128 bytes.
-        constexpr uint32_t kHiMn = smem_desc_hi(512, kLayoutSW128Base32B), kHiK = smem_desc_hi(1024, kLayoutSW128);
-        constexpr uint32_t kLaneHi = kLaneMn ? kHiMn : kHiK, kColHi = kColMn ? kHiMn : kHiK;
-        constexpr uint32_t kLaneStep = kLaneMn ? 64 : 2, kColStep = kColMn ? 64 : 2;
-        const bool leader = elect_one();
-        int stage = 0, small = 0, acc = 0;
-        uint32_t phase = 0, small_phase = 0, acc_phase = 0;
-        bool ok = true;
-        for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
-            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
-            const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, kLaneMn, kColMn);
-            const int num_kb = (g.sum + kBK - 1) / kBK;
-            int in_seg = 0;
-            for (int kb = 0; kb < num_kb; ++kb) {
-                bool ready = *abort_flag == 0;
-                if (ready && in_seg == 0) ready = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
-                if (!ready || !mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
-                    !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const bool end_seg = ++in_seg == kGroupedSegKb || kb == num_kb - 1;
-                if (leader) {
-                    const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
-                    const uint32_t big = smem_addr(smem + stage * C::kStageBytes);
-                    const uint32_t low = smem_addr(smem + C::kSmallOffset + small * C::kStageBytes);
-                    const uint32_t bl = smem_desc_lo(big, kLaneMn ? kBoxBytes : 16);
-                    const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, kColMn ? kBoxBytes : 16);
-                    const uint32_t sl = smem_desc_lo(low, kLaneMn ? kBoxBytes : 16);
-                    const uint32_t sc = smem_desc_lo(low + C::kLaneBytes, kColMn ? kBoxBytes : 16);
-                    // The last k-block ends with its own eighth: nothing past the sum is multiplied.
-                    const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
-                    const uint32_t begun = in_seg > 1 ? 1u : 0u;
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        if (kk >= steps) break;
-                        const uint64_t da = smem_desc_of(kLaneHi, bl + kk * kLaneStep);
-                        const uint64_t db = smem_desc_of(kColHi, bc + kk * kColStep);
-                        if (p.split3) {
-                            // Small cross terms first, the dominant product last.
-                            mma_tf32(d, da, smem_desc_of(kColHi, sc + kk * kColStep), idesc, kk ? 1u : begun);
-                            mma_tf32(d, smem_desc_of(kLaneHi, sl + kk * kLaneStep), db, idesc, 1u);
-                            mma_tf32(d, da, db, idesc, 1u);
-                        } else {
-                            mma_tf32(d, da, db, idesc, kk ? 1u : begun);
-                        }
+                    if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+                    if (end_seg) {
+                        in_seg = 0;
+                        acc ^= 1;
+                        if (acc == 0) acc_phase ^= 1u;
                     }
-                    mma_commit(empty_bar(stage));
-                    mma_commit(sfree_bar(small));
-                    if (end_seg) mma_commit(tfull_bar(acc));
-                }
-                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
-                if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
-                if (end_seg) {
-                    in_seg = 0;
-                    acc ^= 1;
-                    if (acc == 0) acc_phase ^= 1u;
                 }
             }
+            if (leader) {
+                if (!ok) raise_grouped(p, abort_flag, kErrMma);
+                mma_commit(drain_bar);
+                if (!mbar_wait(drain_bar, 0, p.timeout_ns)) raise_grouped(p, abort_flag, kErrMma);
+            }
+            __syncwarp();
         }
-        if (leader) {
-            if (!ok) raise_grouped(p, abort_flag, kErrMma);
-            mma_commit(drain_bar);
-            if (!mbar_wait(drain_bar, 0, p.timeout_ns)) raise_grouped(p, abort_flag, kErrMma);
-        }
-        __syncwarp();
     } else if (warp >= kConvWarp) {
-        // ------------------------------------------------------------ converter (4 warps)
+        if constexpr (BT > 32) fewer_registers<C::kConvRegs>();
+        // ------------------------------------------------------------ converter
         const int t0 = threadIdx.x - 32 * kConvWarp;
         int stage = 0, small = 0;
         uint32_t phase = 0, small_phase = 0;
         bool failed = false;
-        for (int t = blockIdx.x; t < total_tiles && !failed; t += gridDim.x) {
+        for (int round = 0; !failed; ++round) {
+                const int t = grouped_turn(round, blockIdx.x, gridDim.x, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
             const int col_boxes = (g.cols + 31) / 32;
             const int num_kb = (g.sum + kBK - 1) / kBK;
@@ -405,7 +503,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                     failed = true;
                     break;
                 }
-                convert_tile<MODE, 128>(smem + stage * C::kStageBytes, smem + C::kSmallOffset + small * C::kStageBytes, t0,
+                convert_tile<MODE, 32 * C::kConvWarps>(smem + stage * C::kStageBytes, smem + C::kSmallOffset + small * C::kStageBytes, t0,
                                         1024 + col_boxes * 256, g.sum - kb * kBK, p.split3);
                 fence_proxy_async_shared();
                 __syncwarp();
@@ -416,6 +514,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         }
     } else {
         // ------------------------------------------------------------ epilogue
+        if constexpr (BT > 32) more_registers<C::kEpiRegs>();
         constexpr int W = 16;
         const int quad = warp & 3;
         const int first_col = (warp >> 2) * C::kTotals;
@@ -423,7 +522,10 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         bool failed = false;
-        for (int t = blockIdx.x; t < total_tiles && !failed; t += gridDim.x) {
+        for (int round = 0; !failed; ++round) {
+                const int t = grouped_turn(round, blockIdx.x, gridDim.x, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
             const int num_kb = (g.sum + kBK - 1) / kBK;
             float total[C::kTotals];
@@ -493,7 +595,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
 // lanes' accumulators; per byte staged the pair multiplies twice as much.
 // The epilogue's 128 totals a thread need more registers than an even
 // split gives: the other warps hand some over (setmaxnreg; the shares add up
-// to the launch's 512 x 128).
+// to the launch's 640 x 96).
 
 struct GroupedPairCfg {
     static constexpr int kCols = 256;
@@ -501,28 +603,19 @@ struct GroupedPairCfg {
     static constexpr int kColBytes = (kCols / 2) * kBK * 4;
     static constexpr int kStageBytes = kLaneBytes + kColBytes;
     static constexpr int kStages = 4, kSmall = 2;
-    static constexpr int kEpiWarps = 8, kConvWarps = 4;
-    static constexpr int kThreads = 512;              // epilogue, converter, and a warpgroup with TMA and MMA
+    static constexpr int kEpiWarps = 8, kConvWarps = 8;
+    static constexpr int kThreads = 640;              // epilogue, converter, and a warpgroup with TMA and MMA
     static constexpr int kTmemCols = 512;
     static constexpr int kTotals = 128;
     static constexpr int kSmallOffset = kStages * kStageBytes;
     static constexpr int kTableOffset = kSmallOffset + kSmall * kStageBytes;
-    static constexpr int kBarOffset = kTableOffset + 3 * MXB_MAX_GROUPS * 4 + 16;
+    static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
     static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;
     static constexpr int kSmemBytes = 1024 + kBarOffset + kNumBars * 8 + 16;
-    static constexpr int kEpiRegs = 192, kConvRegs = 72, kIssueRegs = 56;
-    static_assert(2 * kEpiRegs + kConvRegs + kIssueRegs <= 512, "more registers than the launch has");
+    static constexpr int kEpiRegs = 168, kConvRegs = 48, kIssueRegs = 48;
+    static_assert(2 * kEpiRegs + 2 * kConvRegs + kIssueRegs <= 480, "more registers than the launch has");
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
-
-template <int N>
-__device__ __forceinline__ void more_registers() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
 
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThreads, 1)
@@ -595,7 +688,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             uint32_t phase = 0;
             long long issued = 0;
             bool ok = true;
-            for (int t = pair; t < total_tiles && ok; t += num_pairs) {
+            for (int round = 0; ok; ++round) {
+                const int t = grouped_turn(round, pair, num_pairs, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
                 const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
                 const int half = half_cols(g.cols), col_boxes = (half + 31) / 32;
                 const int lane0 = g.lane0 + static_cast<int>(rank) * 128, col0 = g.col0 + static_cast<int>(rank) * half;
@@ -651,7 +747,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             int stage = 0, small = 0, acc = 0;
             uint32_t small_phase = 0, acc_phase = 0;
             bool ok = true;
-            for (int t = pair; t < total_tiles && ok; t += num_pairs) {
+            for (int round = 0; ok; ++round) {
+                const int t = grouped_turn(round, pair, num_pairs, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
                 const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
                 const uint32_t idesc = idesc_tf32_major(256, 2 * half_cols(g.cols), kLaneMn, kColMn);
                 const int num_kb = (g.sum + kBK - 1) / kBK;
@@ -718,7 +817,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
         int stage = 0, small = 0;
         uint32_t phase = 0, small_phase = 0;
         bool failed = false;
-        for (int t = pair; t < total_tiles && !failed; t += num_pairs) {
+        for (int round = 0; !failed; ++round) {
+                const int t = grouped_turn(round, pair, num_pairs, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
             const int col_boxes = (half_cols(g.cols) + 31) / 32;
             const int num_kb = (g.sum + kBK - 1) / kBK;
@@ -731,11 +833,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
                     failed = true;
                     break;
                 }
-                convert_tile<MODE, 128>(smem + stage * C::kStageBytes, smem + C::kSmallOffset + small * C::kStageBytes, t0,
+                convert_tile<MODE, 32 * C::kConvWarps>(smem + stage * C::kStageBytes, smem + C::kSmallOffset + small * C::kStageBytes, t0,
                                         1024 + col_boxes * 256, g.sum - kb * kBK, p.split3);
                 fence_proxy_async_shared();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(conv_leader + 8u * small);
+                if (lane == 0) mbar_arrive_peer(conv_leader + 8u * small);
                 if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
                 if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
             }
@@ -750,7 +852,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
         int acc = 0;
         uint32_t acc_phase = 0;
         bool failed = false;
-        for (int t = pair; t < total_tiles && !failed; t += num_pairs) {
+        for (int round = 0; !failed; ++round) {
+                const int t = grouped_turn(round, pair, num_pairs, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
             const int num_kb = (g.sum + kBK - 1) / kBK;
             float total[C::kTotals];

@@ -329,6 +329,15 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// The same for writes that the arriving thread has already published to the
+// async proxy (fence_proxy_async_shared): what the barrier guards is read by
+// the pair's MMA from the shared memory of the CTA that wrote it, so no release
+// at cluster scope -- which stalls the thread for about a thousand clocks -- is
+// needed on top.
+__device__ __forceinline__ void mbar_arrive_peer(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
