@@ -79,15 +79,14 @@ struct GroupedCfg {
     static constexpr int kLaneBytes = 128 * kBK * 4;
     static constexpr int kColBytes = BT * kBK * 4;
     static constexpr int kStageBytes = kLaneBytes + kColBytes;
-    static constexpr int kStages = BT <= 32 ? 8 : 4;  // tiles as loaded
+    static constexpr int kStages = 4;                 // tiles as loaded
     static constexpr int kSmall = 2;                  // their small parts
-    static constexpr int kEpiWarps = BT <= 32 ? 4 : 8;
+    static constexpr int kEpiWarps = 8;
     static constexpr int kConvWarps = 8;
     static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 4);  // and a warpgroup with TMA and MMA
-    // Registers a thread: what the launch gets, in shares of 128 threads (BT 128: 5 x 96, BT 32: 4 x 128).
-    static constexpr int kEpiRegs = BT <= 32 ? 128 : 144, kConvRegs = BT <= 32 ? 128 : 64, kIssueRegs = BT <= 32 ? 128 : 64;
-    static_assert(kEpiWarps / 4 * kEpiRegs + kConvWarps / 4 * kConvRegs + kIssueRegs <= (BT <= 32 ? 512 : 480),
-                  "more registers than the launch has");
+    // Registers a thread: the launch has 640 x 96, given out in shares of 128 threads.
+    static constexpr int kEpiRegs = 144, kConvRegs = 64, kIssueRegs = 64;
+    static_assert(2 * kEpiRegs + 2 * kConvRegs + kIssueRegs <= 480, "more registers than the launch has");
     static constexpr int kTmemCols = 2 * BT;          // two segment buffers
     static constexpr int kTotals = BT * 4 / kEpiWarps;  // columns of one epilogue thread
     static constexpr int kSmallOffset = kStages * kStageBytes;
@@ -349,7 +348,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
     const int total_tiles = tab.total;
 
     if (warp >= kTmaWarp) {
-        if constexpr (BT > 32) fewer_registers<C::kIssueRegs>();
+        fewer_registers<C::kIssueRegs>();
         if (warp == kTmaWarp) {
             // ------------------------------------------------------------ TMA producer
             if (lane == 0) {
@@ -481,7 +480,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
             __syncwarp();
         }
     } else if (warp >= kConvWarp) {
-        if constexpr (BT > 32) fewer_registers<C::kConvRegs>();
+        fewer_registers<C::kConvRegs>();
         // ------------------------------------------------------------ converter
         const int t0 = threadIdx.x - 32 * kConvWarp;
         int stage = 0, small = 0;
@@ -514,7 +513,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         }
     } else {
         // ------------------------------------------------------------ epilogue
-        if constexpr (BT > 32) more_registers<C::kEpiRegs>();
+        more_registers<C::kEpiRegs>();
         constexpr int W = 16;
         const int quad = warp & 3;
         const int first_col = (warp >> 2) * C::kTotals;
@@ -577,6 +576,371 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         }
     }
 
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, C::kTmemCols);
+    }
+}
+
+// ------------------------------------------------------------------ few rows per group
+//
+// Groups with a handful of rows: bound by the weights' bytes.  What stands
+// between a weight and HBM's rate is shared memory: every pass over the 128 x
+// 32 tile costs 16 KB of its 128 bytes a clock.  So the tile is read as little
+// as possible: by the MMA once for big, against big and small activations side
+// by side (columns 0 .. n and n .. 2n of one MMA), and once by the
+// converter, a thread to a weight column, which leaves the small parts in
+// tensor memory, from where the second MMA takes them as its A operand.
+// That is 72 KB a k-block (of 32) where the kernel above moves 120.
+//
+// With fewer tiles than SMs, a cluster of `splits` CTAs shares a tile, each
+// summing its own stretch of the sum; the totals meet in distributed shared
+// memory, added in CTA order.
+
+struct GroupedFewCfg {
+    static constexpr int kCols = 32;                  // rows of the group per tile
+    static constexpr int kLaneBytes = 128 * kBK * 4;
+    static constexpr int kColBytes = 2 * kCols * kBK * 4;  // activations, then their small parts
+    static constexpr int kStageBytes = kLaneBytes + kColBytes;
+    static constexpr int kStages = 8;
+    static constexpr int kSmall = 4;                  // small weights in tensor memory: 32 columns each
+    static constexpr int kEpiWarps = 4, kConvWarps = 8;
+    static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 2);
+    static constexpr int kSmallCol = 4 * kCols;       // first TMEM column behind the two accumulators of 64
+    static constexpr int kTmemCols = 256;
+    static constexpr int kSegKb = 4;                  // k-blocks to an accumulator: 32 sums into each column
+    static constexpr int kTableOffset = kStages * kStageBytes;
+    static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
+    static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;
+    static constexpr int kSmemBytes = 1024 + kBarOffset + kNumBars * 8 + 16;
+    static constexpr int kMaxSplits = 8;
+    static_assert(kSmallCol + 32 * kSmall <= kTmemCols, "tensor memory");
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
+};
+
+template <int MODE>
+__global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
+    grouped_few_kernel(const __grid_constant__ CUtensorMap tm_lane, const __grid_constant__ CUtensorMap tm_col,
+                       const __grid_constant__ GroupedParams p, const int splits) {
+    using C = GroupedFewCfg;
+    static_assert(MODE != kGradB, "the rows are the columns here");
+    constexpr int BT = C::kCols;
+    constexpr bool kLaneMn = MODE == kForward;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    GroupedTable& tab = *reinterpret_cast<GroupedTable*>(smem + C::kTableOffset);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBarOffset);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const uint32_t bar0 = smem_addr(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (C::kStages + s); };
+    auto conv_bar = [&](int s) { return bar0 + 8u * (2 * C::kStages + s); };
+    auto sfree_bar = [&](int s) { return bar0 + 8u * (2 * C::kStages + C::kSmall + s); };
+    auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + a); };
+    auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 2 + a); };
+    const uint32_t drain_bar = bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 4);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // (the converter's warp w reads and writes TMEM lanes 32 (w % 4) ..: both roles start at a multiple of four)
+    constexpr int kConvWarp = C::kEpiWarps, kTmaWarp = kConvWarp + C::kConvWarps, kMmaWarp = kTmaWarp + 1;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int s = 0; s < C::kSmall; ++s) {
+            mbar_init(conv_bar(s), C::kConvWarps);
+            mbar_init(sfree_bar(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), C::kEpiWarps);
+        }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        tma_prefetch_desc(&tm_lane);
+        tma_prefetch_desc(&tm_col);
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
+        tmem_relinquish();
+    } else if (warp == kConvWarp) {
+        grouped_scan<MODE, BT>(tab, p, lane);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = tab.total;
+    const int team = blockIdx.x / splits, teams = gridDim.x / splits, rank = blockIdx.x - team * splits;
+    // This CTA's k-blocks [kb0, kb1) of every tile (all sums are as long as sum_dim).
+    const int all_kb = (p.sum_dim + kBK - 1) / kBK;
+    const int kb0 = static_cast<int>(static_cast<long long>(all_kb) * rank / splits);
+    const int kb1 = static_cast<int>(static_cast<long long>(all_kb) * (rank + 1) / splits);
+
+    if (warp == kTmaWarp) {
+        // ------------------------------------------------------------ TMA producer
+        const bool leader = elect_one();
+        int stage = 0;
+        uint32_t phase = 0;
+        long long issued = 0;
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+            const int t = grouped_turn(round, team, teams, total_tiles);
+            if (t == -2) break;
+            if (t < 0) continue;
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
+                    ok = false;
+                    break;
+                }
+                if (leader) {
+                    const uint32_t st = smem_addr(smem + stage * C::kStageBytes), fb = full_bar(stage);
+                    mbar_arrive_expect_tx(fb, C::kLaneBytes + kBoxBytes);
+                    const int q0 = kb * kBK;
+                    if (MODE == kForward) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, q0, g.group);
+                    } else {
+                        tma_load_3d(st, &tm_lane, fb, q0, g.lane0, g.group);
+                    }
+                    tma_load_2d(st + C::kLaneBytes, &tm_col, fb, q0, g.row0 + g.col0);
+                }
+                __syncwarp();
+                ++issued;
+                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+            }
+        }
+        if (!ok && leader) {
+            raise_grouped(p, abort_flag, kErrProducer);
+            // Copies in flight land in this CTA's shared memory: wait for them before leaving.
+            for (long long i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
+                mbar_wait(full_bar(static_cast<int>(i % C::kStages)), static_cast<uint32_t>((i / C::kStages) & 1),
+                          p.timeout_ns);
+        }
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
+        // ------------------------------------------------------------ MMA issuer
+        constexpr uint32_t kHiMn = smem_desc_hi(512, kLayoutSW128Base32B), kHiK = smem_desc_hi(1024, kLayoutSW128);
+        constexpr uint32_t kLaneHi = kLaneMn ? kHiMn : kHiK, kLaneStep = kLaneMn ? 64 : 2;
+        const bool leader = elect_one();
+        int stage = 0, small = 0, acc = 0;
+        uint32_t phase = 0, small_phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int round = 0; ok; ++round) {
+            const int t = grouped_turn(round, team, teams, total_tiles);
+            if (t == -2) break;
+            if (t < 0) continue;
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            const int n = (g.cols + 15) & ~15;
+            const uint32_t both = idesc_tf32_major(128, p.split3 ? 2 * n : n, kLaneMn, 0);
+            const uint32_t one = idesc_tf32_major(128, n, 0, 0);  // (A in tensor memory is K-major)
+            int in_seg = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                bool ready = *abort_flag == 0;
+                if (ready && in_seg == 0) ready = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
+                if (!ready || !mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
+                    !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const bool end_seg = ++in_seg == C::kSegKb || kb == kb1 - 1;
+                if (leader) {
+                    const uint32_t d = tmem_base + static_cast<uint32_t>(acc * 2 * BT);
+                    const uint32_t a_small = tmem_base + static_cast<uint32_t>(C::kSmallCol + 32 * small);
+                    const uint32_t big = smem_addr(smem + stage * C::kStageBytes);
+                    const uint32_t bl = smem_desc_lo(big, kLaneMn ? kBoxBytes : 16);
+                    const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, 16);
+                    const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
+                    const uint32_t begun = in_seg > 1 ? 1u : 0u;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        if (kk >= steps) break;
+                        const uint64_t db = smem_desc_of(kHiK, bc + kk * 2);
+                        mma_tf32(d, smem_desc_of(kLaneHi, bl + kk * kLaneStep), db, both, kk ? 1u : begun);
+                        if (p.split3) mma_tf32_ts(d, a_small + kk * 8, db, one, 1u);
+                    }
+                    mma_commit(empty_bar(stage));
+                    mma_commit(sfree_bar(small));
+                    if (end_seg) mma_commit(tfull_bar(acc));
+                }
+                __syncwarp();
+                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+                if (end_seg) {
+                    in_seg = 0;
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1u;
+                }
+            }
+        }
+        if (leader) {
+            if (!ok) raise_grouped(p, abort_flag, kErrMma);
+            mma_commit(drain_bar);
+            if (!mbar_wait(drain_bar, 0, p.timeout_ns)) raise_grouped(p, abort_flag, kErrMma);
+        }
+        __syncwarp();
+    } else if (warp >= kConvWarp) {
+        // ------------------------------------------------------------ converter: a weight column and 16 k a thread
+        const int t0 = threadIdx.x - 32 * kConvWarp, row = t0 & 127, half = t0 >> 7;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(row & ~31) << 16) + C::kSmallCol + 16 * half;
+        int stage = 0, small = 0;
+        uint32_t phase = 0, small_phase = 0;
+        bool failed = false;
+        for (int round = 0; !failed; ++round) {
+            const int t = grouped_turn(round, team, teams, total_tiles);
+            if (t == -2) break;
+            if (t < 0) continue;
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            const int n = (g.cols + 15) & ~15;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
+                const bool got = !stop && mbar_wait(full_bar(stage), phase, p.timeout_ns) &&
+                                 mbar_wait(sfree_bar(small), small_phase ^ 1u, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0 && !stop) raise_grouped(p, abort_flag, kErrProducer);
+                    failed = true;
+                    break;
+                }
+                if (p.split3) {
+                    tc_fence_after();
+                    const uint8_t* st = smem + stage * C::kStageBytes;
+                    uint32_t r[16];
+                    if (kLaneMn) {
+                        // [k][n]: box n / 32, 128 bytes a k, its 32-byte chunks swizzled by k % 4.
+                        const uint8_t* src = st + (row >> 5) * kBoxBytes + half * 16 * 128 + (row & 7) * 4;
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            r[k] = __float_as_uint(small_of(
+                                *reinterpret_cast<const float*>(src + k * 128 + ((((row >> 3) & 3) ^ (k & 3)) << 5))));
+                    } else {
+                        // [n][k]: 128 bytes a weight column, 16-byte chunks swizzled by n % 8.
+                        const uint8_t* src = st + row * 128;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const float4 v = *reinterpret_cast<const float4*>(src + (((half * 4 + c) ^ (row & 7)) << 4));
+                            r[4 * c] = __float_as_uint(small_of(v.x));
+                            r[4 * c + 1] = __float_as_uint(small_of(v.y));
+                            r[4 * c + 2] = __float_as_uint(small_of(v.z));
+                            r[4 * c + 3] = __float_as_uint(small_of(v.w));
+                        }
+                    }
+                    tmem_st_32x32b_x16(lane_base + static_cast<uint32_t>(32 * small), r);
+                    // The activations' small parts go behind them, to rows n .. 2n of the same swizzled tile.
+                    float4* x = reinterpret_cast<float4*>(smem + stage * C::kStageBytes + C::kLaneBytes);
+                    const float4 v = x[t0];
+                    __syncwarp();
+                    if (t0 < n * 8) x[t0 + n * 8] = make_float4(small_of(v.x), small_of(v.y), small_of(v.z), small_of(v.w));
+                    tmem_st_wait();
+                    fence_proxy_async_shared();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(conv_bar(small));
+                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue: a result column and 32 rows a thread
+        constexpr int W = 16;
+        const int quad = warp & 3;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool failed = false;
+        for (int round = 0; !failed; ++round) {
+            const int t = grouped_turn(round, team, teams, total_tiles);
+            if (t == -2) break;
+            if (t < 0) continue;
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            const int n = (g.cols + 15) & ~15;
+            float total[BT];
+#pragma unroll
+            for (int i = 0; i < BT; ++i) total[i] = 0.0f;
+            for (int k_begin = kb0; k_begin < kb1; k_begin += C::kSegKb) {
+                const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
+                const bool got = !stop && mbar_wait(tfull_bar(acc), acc_phase, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0 && !stop) raise_grouped(p, abort_flag, kErrEpilogue);
+                    failed = true;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < BT; c += W) {
+                    if (c < n) {
+                        uint32_t r[W], s[W];
+                        tmem_ld_32x32b_x16(lane_base + static_cast<uint32_t>(acc * 2 * BT + c), r);
+                        if (p.split3) tmem_ld_32x32b_x16(lane_base + static_cast<uint32_t>(acc * 2 * BT + n + c), s);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < W; ++i)
+                            total[c + i] += p.split3 ? __uint_as_float(r[i]) + __uint_as_float(s[i]) : __uint_as_float(r[i]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tempty_bar(acc));
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1u;
+            }
+            if (failed) break;
+            const int col = g.lane0 + quad * 32 + lane;
+            if (splits > 1) {
+                // The one tile of this cluster: every copy and MMA of it is done, so stage 0 can hold the totals,
+                // [row][column].
+                float* share = reinterpret_cast<float*>(smem) + quad * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < BT; ++i) share[i * 128] = total[i];
+                continue;
+            }
+            if (col < p.lane_dim) {
+#pragma unroll
+                for (int c = 0; c < BT; c += W) {
+                    const int m = min(W, g.cols - c);
+                    if (m <= 0) continue;
+                    float v[W];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) v[i] = total[c + i];
+                    const long long row = g.row0 + g.col0 + c;
+                    apply_column<W>(v, row, m, col, g.group, p.epi);
+                    float* dst = p.out + row * p.ldo + col;
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+                        if (i < m) __stcs(dst + i * p.ldo, v[i]);
+                }
+            }
+        }
+    }
+
+    if (splits > 1) {
+        __syncwarp();
+        cluster_sync();  // the totals of every CTA of the tile are in place (or a CTA gave up)
+        if (team < total_tiles && *abort_flag == 0) {
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, team, p);
+            // Every thread an output, this CTA the rows rank, rank + splits, ...
+            const int share = (g.cols - rank + splits - 1) / splits;
+            for (int i = threadIdx.x; i < share * 128; i += C::kThreads) {
+                const int row = rank + (i >> 7) * splits, col = g.lane0 + (i & 127);
+                if (col >= p.lane_dim) continue;
+                const uint32_t at = smem_addr(smem) + static_cast<uint32_t>(row * 128 + (i & 127)) * 4;
+                float v = 0.0f;
+                for (int r = 0; r < splits; ++r) v += ld_shared_cluster_f32(mapa_shared(at, static_cast<uint32_t>(r)));
+                const long long out_row = g.row0 + g.col0 + row;
+                p.out[out_row * p.ldo + col] = apply_cell(v, out_row, col, g.group, p.epi);
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while another still reads its totals
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp) {
@@ -997,6 +1361,48 @@ cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int
 }
 
 template <int MODE>
+cudaError_t run_grouped_few(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
+    using C = GroupedFewCfg;
+    auto kernel = grouped_few_kernel<MODE>;
+    static std::mutex mu;
+    static uint64_t configured = 0;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (dev >= 64 || !(configured & (1ull << dev))) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+            if (e != cudaSuccess) return e;
+            if (dev < 64) configured |= 1ull << dev;
+        }
+    }
+    CUtensorMap lane, col;
+    if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
+    p.lane_tiles = (p.lane_dim + 127) / 128;
+    const long long tiles = most_col_tiles<MODE>(g, C::kCols) * p.lane_tiles;
+    // Splits while every cluster still has SMs of its own and every CTA at least two k-blocks.
+    const int all_kb = (p.sum_dim + kBK - 1) / kBK;
+    int splits = 1;
+    while (splits < C::kMaxSplits && 2 * splits * tiles <= num_sms && all_kb >= 4 * splits) splits *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = splits;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(splits > 1 ? tiles * splits : std::min<long long>(tiles, num_sms)), 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, lane, col, p, splits);
+    note_launch();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int MODE>
 cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
     using C = GroupedPairCfg;
     auto kernel = grouped_pair_kernel<MODE>;
@@ -1052,8 +1458,10 @@ cudaError_t run_grouped_mode(const GroupedCall& g, GroupedParams& p, bool split3
     const int per_group = MODE == kGradB ? g.K : (g.rows + g.groups - 1) / g.groups;
     static const char* force = getenv("GR_PAIR");
     if (force ? force[0] == '1' : per_group > 160) return run_grouped_pair<MODE>(g, p, split3, num_sms, stream);
-    return per_group <= 32 ? run_grouped<MODE, 32>(g, p, split3, num_sms, stream)
-                           : run_grouped<MODE, 128>(g, p, split3, num_sms, stream);
+    if constexpr (MODE != kGradB) {
+        if (per_group <= 32) return run_grouped_few<MODE>(g, p, split3, num_sms, stream);
+    }
+    return run_grouped<MODE, 128>(g, p, split3, num_sms, stream);
 }
 
 int grouped_gemm(const char* fn, GpuCtx* ctx, const GroupedCall& g, const mxb_ep_step* steps, int n_steps,
