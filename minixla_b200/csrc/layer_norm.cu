@@ -11,13 +11,19 @@
 // Bound by HBM: x in, y out (backward: x and dy in, dx out), each once.  A
 // row is held in registers between its sums and its output, by one warp up
 // to 1024 columns and by a block beyond; only rows longer than a block can
-// hold are read again (from L2).  The gradients of gamma and beta are summed
-// per thread over the rows its block walks through, then stored as one
-// partial row per block and summed by a second small kernel in block order,
-// so the result does not depend on timing.
+// hold are read again (from L2).  A block's rows arrive through a ring in shared
+// memory that bulk copies keep full: with loads by the threads themselves,
+// which can only be issued between a row's two barriers, the same kernels
+// reached 5.3 (forward) and 5.4 TB/s (backward).  The
+// gradients of gamma and beta are summed per thread over the rows its block
+// walks through, then stored as one partial row per block and summed by a
+// second small kernel in block order, so the result does not depend on timing.
+#include "gemm_common.cuh"
+
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <exception>
 
 #include "runtime_internal.h"
@@ -38,6 +44,8 @@ struct NormParams {
     float* rstd;
     long long rows;
     int cols;
+    unsigned long long timeout_ns;
+    int* err;
 };
 
 struct NormGradParams {
@@ -53,6 +61,8 @@ struct NormGradParams {
     float* partial;   // [block][2][cols]: dgamma, dbeta (nullptr: neither is wanted)
     long long rows;
     int cols;
+    unsigned long long timeout_ns;
+    int* err;
 };
 
 // W consecutive floats at p + c, zeros from column `cols` on.
@@ -128,55 +138,225 @@ struct RowSum {
     }
 };
 
+// ------------------------------------------------------------------ rows through shared memory
+//
+// A ring of slots, each for one row of up to two matrices, filled by bulk
+// copies that one thread asks for.  A copy starts and ends on 16-byte
+// boundaries, so it may bring up to three floats of the neighbouring rows (or of
+// the gap between them) along; a row whose copy would leave the matrix at
+// either end is read directly instead.
+
+constexpr int kMaxSlots = 8;
+
+struct RowSource {
+    const float* base;
+    long long ld;
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
+// Where a row's 16-byte aligned copy begins, how long it is, and whether it stays inside the matrix.
+struct RowSpan {
+    uintptr_t begin;
+    uint32_t bytes, skip;  // skip: floats before the row's first
+    bool inside;
+};
+
+__device__ __forceinline__ RowSpan row_span(const RowSource& m, long long row, long long rows, int cols) {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(m.base + row * m.ld);
+    const uintptr_t last = first + static_cast<uintptr_t>(cols) * 4;
+    RowSpan s;
+    s.begin = first & ~static_cast<uintptr_t>(15);
+    s.bytes = static_cast<uint32_t>(((last + 15) & ~static_cast<uintptr_t>(15)) - s.begin);
+    s.skip = static_cast<uint32_t>(first - s.begin) / 4;
+    s.inside = s.begin >= reinterpret_cast<uintptr_t>(m.base) &&
+               s.begin + s.bytes <= reinterpret_cast<uintptr_t>(m.base + (rows - 1) * m.ld + cols);
+    return s;
+}
+
+__host__ __device__ constexpr int row_slot_bytes(int cols) { return (cols * 4 + 12 + 15) / 16 * 16; }
+
+template <int MATS>
+struct RowRing {
+    RowSource mats[MATS];
+    uint8_t* slots;
+    uint32_t bar0;
+    int n, cols;
+    long long rows;
+
+    // Asks for `row` into `slot`; one thread.
+    __device__ __forceinline__ void ask(long long row, int slot) const {
+        const uint32_t bar = bar0 + 8 * slot, dst = smem_addr(slots) + slot * MATS * row_slot_bytes(cols);
+        RowSpan s[MATS];
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+            s[m] = row_span(mats[m], row, rows, cols);
+            bytes += s[m].inside ? s[m].bytes : 0;
+        }
+        mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+            if (s[m].inside)
+                bulk_load(dst + m * row_slot_bytes(cols), reinterpret_cast<const void*>(s[m].begin), s[m].bytes, bar);
+    }
+    // Where a thread finds matrix m's row: in its slot or, at the matrix's ends, where it lies.
+    __device__ __forceinline__ const float* find(int m, long long row, int slot) const {
+        const RowSpan s = row_span(mats[m], row, rows, cols);
+        if (!s.inside) return mats[m].base + row * mats[m].ld;
+        return reinterpret_cast<const float*>(slots + (slot * MATS + m) * row_slot_bytes(cols)) + s.skip;
+    }
+};
+
+// W consecutive floats at p + c of a row in a slot (generic address), zeros from column `cols` on.
+template <int W>
+__device__ __forceinline__ void take_unit(float (&v)[W], const float* p, int c, int cols) {
+    if (W == 4 && c + W <= cols) {
+        const float4 t = *reinterpret_cast<const float4*>(p + c);
+        v[0] = t.x;
+        v[W > 1 ? 1 : 0] = t.y;
+        v[W > 2 ? 2 : 0] = t.z;
+        v[W > 3 ? 3 : 0] = t.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = c + i < cols ? p[c + i] : 0.0f;
+    }
+}
+
 constexpr int kWarpRowThreads = 256;  // blocks of eight warps, a row each
 
-// Each thread holds NV units of W floats of its row, unit u at columns
-// (u * threads + t) * W.
-template <int W, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? kWarpRowThreads : 1024)
-    layer_norm_kernel(const NormParams p) {
-    __shared__ float2 buf[2][32];
-    RowSum<WARP> row_sum{buf};
-    const int threads = WARP ? 32 : blockDim.x;
-    const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const long long rows_at_once = static_cast<long long>(gridDim.x) * (WARP ? kWarpRowThreads / 32 : 1);
-    long long row = WARP ? blockIdx.x * static_cast<long long>(kWarpRowThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
+struct NormStats {
+    float mean, rstd;
+};
+
+// Mean and 1 / sqrt(var + eps) of a row that its threads hold in v; `sum` adds over them.
+template <int W, int NV, typename Sum>
+__device__ __forceinline__ NormStats norm_stats(const float (&v)[NV][W], int t, int threads, const NormParams& p, float inv,
+                                                Sum sum) {
+    float s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int i = 0; i < W; ++i) s += v[u][i];
+    NormStats st;
+    st.mean = sum(s) * inv;
+    s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float d = (u * threads + t) * W + i < p.cols ? v[u][i] - st.mean : 0.0f;
+            s += d * d;
+        }
+    st.rstd = 1.0f / sqrtf(sum(s) * inv + p.eps);
+    return st;
+}
+
+// gamma and beta of a thread's columns, in registers: the ring leaves L1 little room, and read again for every row
+// they took 16384 x 4096 from 88 to 114 us.  (The warp kernels, whose blocks leave L1 alone, read them from there
+// where a lane holds more than 16 columns.)
+template <int W, int NV, bool HELD>
+struct NormAffine {
+    static constexpr bool kHeld = HELD;
+    float g[kHeld ? NV : 1][W], b[kHeld ? NV : 1][W];
+    __device__ __forceinline__ NormAffine(const NormParams& p, int t, int threads) {
+        if constexpr (kHeld) {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) read(u, u, p, t, threads);
+        }
+    }
+    __device__ __forceinline__ void read(int into, int u, const NormParams& p, int t, int threads) {
+        load_param<W>(g[into], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
+        load_param<W>(b[into], p.beta, (u * threads + t) * W, p.cols, 0.0f);
+    }
+};
+
+template <int W, int NV, bool HELD>
+__device__ __forceinline__ void norm_out(float (&v)[NV][W], const NormStats& st, NormAffine<W, NV, HELD>& affine, int t, int threads,
+                                         long long row, const NormParams& p) {
+    if (t == 0) {
+        if (p.mean) p.mean[row] = st.mean;
+        if (p.rstd) p.rstd[row] = st.rstd;
+    }
+    float* y = p.y + row * p.ldy;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        const int at = HELD ? u : 0;
+        if constexpr (!HELD) affine.read(0, u, p, t, threads);
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[u][i] = (v[u][i] - st.mean) * st.rstd * affine.g[at][i] + affine.b[at][i];
+        store_unit<W>(v[u], y, (u * threads + t) * W, p.cols);
+    }
+}
+
+// Rows of up to 1024 columns, a warp each: lane t holds NV units of W floats, unit u at columns (32 u + t) * W.
+template <int W, int NV>
+__global__ void __launch_bounds__(kWarpRowThreads) layer_norm_warp_kernel(const NormParams p) {
+    const int t = threadIdx.x & 31;
+    const long long rows_at_once = static_cast<long long>(gridDim.x) * (kWarpRowThreads / 32);
     const float inv = 1.0f / static_cast<float>(p.cols);
-    for (; row < p.rows; row += rows_at_once) {
+    NormAffine<W, NV, W * NV <= 16> affine(p, t, 32);
+    for (long long row = blockIdx.x * static_cast<long long>(kWarpRowThreads / 32) + (threadIdx.x >> 5); row < p.rows;
+         row += rows_at_once) {
         const float* x = p.x + row * p.ldx;
         float v[NV][W];
-        float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int u = 0; u < NV; ++u) load_unit<W>(v[u], x, (u * threads + t) * W, p.cols);
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-#pragma unroll
-            for (int i = 0; i < W; ++i) s.x += v[u][i];
-        const float mean = row_sum(s).x * inv;
-        s = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float d = (u * threads + t) * W + i < p.cols ? v[u][i] - mean : 0.0f;
-                s.x += d * d;
-            }
-        const float rstd = 1.0f / sqrtf(row_sum(s).x * inv + p.eps);
-        if (t == 0) {
-            if (p.mean) p.mean[row] = mean;
-            if (p.rstd) p.rstd[row] = rstd;
+        for (int u = 0; u < NV; ++u) load_unit<W>(v[u], x, (u * 32 + t) * W, p.cols);
+        const NormStats st = norm_stats<W, NV>(v, t, 32, p, inv, [](float s) { return warp_sum(make_float2(s, 0.0f)).x; });
+        norm_out(v, st, affine, t, 32, row, p);
+    }
+}
+
+// Longer rows, a block each.
+template <int W, int NV>
+__global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_block_kernel(const NormParams p, int slots) {
+    __shared__ float2 buf[2][32];
+    __shared__ uint64_t bars[kMaxSlots];
+    __shared__ int failed;  // the first round whose copy did not arrive: every thread leaves in that round
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    RowSum<false> row_sum{buf};
+    const RowRing<1> ring{{{p.x, p.ldx}}, ring_smem, smem_addr(bars), slots, p.cols, p.rows};
+    const int threads = blockDim.x, t = threadIdx.x;
+    const float inv = 1.0f / static_cast<float>(p.cols);
+    if (t == 0) {
+        for (int s = 0; s < slots; ++s) mbar_init(ring.bar0 + 8 * s, 1);
+        failed = INT_MAX;
+        fence_barrier_init();
+        for (int s = 0; s < slots; ++s) {
+            const long long row = blockIdx.x + static_cast<long long>(s) * gridDim.x;
+            if (row < p.rows) ring.ask(row, s);
         }
-        float* y = p.y + row * p.ldy;
+    }
+    __syncthreads();
+    NormAffine<W, NV, true> affine(p, t, threads);
+    int slot = 0, round = 0;
+    uint32_t phase = 0;
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, ++round) {
+        if (!mbar_wait(ring.bar0 + 8 * slot, phase, p.timeout_ns)) atomicMin(&failed, round);
+        const float* x = ring.find(0, row, slot);
+        float v[NV][W];
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int c = (u * threads + t) * W;
-            float g[W], b[W];
-            load_param<W>(g, p.gamma, c, p.cols, 1.0f);
-            load_param<W>(b, p.beta, c, p.cols, 0.0f);
-#pragma unroll
-            for (int i = 0; i < W; ++i) v[u][i] = (v[u][i] - mean) * rstd * g[i] + b[i];
-            store_unit<W>(v[u], y, c, p.cols);
-        }
+        for (int u = 0; u < NV; ++u) take_unit<W>(v[u], x, (u * threads + t) * W, p.cols);
+        // The first sum's barrier says that every thread has taken its part: the slot can be filled again.
+        bool first = true;
+        const NormStats st = norm_stats<W, NV>(v, t, threads, p, inv, [&](float s) {
+            const float r = row_sum(make_float2(s, 0.0f)).x;
+            const long long ahead = row + static_cast<long long>(slots) * gridDim.x;
+            if (first && t == 0 && ahead < p.rows && failed > round) ring.ask(ahead, slot);
+            first = false;
+            return r;
+        });
+        if (failed <= round) break;
+        norm_out(v, st, affine, t, threads, row, p);
+        if (++slot == slots) { slot = 0; phase ^= 1u; }
+    }
+    if (t == 0 && failed != INT_MAX) {
+        atomicOr(p.err, kErrProducer);
+        for (int s = 0; s < 2 * slots; ++s) mbar_wait(ring.bar0 + 8 * (s % slots), s / slots, p.timeout_ns);
     }
 }
 
@@ -225,90 +405,210 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const NormParams 
     }
 }
 
-template <int W, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? kWarpRowThreads : 512)
-    layer_norm_grad_kernel(const NormGradParams p) {
-    __shared__ float2 buf[2][32];
-    extern __shared__ float block_acc[];  // WARP: [2][cols], the block's sums over its warps
-    RowSum<WARP> row_sum{buf};
-    const int threads = WARP ? 32 : blockDim.x;
-    const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const long long rows_at_once = static_cast<long long>(gridDim.x) * (WARP ? kWarpRowThreads / 32 : 1);
-    long long row = WARP ? blockIdx.x * static_cast<long long>(kWarpRowThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
-    const float inv = 1.0f / static_cast<float>(p.cols);
-    float dg[NV][W], db[NV][W], g[NV][W];
+// What the forward pass saved of a row.
+__device__ __forceinline__ NormStats saved_stats(const NormGradParams& p, long long row) {
+    if (row >= p.rows) return {0.0f, 0.0f};
+    return {__ldg(p.mean + row), __ldg(p.rstd + row)};
+}
+
+// One row of the backward pass, held by `threads` threads: xh and d come in as x and dy; dx goes out, and the
+// thread's columns of dgamma and dbeta grow.
+template <int W, int NV, typename Sum>
+__device__ __forceinline__ void norm_grad_row(float (&xh)[NV][W], float (&d)[NV][W], float (&dg)[NV][W], float (&db)[NV][W],
+                                              const float (&gamma)[NV][W], NormStats st, int t, int threads, long long row, const NormGradParams& p, float inv, Sum sum) {
+    const float mean = st.mean, rstd = st.rstd;
+    float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-        load_param<W>(g[u], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
 #pragma unroll
-        for (int i = 0; i < W; ++i) dg[u][i] = db[u][i] = 0.0f;
+        for (int i = 0; i < W; ++i) {
+            // Columns past the row have d = 0: they add nothing to any sum.
+            xh[u][i] = (xh[u][i] - mean) * rstd;
+            dg[u][i] += d[u][i] * xh[u][i];
+            db[u][i] += d[u][i];
+            d[u][i] *= gamma[u][i];
+            s.x += d[u][i];
+            s.y += d[u][i] * xh[u][i];
+        }
     }
+    s = sum(s);
+    if (!p.dx) return;
+    const float m1 = s.x * inv, m2 = s.y * inv;
+    float* dx = p.dx + row * p.lddx;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) d[u][i] = rstd * (d[u][i] - m1 - xh[u][i] * m2);
+        store_unit<W>(d[u], dx, (u * threads + t) * W, p.cols);
+    }
+}
+
+template <int W, int NV>
+__global__ void __launch_bounds__(kWarpRowThreads) layer_norm_grad_warp_kernel(const NormGradParams p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* block_acc = reinterpret_cast<float*>(smem);  // [2][cols]: the block's sums over its warps
+    constexpr int threads = 32;
+    const int t = threadIdx.x & 31;
+    const long long rows_at_once = static_cast<long long>(gridDim.x) * (kWarpRowThreads / 32);
+    const float inv = 1.0f / static_cast<float>(p.cols);
+    float dg[NV][W] = {}, db[NV][W] = {}, gamma[NV][W];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) load_param<W>(gamma[u], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
+    long long row = blockIdx.x * static_cast<long long>(kWarpRowThreads / 32) + (threadIdx.x >> 5);
+    NormStats next = saved_stats(p, row);  // a row ahead, so that no row waits for its two numbers
     for (; row < p.rows; row += rows_at_once) {
-        const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
-        const float* x = p.x + row * p.ldx;
-        const float* dy = p.dy + row * p.lddy;
+        const NormStats st = next;
+        next = saved_stats(p, row + rows_at_once);
         float xh[NV][W], d[NV][W];
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            load_unit<W>(xh[u], x, (u * threads + t) * W, p.cols);
-            load_unit<W>(d[u], dy, (u * threads + t) * W, p.cols);
+            load_unit<W>(xh[u], p.x + row * p.ldx, (u * 32 + t) * W, p.cols);
+            load_unit<W>(d[u], p.dy + row * p.lddy, (u * 32 + t) * W, p.cols);
+        }
+        norm_grad_row<W, NV>(xh, d, dg, db, gamma, st, t, 32, row, p, inv, [](float2 s) { return warp_sum(s); });
+    }
+    if (!p.partial) return;
+    // The warps add their sums one after the other, in warp order.
+    for (int w = 0; w < kWarpRowThreads / 32; ++w) {
+        if (static_cast<int>(threadIdx.x >> 5) == w) {
+#pragma unroll
+            for (int u = 0; u < NV; ++u)
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const int c = (u * 32 + t) * W + i;
+                    if (c < p.cols) {
+                        block_acc[c] = (w ? block_acc[c] : 0.0f) + dg[u][i];
+                        block_acc[p.cols + c] = (w ? block_acc[p.cols + c] : 0.0f) + db[u][i];
+                    }
+                }
+        }
+        __syncthreads();
+    }
+    float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
+    for (int c = threadIdx.x; c < 2 * p.cols; c += kWarpRowThreads) out[c] = block_acc[c];
+}
+
+template <int W, int NV>
+__global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_grad_block_kernel(const NormGradParams p, int slots) {
+    __shared__ float2 buf[2][32];
+    __shared__ uint64_t bars[kMaxSlots];
+    __shared__ int failed;  // the first round whose copy did not arrive: every thread leaves in that round
+    extern __shared__ __align__(16) uint8_t smem[];
+    RowSum<false> row_sum{buf};
+    const RowRing<2> ring{{{p.x, p.ldx}, {p.dy, p.lddy}}, smem, smem_addr(bars), slots, p.cols, p.rows};
+    const int threads = blockDim.x, t = threadIdx.x;
+    const float inv = 1.0f / static_cast<float>(p.cols);
+    if (t == 0) {
+        for (int s = 0; s < slots; ++s) mbar_init(ring.bar0 + 8 * s, 1);
+        failed = INT_MAX;
+        fence_barrier_init();
+        for (int s = 0; s < slots; ++s) {
+            const long long row = blockIdx.x + static_cast<long long>(s) * gridDim.x;
+            if (row < p.rows) ring.ask(row, s);
+        }
+    }
+    __syncthreads();
+    float dg[NV][W] = {}, db[NV][W] = {}, gamma[NV][W];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) load_param<W>(gamma[u], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
+    int slot = 0, round = 0;
+    uint32_t phase = 0;
+    NormStats next = saved_stats(p, blockIdx.x);  // a row ahead, so that no row waits for its two numbers
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, ++round) {
+        const NormStats st = next;
+        next = saved_stats(p, row + gridDim.x);
+        if (!mbar_wait(ring.bar0 + 8 * slot, phase, p.timeout_ns)) atomicMin(&failed, round);
+        const float* x = ring.find(0, row, slot);
+        const float* dy = ring.find(1, row, slot);
+        float xh[NV][W], d[NV][W];
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            take_unit<W>(xh[u], x, (u * threads + t) * W, p.cols);
+            take_unit<W>(d[u], dy, (u * threads + t) * W, p.cols);
+        }
+        // The sum's barrier says that every thread has taken its part: the slot can be filled again.
+        norm_grad_row<W, NV>(xh, d, dg, db, gamma, st, t, threads, row, p, inv, [&](float2 s) {
+            s = row_sum(s);
+            const long long ahead = row + static_cast<long long>(slots) * gridDim.x;
+            if (t == 0 && ahead < p.rows && failed > round) ring.ask(ahead, slot);
+            return s;
+        });
+        if (failed <= round) break;
+        if (++slot == slots) { slot = 0; phase ^= 1u; }
+    }
+    if (t == 0 && failed != INT_MAX) {
+        atomicOr(p.err, kErrProducer);
+        for (int s = 0; s < 2 * slots; ++s) mbar_wait(ring.bar0 + 8 * (s % slots), s / slots, p.timeout_ns);
+    }
+    if (!p.partial) return;
+    float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int c = (u * threads + t) * W + i;
+            if (c < p.cols) {
+                out[c] = dg[u][i];
+                out[p.cols + c] = db[u][i];
+            }
+        }
+}
+
+// Rows of up to 16384 columns: x and dy in the registers of 1024 threads, the sums for dgamma and dbeta, for
+// which none are left, in shared memory, each column touched by one thread only.
+template <int W>
+__global__ void __launch_bounds__(1024) layer_norm_grad_wide_kernel(const NormGradParams p) {
+    constexpr int NV = 16 / W;
+    __shared__ float2 buf[2][32];
+    extern __shared__ __align__(16) uint8_t smem[];
+    float* acc = reinterpret_cast<float*>(smem);  // [2][cols]
+    RowSum<false> row_sum{buf};
+    const int t = threadIdx.x;
+    const float inv = 1.0f / static_cast<float>(p.cols);
+    for (int c = t; c < 2 * p.cols; c += 1024) acc[c] = 0.0f;
+    __syncthreads();
+    NormStats next = saved_stats(p, blockIdx.x);
+    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        const NormStats st = next;
+        next = saved_stats(p, row + gridDim.x);
+        float xh[NV][W], d[NV][W];
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            load_unit<W>(xh[u], p.x + row * p.ldx, (u * 1024 + t) * W, p.cols);
+            load_unit<W>(d[u], p.dy + row * p.lddy, (u * 1024 + t) * W, p.cols);
         }
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int u = 0; u < NV; ++u)
+        for (int u = 0; u < NV; ++u) {
+            float g[W];
+            load_param<W>(g, p.gamma, (u * 1024 + t) * W, p.cols, 1.0f);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                // Columns past the row have d = 0: they add nothing to any sum.
-                xh[u][i] = (xh[u][i] - mean) * rstd;
-                dg[u][i] += d[u][i] * xh[u][i];
-                db[u][i] += d[u][i];
-                d[u][i] *= g[u][i];
+                const int c = (u * 1024 + t) * W + i;
+                xh[u][i] = (xh[u][i] - st.mean) * st.rstd;
+                if (c < p.cols) {
+                    acc[c] += d[u][i] * xh[u][i];
+                    acc[p.cols + c] += d[u][i];
+                }
+                d[u][i] *= g[i];
                 s.x += d[u][i];
                 s.y += d[u][i] * xh[u][i];
             }
+        }
         if (!p.dx) continue;
         s = row_sum(s);
         const float m1 = s.x * inv, m2 = s.y * inv;
-        float* dx = p.dx + row * p.lddx;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) d[u][i] = rstd * (d[u][i] - m1 - xh[u][i] * m2);
-            store_unit<W>(d[u], dx, (u * threads + t) * W, p.cols);
+            for (int i = 0; i < W; ++i) d[u][i] = st.rstd * (d[u][i] - m1 - xh[u][i] * m2);
+            store_unit<W>(d[u], p.dx + row * p.lddx, (u * 1024 + t) * W, p.cols);
         }
     }
     if (!p.partial) return;
     float* out = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
-    if constexpr (!WARP) {
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const int c = (u * threads + t) * W + i;
-                if (c < p.cols) {
-                    out[c] = dg[u][i];
-                    out[p.cols + c] = db[u][i];
-                }
-            }
-    } else {
-        // The warps add their sums one after the other, in warp order.
-        for (int w = 0; w < kWarpRowThreads / 32; ++w) {
-            if (static_cast<int>(threadIdx.x >> 5) == w) {
-#pragma unroll
-                for (int u = 0; u < NV; ++u)
-#pragma unroll
-                    for (int i = 0; i < W; ++i) {
-                        const int c = (u * 32 + t) * W + i;
-                        if (c < p.cols) {
-                            block_acc[c] = (w ? block_acc[c] : 0.0f) + dg[u][i];
-                            block_acc[p.cols + c] = (w ? block_acc[p.cols + c] : 0.0f) + db[u][i];
-                        }
-                    }
-            }
-            __syncthreads();
-        }
-        for (int c = threadIdx.x; c < 2 * p.cols; c += kWarpRowThreads) out[c] = block_acc[c];
-    }
+    __syncthreads();
+    for (int c = t; c < 2 * p.cols; c += 1024) out[c] = acc[c];
 }
 
 // Rows too long for a block's registers: x and dy are read twice, and the
@@ -364,27 +664,35 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(const NormGr
     }
 }
 
-// dgamma[c] (blockIdx.y 0) or dbeta[c] (1): the blocks' partial rows, summed
-// by 32 threads per column and then in thread order.
-__global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial, int blocks, int cols, float* dgamma,
-                                                            float* dbeta) {
-    __shared__ float part[32][33];
+// dgamma[c] (blockIdx.y 0) or dbeta[c] (1): the blocks' partial rows, summed by ROWS threads per column and then in
+// thread order.  Launched while the backward kernel still runs (its launch latency hides there).
+template <int ROWS>
+__global__ void __launch_bounds__(32 * ROWS) sum_partials_kernel(const float* partial, int blocks, int cols, float* dgamma,
+                                                                 float* dbeta) {
+    __shared__ float part[ROWS][33];
     float* out = blockIdx.y ? dbeta : dgamma;
-    if (!out) return;
     const int c = blockIdx.x * 32 + threadIdx.x;
+    cudaGridDependencySynchronize();
+    if (!out) return;
     float s = 0.0f;
     if (c < cols) {
         const float* src = partial + static_cast<long long>(blockIdx.y) * cols + c;
-        for (int b = threadIdx.y; b < blocks; b += 32) s += src[static_cast<long long>(b) * 2 * cols];
+#pragma unroll 8
+        for (int b = threadIdx.y; b < blocks; b += ROWS) s += __ldcg(src + static_cast<long long>(b) * 2 * cols);
     }
     part[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
-    s = warp_sum(make_float2(part[threadIdx.x][threadIdx.y], 0.0f)).x;
-    const int cc = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && cc < cols) out[cc] = s;
+    if (threadIdx.y == 0 && c < cols) {
+#pragma unroll
+        for (int i = 1; i < ROWS; ++i) s += part[i][threadIdx.x];
+        out[c] = s;
+    }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr int kBlockThreads = 512;                      // of a block that holds more than kWideFloats of a row a thread
+constexpr int kWideThreads = 1024, kWideFloats = 8;
 
 // How a row is spread: `threads` threads (32: a warp, eight rows to a block)
 // holding `units` units each; units == 0: the kernel for long rows.
@@ -393,22 +701,32 @@ struct RowPlan {
     bool warp;
 };
 
-// max_floats: what a thread may hold of one row; max_threads: of one block.
-RowPlan plan_row(int cols, int width, long long rows, int num_sms, int max_floats, int max_threads) {
-    const int total = (cols + width - 1) / width, max_units = max_floats / width;
-    auto pow2 = [](int n) {
-        int p = 1;
-        while (p < n) p *= 2;
-        return p;
-    };
+// warp_floats, block_floats: what a thread may hold of one row.
+RowPlan plan_row(int cols, int width, long long rows, int num_sms, int warp_floats, int block_floats) {
+    const int total = (cols + width - 1) / width;
     // Few rows leave most SMs without one: the widest block shortens each thread's share of a row.
     const bool few = rows <= 2ll * num_sms;
-    if (total <= 32 || (!few && total <= 32 * max_units)) return {32, pow2((total + 31) / 32), true};
-    int threads = few ? max_threads : std::min(256, max_threads);
-    while (threads < max_threads && total > threads * max_units) threads *= 2;
-    while (few && threads / 2 >= total) threads /= 2;
-    if (total > threads * max_units) return {max_threads, 0, false};
-    return {threads, pow2((total + threads - 1) / threads), false};
+    if (total <= 32 || (!few && total * width <= 32 * warp_floats)) {
+        int units = 1;
+        while (32 * units < total) units *= 2;
+        return {32, units, true};
+    }
+    auto threads_for = [&](int units) { return ((total + units - 1) / units + 31) / 32 * 32; };
+    if (few) {
+        for (int units = 1; units * width <= kWideFloats; units *= 2)
+            if (threads_for(units) <= kWideThreads) return {threads_for(units), units, false};
+    }
+    // Else the smallest block, for many rows side by side on an SM (65536 x 1024 backward: 139 us with 64 threads, 222
+    // with 256), unless whole warps of it would idle; 16 floats before more.
+    for (int floats = std::min(16, block_floats); floats <= block_floats; floats *= 2) {
+        for (int units = floats / width; units >= 1; units /= 2) {
+            const int threads = threads_for(units);
+            if (threads <= kBlockThreads && 4ll * threads * units <= 5ll * total + 128) return {threads, units, false};
+        }
+        for (int units = floats / width; units >= 1; units /= 2)
+            if (threads_for(units) <= kBlockThreads) return {threads_for(units), units, false};
+    }
+    return {kWideThreads, 0, false};
 }
 
 template <typename Kernel>
@@ -421,96 +739,136 @@ int resident_blocks(Kernel kernel, int threads, size_t smem, int num_sms) {
     return n * num_sms;
 }
 
-template <int W, int NV, bool WARP>
+// Slots of a ring with `mats` rows to a slot, for a kernel of which `blocks` fit on an SM by their registers: what
+// shared memory gives each of them, two at least.
+int ring_slots(int blocks, int cols, int mats) {
+    return std::max(2, std::min(kMaxSlots, 216 * 1024 / std::min(blocks, 16) / (mats * row_slot_bytes(cols))));
+}
+
+// Allows `kernel` the shared memory that a ring may take, once per device.
+template <typename Kernel>
+cudaError_t allow_ring(Kernel kernel, uint64_t* done) {
+    static std::mutex mu;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev < 64 && (*done & (1ull << dev))) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    if (e == cudaSuccess && dev < 64) *done |= 1ull << dev;
+    return e;
+}
+
+constexpr int kNormFloats = 32;      // of a row per thread: 1024 columns per warp, 16384 per block
+constexpr int kNormGradFloats = 16;  // x, dy and two sums for each: 512 columns per warp, 8192 per block
+
+template <int W, int NV>
 cudaError_t launch_norm(const NormParams& p, const RowPlan& plan, int num_sms, cudaStream_t stream) {
-    const int threads = WARP ? kWarpRowThreads : plan.threads;
-    const long long want = WARP ? (p.rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32) : p.rows;
-    const int blocks = static_cast<int>(
-        std::min<long long>(want, resident_blocks(layer_norm_kernel<W, NV, WARP>, threads, 0, num_sms)));
-    layer_norm_kernel<W, NV, WARP><<<blocks, threads, 0, stream>>>(p);
+    if (plan.warp) {
+        const long long want = (p.rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32);
+        const int blocks = static_cast<int>(
+            std::min<long long>(want, resident_blocks(layer_norm_warp_kernel<W, NV>, kWarpRowThreads, 0, num_sms)));
+        layer_norm_warp_kernel<W, NV><<<blocks, kWarpRowThreads, 0, stream>>>(p);
+    } else {
+        static uint64_t allowed = 0;
+        const cudaError_t e = allow_ring(layer_norm_block_kernel<W, NV>, &allowed);
+        if (e != cudaSuccess) return e;
+        const int slots = ring_slots(resident_blocks(layer_norm_block_kernel<W, NV>, plan.threads, 0, 1), p.cols, 1);
+        const size_t smem = static_cast<size_t>(slots) * row_slot_bytes(p.cols);
+        const int blocks = static_cast<int>(
+            std::min<long long>(p.rows, resident_blocks(layer_norm_block_kernel<W, NV>, plan.threads, smem, num_sms)));
+        layer_norm_block_kernel<W, NV><<<blocks, plan.threads, smem, stream>>>(p, slots);
+    }
     note_launch();
     return cudaGetLastError();
 }
-
-template <int W, bool WARP>
-cudaError_t launch_norm_units(const NormParams& p, const RowPlan& plan, int num_sms, cudaStream_t stream) {
-    switch (plan.units) {
-        case 1: return launch_norm<W, 1, WARP>(p, plan, num_sms, stream);
-        case 2: return launch_norm<W, 2, WARP>(p, plan, num_sms, stream);
-        case 4: return launch_norm<W, 4, WARP>(p, plan, num_sms, stream);
-        case 8: return launch_norm<W, 8, WARP>(p, plan, num_sms, stream);
-        case 16: return launch_norm<W, W == 1 ? 16 : 8, WARP>(p, plan, num_sms, stream);
-        case 32: return launch_norm<W, W == 1 ? 32 : 8, WARP>(p, plan, num_sms, stream);
-        default: return cudaErrorInvalidValue;
-    }
-}
-
-constexpr int kNormFloats = 32;      // of a row per thread: 1024 columns per warp, 32768 per block
-constexpr int kNormGradFloats = 16;  // x, dy and two sums for each: 512 columns per warp, 8192 per block
 
 template <int W>
 cudaError_t launch_norm_width(const NormParams& p, int num_sms, cudaStream_t stream) {
-    const RowPlan plan = plan_row(p.cols, W, p.rows, num_sms, kNormFloats, 1024);
-    if (plan.units == 0) {
-        const int blocks = static_cast<int>(
-            std::min<long long>(p.rows, resident_blocks(layer_norm_long_kernel<W>, plan.threads, 0, num_sms)));
-        layer_norm_long_kernel<W><<<blocks, plan.threads, 0, stream>>>(p);
-        note_launch();
-        return cudaGetLastError();
+    const RowPlan plan = plan_row(p.cols, W, p.rows, num_sms, kNormFloats, kNormFloats);
+    switch (plan.units) {
+        case 1: return launch_norm<W, 1>(p, plan, num_sms, stream);
+        case 2: return launch_norm<W, 2>(p, plan, num_sms, stream);
+        case 4: return launch_norm<W, 4>(p, plan, num_sms, stream);
+        case 8: return launch_norm<W, 8>(p, plan, num_sms, stream);
+        case 16: return launch_norm<W, W == 1 ? 16 : 8>(p, plan, num_sms, stream);
+        case 32: return launch_norm<W, W == 1 ? 32 : 8>(p, plan, num_sms, stream);
+        default: break;
     }
-    return plan.warp ? launch_norm_units<W, true>(p, plan, num_sms, stream)
-                     : launch_norm_units<W, false>(p, plan, num_sms, stream);
-}
-
-// One launch of the backward kernel, or (p == nullptr) the number of blocks it takes.
-template <int W, int NV, bool WARP>
-cudaError_t launch_norm_grad(const NormGradParams* p, const RowPlan& plan, long long rows, int cols, int num_sms,
-                             int* blocks, cudaStream_t stream) {
-    const int threads = WARP ? kWarpRowThreads : plan.threads;
-    const size_t smem = WARP ? 2 * sizeof(float) * cols : 0;
-    if (!p) {
-        const long long want = WARP ? (rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32) : rows;
-        *blocks = static_cast<int>(
-            std::min<long long>(want, resident_blocks(layer_norm_grad_kernel<W, NV, WARP>, threads, smem, num_sms)));
-        return cudaSuccess;
-    }
-    layer_norm_grad_kernel<W, NV, WARP><<<*blocks, threads, smem, stream>>>(*p);
+    const int blocks = static_cast<int>(
+        std::min<long long>(p.rows, resident_blocks(layer_norm_long_kernel<W>, plan.threads, 0, num_sms)));
+    layer_norm_long_kernel<W><<<blocks, plan.threads, 0, stream>>>(p);
     note_launch();
     return cudaGetLastError();
 }
 
-template <int W, bool WARP>
-cudaError_t launch_norm_grad_units(const NormGradParams* p, const RowPlan& plan, long long rows, int cols, int num_sms,
-                                   int* blocks, cudaStream_t stream) {
-    switch (plan.units) {
-        case 1: return launch_norm_grad<W, 1, WARP>(p, plan, rows, cols, num_sms, blocks, stream);
-        case 2: return launch_norm_grad<W, 2, WARP>(p, plan, rows, cols, num_sms, blocks, stream);
-        case 4: return launch_norm_grad<W, 4, WARP>(p, plan, rows, cols, num_sms, blocks, stream);
-        case 8: return launch_norm_grad<W, W == 1 ? 8 : 4, WARP>(p, plan, rows, cols, num_sms, blocks, stream);
-        case 16: return launch_norm_grad<W, W == 1 ? 16 : 4, WARP>(p, plan, rows, cols, num_sms, blocks, stream);
-        default: return cudaErrorInvalidValue;
+// One launch of the backward kernel, or (p == nullptr) the number of blocks it takes.
+template <int W, int NV>
+cudaError_t launch_norm_grad(const NormGradParams* p, const RowPlan& plan, long long rows, int cols, int num_sms,
+                             int* blocks, cudaStream_t stream) {
+    if (plan.warp) {
+        const size_t smem = 2 * sizeof(float) * cols;
+        if (!p) {
+            const long long want = (rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32);
+            *blocks = static_cast<int>(
+                std::min<long long>(want, resident_blocks(layer_norm_grad_warp_kernel<W, NV>, kWarpRowThreads, smem, num_sms)));
+            return cudaSuccess;
+        }
+        layer_norm_grad_warp_kernel<W, NV><<<*blocks, kWarpRowThreads, smem, stream>>>(*p);
+    } else {
+        const int slots = ring_slots(resident_blocks(layer_norm_grad_block_kernel<W, NV>, plan.threads, 0, 1), cols, 2);
+        const size_t smem = static_cast<size_t>(slots) * 2 * row_slot_bytes(cols);
+        if (!p) {
+            static uint64_t allowed = 0;
+            const cudaError_t e = allow_ring(layer_norm_grad_block_kernel<W, NV>, &allowed);
+            if (e != cudaSuccess) return e;
+            *blocks = static_cast<int>(
+                std::min<long long>(rows, resident_blocks(layer_norm_grad_block_kernel<W, NV>, plan.threads, smem, num_sms)));
+            return cudaSuccess;
+        }
+        layer_norm_grad_block_kernel<W, NV><<<*blocks, plan.threads, smem, stream>>>(*p, slots);
     }
+    note_launch();
+    return cudaGetLastError();
 }
 
 template <int W>
 cudaError_t launch_norm_grad_width(const NormGradParams* p, long long rows, int cols, int num_sms, int* blocks,
                                    cudaStream_t stream) {
-    const RowPlan plan = plan_row(cols, W, rows, num_sms, kNormGradFloats, 512);
-    if (plan.units == 0) {
+    const RowPlan plan = plan_row(cols, W, rows, num_sms, kNormGradFloats, kNormGradFloats);
+    switch (plan.units) {
+        case 1: return launch_norm_grad<W, 1>(p, plan, rows, cols, num_sms, blocks, stream);
+        case 2: return launch_norm_grad<W, 2>(p, plan, rows, cols, num_sms, blocks, stream);
+        case 4: return launch_norm_grad<W, 4>(p, plan, rows, cols, num_sms, blocks, stream);
+        case 8: return launch_norm_grad<W, W == 1 ? 8 : 4>(p, plan, rows, cols, num_sms, blocks, stream);
+        case 16: return launch_norm_grad<W, W == 1 ? 16 : 4>(p, plan, rows, cols, num_sms, blocks, stream);
+        default: break;
+    }
+    if (cols <= 16 * 1024) {
+        const size_t smem = 2 * sizeof(float) * cols;
         if (!p) {
+            static uint64_t allowed = 0;
+            const cudaError_t e = allow_ring(layer_norm_grad_wide_kernel<W>, &allowed);
+            if (e != cudaSuccess) return e;
             *blocks = static_cast<int>(
-                std::min<long long>(rows, resident_blocks(layer_norm_grad_long_kernel<W>, plan.threads, 0, num_sms)));
+                std::min<long long>(rows, resident_blocks(layer_norm_grad_wide_kernel<W>, kWideThreads, smem, num_sms)));
             return cudaSuccess;
         }
-        layer_norm_grad_long_kernel<W><<<*blocks, plan.threads, 0, stream>>>(*p);
+        layer_norm_grad_wide_kernel<W><<<*blocks, kWideThreads, smem, stream>>>(*p);
         note_launch();
         return cudaGetLastError();
     }
-    return plan.warp ? launch_norm_grad_units<W, true>(p, plan, rows, cols, num_sms, blocks, stream)
-                     : launch_norm_grad_units<W, false>(p, plan, rows, cols, num_sms, blocks, stream);
+    if (!p) {
+        *blocks = static_cast<int>(
+            std::min<long long>(rows, resident_blocks(layer_norm_grad_long_kernel<W>, plan.threads, 0, num_sms)));
+        return cudaSuccess;
+    }
+    layer_norm_grad_long_kernel<W><<<*blocks, plan.threads, 0, stream>>>(*p);
+    note_launch();
+    return cudaGetLastError();
 }
 
-int layer_norm(GpuCtx* ctx, const NormParams& p, void* stream) {
+int layer_norm(GpuCtx* ctx, NormParams p, void* stream) {
     if (!ctx || p.rows < 0 || p.cols < 1 || p.ldx < p.cols || p.ldy < p.cols || (p.rows > 0 && (!p.x || !p.y))) {
         set_error("mxb_layer_norm: invalid arguments");
         return MXB_E_ARG;
@@ -524,6 +882,8 @@ int layer_norm(GpuCtx* ctx, const NormParams& p, void* stream) {
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     const bool vec = aligned16(p.x) && aligned16(p.y) && aligned16(p.gamma) && aligned16(p.beta) && p.ldx % 4 == 0 &&
                      p.ldy % 4 == 0;
+    p.timeout_ns = ctx->timeout_ns;
+    p.err = ctx->d_err;
     const cudaError_t e = vec ? launch_norm_width<4>(p, ctx->num_sms, st) : launch_norm_width<1>(p, ctx->num_sms, st);
     return cuda_ok(e, "layer norm launch") ? MXB_OK : MXB_E_CUDA;
 }
@@ -554,6 +914,8 @@ int layer_norm_backward(GpuCtx* ctx, NormGradParams p, float* dgamma, float* dbe
         return vec ? launch_norm_grad_width<4>(q, p.rows, p.cols, ctx->num_sms, blocks, st)
                    : launch_norm_grad_width<1>(q, p.rows, p.cols, ctx->num_sms, blocks, st);
     };
+    p.timeout_ns = ctx->timeout_ns;
+    p.err = ctx->d_err;
     int blocks = 0;
     if (!cuda_ok(run(nullptr, &blocks), "layer norm backward plan")) return MXB_E_CUDA;
     Scratch scratch(ctx, st);
@@ -563,9 +925,21 @@ int layer_norm_backward(GpuCtx* ctx, NormGradParams p, float* dgamma, float* dbe
     }
     if (!cuda_ok(run(&p, &blocks), "layer norm backward launch")) return MXB_E_CUDA;
     if (!p.partial) return MXB_OK;
-    sum_partials_kernel<<<dim3((p.cols + 31) / 32, 2), dim3(32, 32), 0, st>>>(p.partial, blocks, p.cols, dgamma, dbeta);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((p.cols + 31) / 32, 2);
+    // Many columns fill the SMs with small blocks; few columns need more threads for each.
+    const bool tall = p.cols <= 32 * ctx->num_sms;
+    cfg.blockDim = dim3(32, tall ? 32 : 8);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, tall ? sum_partials_kernel<32> : sum_partials_kernel<8>,
+                                             static_cast<const float*>(p.partial), blocks, p.cols, dgamma, dbeta);
     note_launch();
-    return cuda_ok(cudaGetLastError(), "layer norm gradient sums launch") ? MXB_OK : MXB_E_CUDA;
+    return cuda_ok(e, "layer norm gradient sums launch") ? MXB_OK : MXB_E_CUDA;
 }
 
 }  // namespace
@@ -575,7 +949,8 @@ extern "C" {
 
 int mxb_layer_norm(GpuCtx* ctx, const float* x, long long ldx, const float* gamma, const float* beta, float eps,
                    float* y, long long ldy, float* mean, float* rstd, long long rows, int cols, void* stream) {
-    return mxb::layer_norm(ctx, mxb::NormParams{x, ldx, gamma, beta, eps, y, ldy, mean, rstd, rows, cols}, stream);
+    return mxb::layer_norm(ctx, mxb::NormParams{x, ldx, gamma, beta, eps, y, ldy, mean, rstd, rows, cols, 0, nullptr},
+                           stream);
 }
 
 int mxb_layer_norm_backward(GpuCtx* ctx, const float* dy, long long lddy, const float* x, long long ldx,
@@ -583,7 +958,7 @@ int mxb_layer_norm_backward(GpuCtx* ctx, const float* dy, long long lddy, const 
                             float* dgamma, float* dbeta, long long rows, int cols, void* stream) {
     try {
         return mxb::layer_norm_backward(
-            ctx, mxb::NormGradParams{dy, lddy, x, ldx, gamma, mean, rstd, dx, lddx, nullptr, rows, cols}, dgamma,
+            ctx, mxb::NormGradParams{dy, lddy, x, ldx, gamma, mean, rstd, dx, lddx, nullptr, rows, cols, 0, nullptr}, dgamma,
             dbeta, stream);
     } catch (const std::exception& e) {  // host allocations of the pool's lists
         mxb::set_error("mxb_layer_norm_backward: %s", e.what());
