@@ -279,15 +279,6 @@ __device__ __forceinline__ void raise_grouped(const GroupedParams& p, volatile i
     *abort_flag = 1;
 }
 
-template <int N>
-__device__ __forceinline__ void more_registers() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void fewer_registers() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 constexpr int kGroupedSegKb = 2;  // k-blocks (of 32) to an accumulator
 
 template <int MODE, int BT>

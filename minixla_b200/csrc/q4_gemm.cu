@@ -369,35 +369,46 @@ cudaError_t run_few_rows_width(const Q4Params& p, int num_sms, cudaStream_t stre
 // ---------------------------------------------------------------- many rows
 //
 // More than 16 rows: bound by the tensor cores.  A tile is 128 weight columns
-// (TMEM lanes) by up to 128 rows (TMEM columns).  Eight warps turn the 4-bit
-// values of 64 k into a K-major bf16 tile of q - z (exact); the activations'
-// three bf16 parts, cut beforehand into workspace by q4_cut_kernel, arrive by
-// TMA; per 16 k the three parts are multiplied into the same accumulator.
-// That is 3 bf16 products, half the tensor time of the 3xTF32 product that
-// fp32 weights need, and exact up to the fp32 sums.  An accumulator takes the
-// k of one group (at most 128); the epilogue warps, whose lanes each hold one
-// weight column, add it times that column's scale to fp32 totals.
+// (TMEM lanes) by up to 128 rows (TMEM columns).  Eight warps, a thread to a
+// weight column, turn the 4-bit values of 64 k into bf16 q - z (exact) in
+// tensor memory, the MMA's A operand; the activations' three bf16 parts, cut
+// beforehand into workspace by q4_cut_kernel, arrive by TMA; per 16 k the three
+// parts are multiplied into the same accumulator.  That is 3 bf16 products,
+// half the tensor time of the 3xTF32 product that fp32 weights need, and exact
+// up to the fp32 sums.  With the weights in shared memory as well, its 128 bytes
+// a clock were the limit (164 KB a stage against 768 clocks of MMA; now 104 KB).
+// An accumulator takes the k of one group (at most 128); the epilogue warps,
+// whose lanes each hold one weight column, add it times that column's scale to
+// fp32 totals.
 // The eight k of a word keep the order in which its nibbles pair up (k, k + 4):
 // the cut kernel writes the activations in the same order.
+// With fewer tiles than SMs, a cluster of `splits` CTAs shares a tile, each
+// summing its own stretch of K; the totals meet in distributed shared memory,
+// added in CTA order.
 
-constexpr int kManyCols = 128;  // rows of A per tile
+constexpr int kManyCols = 128;  // rows of A per tile, at most
 constexpr int kManyK = 64;      // k per stage: 128 bytes of bf16
 
 struct ManyCfg {
     static constexpr int kXBytes = 3 * kManyCols * kManyK * 2;  // the parts of a stage
-    static constexpr int kXStages = 3;
+    static constexpr int kXStages = 4;
     static constexpr int kRawBytes = 128 * 64;                  // 128 k of 128 weight rows
-    static constexpr int kRawStages = 4;
-    static constexpr int kDeqBytes = 128 * kManyK * 2;
-    static constexpr int kDeqStages = 2;
+    static constexpr int kRawStages = 3;
+    static constexpr int kDeqStages = 4;                        // weights in tensor memory: 32 columns each
     static constexpr int kEpiWarps = 8, kConvWarps = 8;
-    static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 2);
+    static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 4);  // and a warpgroup with TMA and MMA
+    // Registers a thread: the launch has 640 x 96, given out in shares of 128 threads.
+    static constexpr int kEpiRegs = 160, kConvRegs = 56, kIssueRegs = 48;
+    static_assert(2 * kEpiRegs + 2 * kConvRegs + kIssueRegs <= 480, "more registers than the launch has");
     static constexpr int kRawOffset = kXStages * kXBytes;
-    static constexpr int kDeqOffset = kRawOffset + kRawStages * kRawBytes;
-    static constexpr int kBarOffset = kDeqOffset + kDeqStages * kDeqBytes;
+    static constexpr int kBarOffset = kRawOffset + kRawStages * kRawBytes;
     static constexpr int kNumBars = 2 * kXStages + 2 * kRawStages + 2 * kDeqStages + 4 + 1;
-    static constexpr int kTmemCols = 2 * kManyCols;
+    static constexpr int kDeqCol = 2 * kManyCols;               // first TMEM column behind the two accumulators
+    static constexpr int kTmemCols = 512;
     static constexpr int kSmem = 1024 + kBarOffset + kNumBars * 8 + 16;
+    static constexpr int kMaxSplits = 8;
+    static_assert(kDeqCol + 32 * kDeqStages <= kTmemCols, "tensor memory");
+    static_assert(kManyCols * 128 * 4 <= kRawOffset, "a tile's totals fit in the activations' stages");
     static_assert(kSmem <= 227 * 1024, "shared memory budget");
 };
 
@@ -407,13 +418,14 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
            (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                        uint32_t accumulate) {
+// A in tensor memory: lane i holds row i, a 32-bit column two elements along K.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
@@ -447,7 +459,9 @@ __global__ void __launch_bounds__(256) q4_cut_kernel(const float* a, long long l
 
 struct ManyParams {
     Q4Params q;
+    int cols;              // rows of A per tile: a multiple of 16
     int col_tiles, tiles;
+    int splits;
 };
 
 __device__ __forceinline__ void raise_q4(const Q4Params& p, volatile int* abort_flag, int bit) {
@@ -530,71 +544,83 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    const int stages = (p.K + kManyK - 1) / kManyK;
+    const int all_stages = (p.K + kManyK - 1) / kManyK;
     const int halves = (p.K + 31) / 32;                                     // of 32 k
     const int seg = p.group % 128 == 0 ? 4 : p.group % 64 == 0 ? 2 : 1;     // halves to an accumulator
+    const int team = blockIdx.x / mp.splits, teams = gridDim.x / mp.splits, rank = blockIdx.x - team * mp.splits;
+    // This CTA's stages [kb0, kb1) of every tile: whole runs of 128 k, so that no accumulator crosses a group.
+    const int runs = (all_stages + 1) / 2;
+    const int kb0 = static_cast<int>(static_cast<long long>(runs) * rank / mp.splits) * 2;
+    const int kb1 = min(all_stages, static_cast<int>(static_cast<long long>(runs) * (rank + 1) / mp.splits) * 2);
 
-    if (warp == kTmaWarp) {
-        if (lane == 0) {
-            int xs = 0, rs = 0;
-            uint32_t xph = 0, rph = 0;
-            long long xn = 0, rn = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; t < mp.tiles && ok; t += gridDim.x) {
-                const int n0 = t / mp.col_tiles * 128, m0 = t % mp.col_tiles * kManyCols;
-                const int boxes = (min(kManyCols, p.M - m0) + 31) / 32;
-                for (int kb = 0; kb < stages; ++kb) {
-                    if ((kb & 1) == 0) {
-                        if (*abort_flag || !mbar_wait(rempty(rs), rph ^ 1u, p.timeout_ns)) {
-                            ok = false;
-                            break;
-                        }
-                        mbar_arrive_expect_tx(rfull(rs), C::kRawBytes);
-                        tma_load_2d(smem_addr(smem + C::kRawOffset + rs * C::kRawBytes), &tm_w, rfull(rs), kb * 32, n0);
-                        ++rn;
-                        if (++rs == kR) { rs = 0; rph ^= 1u; }
-                    }
-                    if (*abort_flag || !mbar_wait(xempty(xs), xph ^ 1u, p.timeout_ns)) {
+    if (warp >= kTmaWarp) {
+      fewer_registers<C::kIssueRegs>();
+      if (warp == kTmaWarp) {
+        // ------------------------------------------------------------ TMA producer
+        const bool leader = elect_one();
+        const uint32_t x_bytes = static_cast<uint32_t>(3 * mp.cols * kManyK * 2);
+        int xs = 0, rs = 0;
+        uint32_t xph = 0, rph = 0;
+        long long xn = 0, rn = 0;
+        bool ok = true;
+        for (int t = team; t < mp.tiles && ok; t += teams) {
+            const int n0 = t / mp.col_tiles * 128, m0 = t % mp.col_tiles * mp.cols;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if ((kb & 1) == 0) {
+                    if (*abort_flag || !mbar_wait(rempty(rs), rph ^ 1u, p.timeout_ns)) {
                         ok = false;
                         break;
                     }
-                    mbar_arrive_expect_tx(xfull(xs), 3 * boxes * 4096);
-                    const uint32_t dst = smem_addr(smem + xs * C::kXBytes);
-                    for (int q = 0; q < 3; ++q)
-                        for (int j = 0; j < boxes; ++j)
-                            tma_load_3d(dst + (q * 4 + j) * 4096, &tm_x, xfull(xs), kb * kManyK, m0 + 32 * j, q);
-                    ++xn;
-                    if (++xs == kX) { xs = 0; xph ^= 1u; }
+                    if (leader) {
+                        mbar_arrive_expect_tx(rfull(rs), C::kRawBytes);
+                        tma_load_2d(smem_addr(smem + C::kRawOffset + rs * C::kRawBytes), &tm_w, rfull(rs), kb * 32, n0);
+                    }
+                    __syncwarp();
+                    ++rn;
+                    if (++rs == kR) { rs = 0; rph ^= 1u; }
                 }
-            }
-            if (!ok) {
-                raise_q4(p, abort_flag, kErrProducer);
-                // Copies in flight land in this CTA's shared memory: wait for them before leaving.
-                for (long long i = xn > kX ? xn - kX : 0; i < xn; ++i)
-                    mbar_wait(xfull(static_cast<int>(i % kX)), static_cast<uint32_t>((i / kX) & 1), p.timeout_ns);
-                for (long long i = rn > kR ? rn - kR : 0; i < rn; ++i)
-                    mbar_wait(rfull(static_cast<int>(i % kR)), static_cast<uint32_t>((i / kR) & 1), p.timeout_ns);
+                if (*abort_flag || !mbar_wait(xempty(xs), xph ^ 1u, p.timeout_ns)) {
+                    ok = false;
+                    break;
+                }
+                if (leader) {
+                    mbar_arrive_expect_tx(xfull(xs), x_bytes);
+                    tma_load_3d(smem_addr(smem + xs * C::kXBytes), &tm_x, xfull(xs), kb * kManyK, m0, 0);
+                }
+                __syncwarp();
+                ++xn;
+                if (++xs == kX) { xs = 0; xph ^= 1u; }
             }
         }
-    } else if (warp == kMmaWarp) {
+        if (!ok && leader) {
+            raise_q4(p, abort_flag, kErrProducer);
+            // Copies in flight land in this CTA's shared memory: wait for them before leaving.
+            for (long long i = xn > kX ? xn - kX : 0; i < xn; ++i)
+                mbar_wait(xfull(static_cast<int>(i % kX)), static_cast<uint32_t>((i / kX) & 1), p.timeout_ns);
+            for (long long i = rn > kR ? rn - kR : 0; i < rn; ++i)
+                mbar_wait(rfull(static_cast<int>(i % kR)), static_cast<uint32_t>((i / kR) & 1), p.timeout_ns);
+        }
+        __syncwarp();
+      } else if (warp == kMmaWarp) {
         // ------------------------------------------------------------ MMA issuer
         constexpr uint32_t kHi = smem_desc_hi(1024, kLayoutSW128);
         const bool leader = elect_one();
         int xs = 0, ds = 0, acc = 0;
         uint32_t xph = 0, dph = 0, aph = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < mp.tiles && ok; t += gridDim.x) {
-            const int m0 = t % mp.col_tiles * kManyCols;
-            const uint32_t idesc = idesc_bf16(128, (min(kManyCols, p.M - m0) + 15) & ~15);
+        for (int t = team; t < mp.tiles && ok; t += teams) {
+            const int m0 = t % mp.col_tiles * mp.cols;
+            const uint32_t idesc = idesc_bf16(128, (min(mp.cols, p.M - m0) + 15) & ~15);
+            const uint32_t part = static_cast<uint32_t>(mp.cols * 8);  // 128 bytes a row, in descriptor steps of 16
             int in_seg = 0;
-            for (int kb = 0; kb < stages && ok; ++kb) {
+            for (int kb = kb0; kb < kb1 && ok; ++kb) {
                 if (*abort_flag || !mbar_wait(xfull(xs), xph, p.timeout_ns) ||
                     !mbar_wait(dfull(ds), dph, p.timeout_ns)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t w = smem_desc_lo(smem_addr(smem + C::kDeqOffset + ds * C::kDeqBytes), 16);
+                const uint32_t w = tmem_base + static_cast<uint32_t>(C::kDeqCol + 32 * ds);
                 const uint32_t x = smem_desc_lo(smem_addr(smem + xs * C::kXBytes), 16);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -612,11 +638,10 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
                         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                             for (int q = 2; q >= 0; --q)  // small parts first
-                                mma_f16(d, smem_desc_of(kHi, w + 2 * (2 * h + kk)),
-                                        smem_desc_of(kHi, x + q * 1024 + 2 * (2 * h + kk)), idesc,
-                                        kk == 0 && q == 2 ? (in_seg != 0 ? 1u : 0u) : 1u);
+                                mma_f16_ts(d, w + 8 * (2 * h + kk), smem_desc_of(kHi, x + q * part + 2 * (2 * h + kk)),
+                                           idesc, kk == 0 && q == 2 ? (in_seg != 0 ? 1u : 0u) : 1u);
                     }
-                    if (++in_seg == seg || 2 * kb + h == halves - 1) {
+                    if (++in_seg == seg || 2 * kb + h == min(2 * kb1, halves) - 1) {
                         if (leader) mma_commit(tfull(acc));
                         in_seg = 0;
                         acc ^= 1;
@@ -637,24 +662,27 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
             if (!mbar_wait(drain, 0, p.timeout_ns)) raise_q4(p, abort_flag, kErrMma);
         }
         __syncwarp();
+      }
     } else if (warp >= kConvWarp) {
-        // ------------------------------------------------------------ 4 bits to bf16: a row and 32 k a thread
+        // ------------------------------------------------------------ 4 bits to bf16: a weight column and 32 k a thread
+        fewer_registers<C::kConvRegs>();
         const int tid = threadIdx.x - 32 * kConvWarp, row = tid & 127, half = tid >> 7;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(row & ~31) << 16) + C::kDeqCol + 16 * half;
         int rs = 0, ds = 0;
         uint32_t rph = 0, dph = 0;
         bool failed = false;
-        for (int t = blockIdx.x; t < mp.tiles && !failed; t += gridDim.x) {
+        for (int t = team; t < mp.tiles && !failed; t += teams) {
             const int n = min(t / mp.col_tiles * 128 + row, p.N - 1);
             GroupWalk at{p.group, 0, 0};
-            at.step(32 * half);
+            at.step(kb0 * kManyK + 32 * half);
             auto zero_of = [&](int kb) -> uint32_t {
                 return p.zeros && kb * kManyK + 32 * half < p.K ? __ldg(p.zeros + n * p.lds + at.index) : 8u;
             };
-            uint32_t z_next = zero_of(0);
-            for (int kb = 0; kb < stages; ++kb) {
+            uint32_t z_next = zero_of(kb0);
+            for (int kb = kb0; kb < kb1; ++kb) {
                 const uint32_t z = z_next & 15u;
                 at.step(kManyK);
-                if (kb + 1 < stages) z_next = zero_of(kb + 1);
+                if (kb + 1 < kb1) z_next = zero_of(kb + 1);
                 const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
                 const bool got = !stop && mbar_wait(rfull(rs), rph, p.timeout_ns) &&
                                  mbar_wait(dempty(ds), dph ^ 1u, p.timeout_ns);
@@ -667,46 +695,49 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
                 const uint4 w4 = *reinterpret_cast<const uint4*>(smem + C::kRawOffset + rs * C::kRawBytes + row * 64 +
                                                                  ((chunk ^ ((row >> 1) & 3)) << 4));
                 const uint32_t z128 = 0x43004300u | z | (z << 16);
-                uint8_t* dst = smem + C::kDeqOffset + ds * C::kDeqBytes + row * 128;
                 const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                uint32_t r[16];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<uint4*>(dst + (((4 * half + j) ^ (row & 7)) << 4)) =
-                        make_uint4(weight_pair(w[j], z128), weight_pair(w[j] >> 4, z128), weight_pair(w[j] >> 8, z128),
-                                   weight_pair(w[j] >> 12, z128));
-                fence_proxy_async_shared();
+                for (int j = 0; j < 16; ++j) r[j] = weight_pair(w[j >> 2] >> (4 * (j & 3)), z128);
+                tc_fence_after();
+                tmem_st_32x32b_x16(lane_base + static_cast<uint32_t>(32 * ds), r);
+                tmem_st_wait();
+                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(dfull(ds));
-                    if ((kb & 1) || kb == stages - 1) mbar_arrive(rempty(rs));
+                    if ((kb & 1) || kb == kb1 - 1) mbar_arrive(rempty(rs));
                 }
                 if (++ds == kD) { ds = 0; dph ^= 1u; }
-                if ((kb & 1) || kb == stages - 1) {
+                if ((kb & 1) || kb == kb1 - 1) {
                     if (++rs == kR) { rs = 0; rph ^= 1u; }
                 }
             }
         }
     } else {
         // ------------------------------------------------------------ epilogue: a weight column and 64 rows a thread
+        more_registers<C::kEpiRegs>();
         constexpr int W = 16, kTotals = kManyCols / 2;
         const int quad = warp & 3, first_col = (warp >> 2) * kTotals;
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + first_col;
         int acc = 0;
         uint32_t aph = 0;
         bool failed = false;
-        for (int t = blockIdx.x; t < mp.tiles && !failed; t += gridDim.x) {
-            const int col = t / mp.col_tiles * 128 + quad * 32 + lane, m0 = t % mp.col_tiles * kManyCols;
-            const int cols = min(kManyCols, p.M - m0);
+        for (int t = team; t < mp.tiles && !failed; t += teams) {
+            const int col = t / mp.col_tiles * 128 + quad * 32 + lane, m0 = t % mp.col_tiles * mp.cols;
+            const int cols = min(mp.cols, p.M - m0);
             const long long scale_row = min(col, p.N - 1) * p.lds;
             float total[kTotals];
 #pragma unroll
             for (int i = 0; i < kTotals; ++i) total[i] = 0.0f;
-            uint32_t s_next = scale_raw(p, scale_row);
             GroupWalk at{p.group, 0, 0};
-            for (int h = 0; h < halves; h += seg) {
+            at.step(kb0 * kManyK);
+            uint32_t s_next = scale_raw(p, scale_row + at.index);
+            const int h1 = min(2 * kb1, halves);
+            for (int h = 2 * kb0; h < h1; h += seg) {
                 const float s = scale_value(p, s_next);
                 at.step(32 * seg);
-                if (h + seg < halves) s_next = scale_raw(p, scale_row + at.index);
+                if (h + seg < h1) s_next = scale_raw(p, scale_row + at.index);
                 const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
                 const bool got = !stop && mbar_wait(tfull(acc), aph, p.timeout_ns);
                 if (!__all_sync(0xffffffffu, got)) {
@@ -715,14 +746,19 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
                     break;
                 }
                 tc_fence_after();
+                // The second half's load is under way while the first is added.
+                const uint32_t src = lane_base + static_cast<uint32_t>(acc * kManyCols);
+                if (first_col < cols) {
+                    uint32_t r[32], q[32];
+                    tmem_ld_32x32b_x32(src, r);
+                    tmem_ld_wait();
+                    if (first_col + 32 < cols) tmem_ld_32x32b_x32(src + 32, q);
 #pragma unroll
-                for (int c = 0; c < kTotals; c += W) {
-                    if (first_col + c < cols) {
-                        uint32_t r[W];
-                        tmem_ld_32x32b_x16(lane_base + static_cast<uint32_t>(acc * kManyCols + c), r);
+                    for (int i = 0; i < 32; ++i) total[i] += s * __uint_as_float(r[i]);
+                    if (first_col + 32 < cols) {
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < W; ++i) total[c + i] += s * __uint_as_float(r[i]);
+                        for (int i = 0; i < 32; ++i) total[32 + i] += s * __uint_as_float(q[i]);
                     }
                 }
                 tc_fence_before();
@@ -732,6 +768,14 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
                 if (acc == 0) aph ^= 1u;
             }
             if (failed) break;
+            if (mp.splits > 1) {
+                // The one tile of this cluster: every copy and MMA of it is done, so the activations' stages can hold
+                // the totals, [row][weight column].
+                float* share = reinterpret_cast<float*>(smem) + first_col * 128 + quad * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < kTotals; ++i) share[i * 128] = total[i];
+                continue;
+            }
             if (col < p.N) {
 #pragma unroll
                 for (int c = 0; c < kTotals; c += W) {
@@ -751,6 +795,25 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
         }
     }
 
+    if (mp.splits > 1) {
+        __syncwarp();
+        cluster_sync();  // the totals of every CTA of the tile are in place (or a CTA gave up)
+        if (team < mp.tiles && *abort_flag == 0) {
+            const int n0 = team / mp.col_tiles * 128, m0 = team % mp.col_tiles * mp.cols;
+            // Every thread an output, this CTA the rows rank, rank + splits, ...
+            const int share = (min(mp.cols, p.M - m0) - rank + mp.splits - 1) / mp.splits;
+            for (int i = threadIdx.x; i < share * 128; i += C::kThreads) {
+                const int row = rank + (i >> 7) * mp.splits, col = n0 + (i & 127);
+                if (col >= p.N) continue;
+                const uint32_t at = smem_addr(smem) + static_cast<uint32_t>(row * 128 + (i & 127)) * 4;
+                float v = 0.0f;
+                for (int r = 0; r < mp.splits; ++r) v += ld_shared_cluster_f32(mapa_shared(at, static_cast<uint32_t>(r)));
+                p.out[(m0 + row) * p.ldo + col] = apply_cell(v, m0 + row, col, 0, p.epi);
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while another still reads its totals
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp) {
@@ -782,6 +845,28 @@ int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
     note_launch();
     if (!cuda_ok(cudaGetLastError(), "4-bit product: cutting the rows")) return MXB_E_CUDA;
 
+    // The tile width (a multiple of 16) that needs the least time in whole rounds of the SMs: a round costs its width and
+    // about 16 columns more.  1000 rows x 8192: 9 tiles of 112 in 4 rounds instead of 8 of 128 in 4.
+    const long long lane_tiles = (p.N + 127) / 128;
+    ManyParams mp{p, kManyCols, 0, 0, 1};
+    long long best = -1;
+    for (int w = kManyCols; w >= 16; w -= 16) {
+        const long long rounds = ((p.M + w - 1) / w * lane_tiles + ctx->num_sms - 1) / ctx->num_sms;
+        if (best < 0 || rounds * (w + 16) < best) {
+            best = rounds * (w + 16);
+            mp.cols = w;
+        }
+    }
+    mp.col_tiles = (p.M + mp.cols - 1) / mp.cols;
+    const long long tiles = mp.col_tiles * lane_tiles;
+    if (tiles >= (1ll << 31)) {
+        set_error("mxb_q4_gemm: too many tiles");
+        return MXB_E_UNSUPPORTED;
+    }
+    mp.tiles = static_cast<int>(tiles);
+    // Splits while every cluster still has SMs of its own and every CTA at least two runs of 128 k.
+    const int runs = (p.K + 127) / 128;
+    while (mp.splits < C::kMaxSplits && 2 * mp.splits * tiles <= ctx->num_sms && runs >= 4 * mp.splits) mp.splits *= 2;
     CUtensorMap mw, mx;
     const unsigned long long w_dims[2] = {static_cast<unsigned long long>(p.ldq), static_cast<unsigned long long>(p.N)};
     const unsigned long long w_stride[1] = {static_cast<unsigned long long>(p.ldq)};
@@ -789,7 +874,7 @@ int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
     const unsigned long long x_dims[3] = {static_cast<unsigned long long>(kp), static_cast<unsigned long long>(p.M), 3};
     const unsigned long long x_strides[2] = {static_cast<unsigned long long>(kp) * 2,
                                              static_cast<unsigned long long>(kp) * 2 * p.M};
-    const unsigned x_box[3] = {kManyK, 32, 1};
+    const unsigned x_box[3] = {kManyK, static_cast<unsigned>(mp.cols), 3};
     if (!encode_tensor_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p.q, w_dims, w_stride, w_box,
                            CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B) ||
         !encode_tensor_map(&mx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, parts, x_dims, x_strides, x_box,
@@ -797,17 +882,21 @@ int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
         set_error("mxb_q4_gemm: the tensor maps could not be made");
         return MXB_E_CUDA;
     }
-    ManyParams mp{p, (p.M + kManyCols - 1) / kManyCols, 0};
-    const long long tiles = static_cast<long long>(mp.col_tiles) * ((p.N + 127) / 128);
-    if (tiles >= (1ll << 31)) {
-        set_error("mxb_q4_gemm: too many tiles");
-        return MXB_E_UNSUPPORTED;
-    }
-    mp.tiles = static_cast<int>(tiles);
-    q4_many_rows_kernel<<<static_cast<int>(std::min<long long>(tiles, ctx->num_sms)), C::kThreads, C::kSmem, stream>>>(
-        mw, mx, mp);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = mp.splits;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(mp.splits > 1 ? tiles * mp.splits : std::min<long long>(tiles, ctx->num_sms)));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, q4_many_rows_kernel, mw, mx, mp);
     note_launch();
-    return cuda_ok(cudaGetLastError(), "4-bit product launch") ? MXB_OK : MXB_E_CUDA;
+    return cuda_ok(e, "4-bit product launch") ? MXB_OK : MXB_E_CUDA;
 }
 
 int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, void* stream) {

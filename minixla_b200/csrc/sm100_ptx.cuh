@@ -431,6 +431,22 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint16_t cta_mask)
         : "memory");
 }
 
+// ---------------------------------------------------------------- registers between warpgroups
+//
+// A warpgroup (four warps, all of them together) gives up registers, or takes
+// those that others gave up: the shares of a block must not add up to more than
+// its launch got.
+
+template <int N>
+__device__ __forceinline__ void more_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 // ---------------------------------------------------------------- descriptors
 
 // Shared-memory matrix descriptor (sm_100 version field = 1); addresses and
