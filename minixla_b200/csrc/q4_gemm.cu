@@ -418,14 +418,17 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int m, int n) {
            (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-// A in tensor memory: lane i holds row i, a 32-bit column two elements along K.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                           uint32_t accumulate) {
+// A in tensor memory: lane i holds row i, a 32-bit column two elements along K.  The whole warp comes here and one
+// thread issues (`leader`): without a branch around it the operands stay in uniform registers, which the instruction
+// reads, instead of being moved there for every MMA.
+__device__ __forceinline__ void mma_f16_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                           uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
         : "memory");
 }
 
@@ -633,14 +636,12 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
                         tc_fence_after();
                     }
                     const uint32_t d = tmem_base + static_cast<uint32_t>(acc * kManyCols);
-                    if (leader) {
 #pragma unroll
-                        for (int kk = 0; kk < 2; ++kk)
+                    for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-                            for (int q = 2; q >= 0; --q)  // small parts first
-                                mma_f16_ts(d, w + 8 * (2 * h + kk), smem_desc_of(kHi, x + q * part + 2 * (2 * h + kk)),
-                                           idesc, kk == 0 && q == 2 ? (in_seg != 0 ? 1u : 0u) : 1u);
-                    }
+                        for (int q = 2; q >= 0; --q)  // small parts first
+                            mma_f16_ts(leader, d, w + 8 * (2 * h + kk), smem_desc_of(kHi, x + q * part + 2 * (2 * h + kk)),
+                                       idesc, kk == 0 && q == 2 ? (in_seg != 0 ? 1u : 0u) : 1u);
                     if (++in_seg == seg || 2 * kb + h == min(2 * kb1, halves) - 1) {
                         if (leader) mma_commit(tfull(acc));
                         in_seg = 0;
@@ -716,6 +717,8 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
         }
     } else {
         // ------------------------------------------------------------ epilogue: a weight column and 64 rows a thread
+        // (Sixteen warps, with 32 rows a thread, were no faster: 606 against 620 us with groups of 32, 340 against 326 with
+        // groups of 128.)
         more_registers<C::kEpiRegs>();
         constexpr int W = 16, kTotals = kManyCols / 2;
         const int quad = warp & 3, first_col = (warp >> 2) * kTotals;
@@ -845,15 +848,17 @@ int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
     note_launch();
     if (!cuda_ok(cudaGetLastError(), "4-bit product: cutting the rows")) return MXB_E_CUDA;
 
-    // The tile width (a multiple of 16) that needs the least time in whole rounds of the SMs: a round costs its width and
-    // about 16 columns more.  1000 rows x 8192: 9 tiles of 112 in 4 rounds instead of 8 of 128 in 4.
+    // The tile width (a multiple of 16) that needs the least time in whole rounds of the SMs: a round costs its width (96
+    // columns at least: a narrower MMA takes no less) and about 32 columns more.  1000 rows x 8192: 9 tiles of 112 in 4
+    // rounds instead of 8 of 128 in 4.
     const long long lane_tiles = (p.N + 127) / 128;
     ManyParams mp{p, kManyCols, 0, 0, 1};
     long long best = -1;
     for (int w = kManyCols; w >= 16; w -= 16) {
         const long long rounds = ((p.M + w - 1) / w * lane_tiles + ctx->num_sms - 1) / ctx->num_sms;
-        if (best < 0 || rounds * (w + 16) < best) {
-            best = rounds * (w + 16);
+        const long long cost = rounds * (std::max(w, 96) + 32);
+        if (best < 0 || cost < best) {
+            best = cost;
             mp.cols = w;
         }
     }
