@@ -601,7 +601,7 @@ struct GroupedFewCfg {
     static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 2);
     static constexpr int kSmallCol = 4 * kCols;       // first TMEM column behind the two accumulators of 64
     static constexpr int kTmemCols = 256;
-    static constexpr int kSegKb = 4;                  // k-blocks to an accumulator: 32 sums into each column
+    static constexpr int kSegKb = 2;                  // k-blocks to an accumulator: 16 sums into each column
     static constexpr int kTableOffset = kStages * kStageBytes;
     static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
     static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;

@@ -729,14 +729,22 @@ RowPlan plan_row(int cols, int width, long long rows, int num_sms, int warp_floa
     return {kWideThreads, 0, false};
 }
 
-template <typename Kernel>
-int resident_blocks(Kernel kernel, int threads, size_t smem, int num_sms) {
-    int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess || n < 1) {
-        cudaGetLastError();
-        n = 1;
-    }
-    return n * num_sms;
+// Blocks of `threads` threads and `smem` bytes of shared memory that fit on an SM: by the kernel's registers (each of
+// the four partitions has 16384, a warp takes 32 times a thread's), the threads and the shared memory.  Computed here,
+// because asking the runtime for it takes longer than a small call.
+template <auto kernel>
+int blocks_per_sm(int threads, size_t smem) {
+    static const int regs = [] {
+        cudaFuncAttributes a;
+        if (cudaFuncGetAttributes(&a, kernel) != cudaSuccess) {
+            cudaGetLastError();
+            return 255;
+        }
+        return (a.numRegs + 7) / 8 * 8;
+    }();
+    const int by_regs = 4 * (16384 / (32 * regs)) / (threads / 32);
+    const int by_smem = static_cast<int>(227 * 1024 / (smem + 2048));
+    return std::max(1, std::min(std::min(by_regs, 2048 / threads), std::min(by_smem, 32)));
 }
 
 // Slots of a ring with `mats` rows to a slot, for a kernel of which `blocks` fit on an SM by their registers: what
@@ -767,16 +775,16 @@ cudaError_t launch_norm(const NormParams& p, const RowPlan& plan, int num_sms, c
     if (plan.warp) {
         const long long want = (p.rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32);
         const int blocks = static_cast<int>(
-            std::min<long long>(want, resident_blocks(layer_norm_warp_kernel<W, NV>, kWarpRowThreads, 0, num_sms)));
+            std::min<long long>(want, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_warp_kernel<W, NV>>(kWarpRowThreads, 0)));
         layer_norm_warp_kernel<W, NV><<<blocks, kWarpRowThreads, 0, stream>>>(p);
     } else {
         static uint64_t allowed = 0;
         const cudaError_t e = allow_ring(layer_norm_block_kernel<W, NV>, &allowed);
         if (e != cudaSuccess) return e;
-        const int slots = ring_slots(resident_blocks(layer_norm_block_kernel<W, NV>, plan.threads, 0, 1), p.cols, 1);
+        const int slots = ring_slots(blocks_per_sm<layer_norm_block_kernel<W, NV>>(plan.threads, 0), p.cols, 1);
         const size_t smem = static_cast<size_t>(slots) * row_slot_bytes(p.cols);
         const int blocks = static_cast<int>(
-            std::min<long long>(p.rows, resident_blocks(layer_norm_block_kernel<W, NV>, plan.threads, smem, num_sms)));
+            std::min<long long>(p.rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_block_kernel<W, NV>>(plan.threads, smem)));
         layer_norm_block_kernel<W, NV><<<blocks, plan.threads, smem, stream>>>(p, slots);
     }
     note_launch();
@@ -796,7 +804,7 @@ cudaError_t launch_norm_width(const NormParams& p, int num_sms, cudaStream_t str
         default: break;
     }
     const int blocks = static_cast<int>(
-        std::min<long long>(p.rows, resident_blocks(layer_norm_long_kernel<W>, plan.threads, 0, num_sms)));
+        std::min<long long>(p.rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_long_kernel<W>>(plan.threads, 0)));
     layer_norm_long_kernel<W><<<blocks, plan.threads, 0, stream>>>(p);
     note_launch();
     return cudaGetLastError();
@@ -811,19 +819,19 @@ cudaError_t launch_norm_grad(const NormGradParams* p, const RowPlan& plan, long 
         if (!p) {
             const long long want = (rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32);
             *blocks = static_cast<int>(
-                std::min<long long>(want, resident_blocks(layer_norm_grad_warp_kernel<W, NV>, kWarpRowThreads, smem, num_sms)));
+                std::min<long long>(want, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_grad_warp_kernel<W, NV>>(kWarpRowThreads, smem)));
             return cudaSuccess;
         }
         layer_norm_grad_warp_kernel<W, NV><<<*blocks, kWarpRowThreads, smem, stream>>>(*p);
     } else {
-        const int slots = ring_slots(resident_blocks(layer_norm_grad_block_kernel<W, NV>, plan.threads, 0, 1), cols, 2);
+        const int slots = ring_slots(blocks_per_sm<layer_norm_grad_block_kernel<W, NV>>(plan.threads, 0), cols, 2);
         const size_t smem = static_cast<size_t>(slots) * 2 * row_slot_bytes(cols);
         if (!p) {
             static uint64_t allowed = 0;
             const cudaError_t e = allow_ring(layer_norm_grad_block_kernel<W, NV>, &allowed);
             if (e != cudaSuccess) return e;
             *blocks = static_cast<int>(
-                std::min<long long>(rows, resident_blocks(layer_norm_grad_block_kernel<W, NV>, plan.threads, smem, num_sms)));
+                std::min<long long>(rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_grad_block_kernel<W, NV>>(plan.threads, smem)));
             return cudaSuccess;
         }
         layer_norm_grad_block_kernel<W, NV><<<*blocks, plan.threads, smem, stream>>>(*p, slots);
@@ -851,7 +859,7 @@ cudaError_t launch_norm_grad_width(const NormGradParams* p, long long rows, int 
             const cudaError_t e = allow_ring(layer_norm_grad_wide_kernel<W>, &allowed);
             if (e != cudaSuccess) return e;
             *blocks = static_cast<int>(
-                std::min<long long>(rows, resident_blocks(layer_norm_grad_wide_kernel<W>, kWideThreads, smem, num_sms)));
+                std::min<long long>(rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_grad_wide_kernel<W>>(kWideThreads, smem)));
             return cudaSuccess;
         }
         layer_norm_grad_wide_kernel<W><<<*blocks, kWideThreads, smem, stream>>>(*p);
@@ -860,7 +868,7 @@ cudaError_t launch_norm_grad_width(const NormGradParams* p, long long rows, int 
     }
     if (!p) {
         *blocks = static_cast<int>(
-            std::min<long long>(rows, resident_blocks(layer_norm_grad_long_kernel<W>, plan.threads, 0, num_sms)));
+            std::min<long long>(rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_grad_long_kernel<W>>(plan.threads, 0)));
         return cudaSuccess;
     }
     layer_norm_grad_long_kernel<W><<<*blocks, plan.threads, 0, stream>>>(*p);
