@@ -284,7 +284,7 @@ constexpr int kGroupedSegKb = 2;  // k-blocks (of 32) to an accumulator
 template <int MODE, int BT>
 __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
     grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_lane, const __grid_constant__ CUtensorMap tm_col,
-                        const __grid_constant__ GroupedParams p) {
+                        const __grid_constant__ GroupedParams p, const int splits) {
     using C = GroupedCfg<BT>;
     constexpr bool kLaneMn = MODE != kGradA, kColMn = MODE == kGradB;
     extern __shared__ uint8_t smem_raw[];
@@ -337,6 +337,12 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = tab.total;
+    const int team = blockIdx.x / splits, teams = gridDim.x / splits, rank = blockIdx.x - team * splits;
+    // This CTA's k-blocks [first, second) of a tile's `num_kb`.
+    auto my_part = [&](int num_kb, int& first) {
+        first = static_cast<int>(static_cast<long long>(num_kb) * rank / splits);
+        return static_cast<int>(static_cast<long long>(num_kb) * (rank + 1) / splits);
+    };
 
     if (warp >= kTmaWarp) {
         fewer_registers<C::kIssueRegs>();
@@ -348,13 +354,14 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                 long long issued = 0;
                 bool ok = true;
                 for (int round = 0; ok; ++round) {
-                    const int t = grouped_turn(round, blockIdx.x, gridDim.x, total_tiles);
+                    const int t = grouped_turn(round, team, teams, total_tiles);
                     if (t == -2) break;
                     if (t < 0) continue;
                     const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
                     const int col_boxes = (g.cols + 31) / 32;
-                    const int num_kb = (g.sum + kBK - 1) / kBK;
-                    for (int kb = 0; kb < num_kb; ++kb) {
+                    int kb0;
+                const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
+                    for (int kb = kb0; kb < kb1; ++kb) {
                         if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
                             raise_grouped(p, abort_flag, kErrProducer);
                             ok = false;
@@ -408,14 +415,15 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
             uint32_t phase = 0, small_phase = 0, acc_phase = 0;
             bool ok = true;
             for (int round = 0; ok; ++round) {
-                    const int t = grouped_turn(round, blockIdx.x, gridDim.x, total_tiles);
+                    const int t = grouped_turn(round, team, teams, total_tiles);
                     if (t == -2) break;
                     if (t < 0) continue;
                 const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
                 const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, kLaneMn, kColMn);
-                const int num_kb = (g.sum + kBK - 1) / kBK;
+                int kb0;
+                const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
                 int in_seg = 0;
-                for (int kb = 0; kb < num_kb; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     bool ready = *abort_flag == 0;
                     if (ready && in_seg == 0) ready = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
                     if (!ready || !mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
@@ -424,7 +432,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                         break;
                     }
                     tc_fence_after();
-                    const bool end_seg = ++in_seg == kGroupedSegKb || kb == num_kb - 1;
+                    const bool end_seg = ++in_seg == kGroupedSegKb || kb == kb1 - 1;
                     if (leader) {
                         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
                         const uint32_t big = smem_addr(smem + stage * C::kStageBytes);
@@ -478,13 +486,14 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         uint32_t phase = 0, small_phase = 0;
         bool failed = false;
         for (int round = 0; !failed; ++round) {
-                const int t = grouped_turn(round, blockIdx.x, gridDim.x, total_tiles);
+                const int t = grouped_turn(round, team, teams, total_tiles);
                 if (t == -2) break;
                 if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
             const int col_boxes = (g.cols + 31) / 32;
-            const int num_kb = (g.sum + kBK - 1) / kBK;
-            for (int kb = 0; kb < num_kb; ++kb) {
+            int kb0;
+                const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
+            for (int kb = kb0; kb < kb1; ++kb) {
                 const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
                 const bool got = !stop && mbar_wait(full_bar(stage), phase, p.timeout_ns) &&
                                  mbar_wait(sfree_bar(small), small_phase ^ 1u, p.timeout_ns);
@@ -513,15 +522,16 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         uint32_t acc_phase = 0;
         bool failed = false;
         for (int round = 0; !failed; ++round) {
-                const int t = grouped_turn(round, blockIdx.x, gridDim.x, total_tiles);
+                const int t = grouped_turn(round, team, teams, total_tiles);
                 if (t == -2) break;
                 if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
-            const int num_kb = (g.sum + kBK - 1) / kBK;
+            int kb0;
+                const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
             float total[C::kTotals];
 #pragma unroll
             for (int i = 0; i < C::kTotals; ++i) total[i] = 0.0f;
-            for (int k_begin = 0; k_begin < num_kb; k_begin += kGroupedSegKb) {
+            for (int k_begin = kb0; k_begin < kb1; k_begin += kGroupedSegKb) {
                 const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
                 const bool got = !stop && mbar_wait(tfull_bar(acc), acc_phase, p.timeout_ns);
                 if (!__all_sync(0xffffffffu, got)) {
@@ -548,6 +558,14 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
             }
             if (failed) break;
             const int col = g.lane0 + quad * 32 + lane;
+            if (splits > 1) {
+                // The one tile of this cluster: every copy and MMA of it is done, so the stages can hold the totals,
+                // [tile column][result column].
+                float* share = reinterpret_cast<float*>(smem) + first_col * 128 + quad * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < C::kTotals; ++i) share[i * 128] = total[i];
+                continue;
+            }
             if (col < p.lane_dim) {
 #pragma unroll
                 for (int c = 0; c < C::kTotals; c += W) {
@@ -567,6 +585,27 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         }
     }
 
+    if (splits > 1) {
+        __syncwarp();
+        cluster_sync();  // the totals of every CTA of the tile are in place (or a CTA gave up)
+        if (team < total_tiles && *abort_flag == 0) {
+            const GroupedTile g = grouped_tile<MODE, BT>(tab, team, p);
+            // Every thread an output, this CTA the tile columns rank, rank + splits, ...
+            const int share = (g.cols - rank + splits - 1) / splits;
+            for (int i = threadIdx.x; i < share * 128; i += C::kThreads) {
+                const int c = rank + (i >> 7) * splits, col = g.lane0 + (i & 127);
+                if (col >= p.lane_dim) continue;
+                const uint32_t at = smem_addr(smem) + static_cast<uint32_t>(c * 128 + (i & 127)) * 4;
+                float v = 0.0f;
+                for (int r = 0; r < splits; ++r) v += ld_shared_cluster_f32(mapa_shared(at, static_cast<uint32_t>(r)));
+                const long long row = g.col0 + c + (MODE == kGradB ? 0 : g.row0);
+                if (MODE != kGradB) v = apply_cell(v, row, col, g.group, p.epi);
+                p.out[row * p.ldo + col + (MODE == kGradB ? g.group * p.out_stride : 0)] = v;
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while another still reads its totals
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp) {
@@ -606,7 +645,6 @@ struct GroupedFewCfg {
     static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
     static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;
     static constexpr int kSmemBytes = 1024 + kBarOffset + kNumBars * 8 + 16;
-    static constexpr int kMaxSplits = 8;
     static_assert(kSmallCol + 32 * kSmall <= kTmemCols, "tensor memory");
     static_assert(kSmemBytes <= 227 * 1024, "shared memory budget");
 };
@@ -1325,6 +1363,32 @@ long long most_col_tiles(const GroupedCall& g, int cols) {
                           : g.rows / cols + std::min(g.groups, g.rows);
 }
 
+constexpr int kMaxSplits = 8;
+
+// Launches `kernel` for at most `tiles` tiles of about all_kb k-blocks: persistent CTAs, or clusters that share a tile
+// while every cluster still has SMs of its own and every CTA two k-blocks.
+template <typename Kernel>
+cudaError_t launch_clusters(Kernel kernel, int threads, int smem, long long tiles, int all_kb, int num_sms,
+                            cudaStream_t stream, const CUtensorMap& lane, const CUtensorMap& col, const GroupedParams& p) {
+    int splits = 1;
+    while (splits < kMaxSplits && 2 * splits * tiles <= num_sms && all_kb >= 4 * splits) splits *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = splits;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(splits > 1 ? tiles * splits : std::min<long long>(tiles, num_sms)), 1, 1);
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, lane, col, p, splits);
+    note_launch();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
 template <int MODE, int BT>
 cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
     using C = GroupedCfg<BT>;
@@ -1345,10 +1409,10 @@ cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int
     CUtensorMap lane, col;
     if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
     p.lane_tiles = (p.lane_dim + 127) / 128;
-    const int grid = static_cast<int>(std::min<long long>(most_col_tiles<MODE>(g, BT) * p.lane_tiles, num_sms));
-    kernel<<<grid, C::kThreads, C::kSmemBytes, stream>>>(lane, col, p);
-    note_launch();
-    return cudaGetLastError();
+    const long long tiles = most_col_tiles<MODE>(g, BT) * p.lane_tiles;
+    // The k-blocks a tile has at most; in grad_b of an even split, which is only a guess.
+    const int all_kb = ((MODE == kGradB ? g.rows / g.groups : p.sum_dim) + kBK - 1) / kBK;
+    return launch_clusters(kernel, C::kThreads, C::kSmemBytes, tiles, all_kb, num_sms, stream, lane, col, p);
 }
 
 template <int MODE>
@@ -1372,25 +1436,8 @@ cudaError_t run_grouped_few(const GroupedCall& g, GroupedParams& p, bool split3,
     if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
     p.lane_tiles = (p.lane_dim + 127) / 128;
     const long long tiles = most_col_tiles<MODE>(g, C::kCols) * p.lane_tiles;
-    // Splits while every cluster still has SMs of its own and every CTA at least two k-blocks.
-    const int all_kb = (p.sum_dim + kBK - 1) / kBK;
-    int splits = 1;
-    while (splits < C::kMaxSplits && 2 * splits * tiles <= num_sms && all_kb >= 4 * splits) splits *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = splits;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(splits > 1 ? tiles * splits : std::min<long long>(tiles, num_sms)), 1, 1);
-    cfg.blockDim = dim3(C::kThreads, 1, 1);
-    cfg.dynamicSmemBytes = C::kSmemBytes;
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, lane, col, p, splits);
-    note_launch();
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return launch_clusters(kernel, C::kThreads, C::kSmemBytes, tiles, (p.sum_dim + kBK - 1) / kBK, num_sms, stream, lane,
+                           col, p);
 }
 
 template <int MODE>
@@ -1446,11 +1493,15 @@ cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3
 
 template <int MODE>
 cudaError_t run_grouped_mode(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
-    const int per_group = MODE == kGradB ? g.K : (g.rows + g.groups - 1) / g.groups;
-    static const char* force = getenv("GR_PAIR");
-    if (force ? force[0] == '1' : per_group > 160) return run_grouped_pair<MODE>(g, p, split3, num_sms, stream);
+    // By the columns that a group's tiles have on average (8 groups, 2048 x 4096, cold L2, few / single / pair in us):
+    // 16 rows 74 / - / 109, 48 rows - / 103 / 118, 64 rows - / 113 / 125, 96 rows - / 160 / 129, 256 rows - / 280 / 203.
+    // A pair's tile is four times a single CTA's, so it also has to have enough of them for all pairs.
+    const int cols = MODE == kGradB ? g.K : (g.rows + g.groups - 1) / g.groups;
+    const long long pair_tiles = most_col_tiles<MODE>(g, GroupedPairCfg::kCols) * ((p.lane_dim + 255) / 256);
+    if (cols > 80 && p.lane_dim > 128 && pair_tiles >= num_sms * 3 / 8)
+        return run_grouped_pair<MODE>(g, p, split3, num_sms, stream);
     if constexpr (MODE != kGradB) {
-        if (per_group <= 32) return run_grouped_few<MODE>(g, p, split3, num_sms, stream);
+        if (cols <= 32) return run_grouped_few<MODE>(g, p, split3, num_sms, stream);
     }
     return run_grouped<MODE, 128>(g, p, split3, num_sms, stream);
 }
