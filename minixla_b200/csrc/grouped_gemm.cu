@@ -66,6 +66,7 @@ struct GroupedParams {
     int sum_dim;                // forward: K, grad_a: N (grad_b: each group's rows)
     int lane_tiles;
     int split3;                 // 3xTF32
+    float* dbias;               // grad_b, 3xTF32 CTA pairs: column sums of dY, [groups][lane_dim] (or nullptr)
     unsigned long long timeout_ns;
     int* err;
     CellEpilogue epi;
@@ -133,6 +134,34 @@ __device__ __forceinline__ void convert_tile(uint8_t* big, uint8_t* low, int t0,
         dst[i] = make_float4(small_of(v.x), small_of(v.y), small_of(v.z), small_of(v.w));
     }
 }
+
+// grad_b's bias gradient, on the way: adds this k-block's rows of the staged lane side to the thread's 16 columns (four
+// of each box).  Thread t0 of 256 has row t0 / 8 and 16-byte chunk t0 % 8 of every box; which columns those are
+// depends on the row (32-byte chunks are swizzled by row % 4), but not on the k-block.
+__device__ __forceinline__ void add_lane_columns(const uint8_t* staged, int t0, float (&sum)[16]) {
+#pragma unroll
+    for (int box = 0; box < 4; ++box) {
+        const float4 v = reinterpret_cast<const float4*>(staged)[box * 256 + t0];
+        sum[4 * box] += v.x;
+        sum[4 * box + 1] += v.y;
+        sum[4 * box + 2] += v.z;
+        sum[4 * box + 3] += v.w;
+    }
+}
+__device__ __forceinline__ void add_lane_columns(const uint8_t*, int, float (&)[1]) {}
+
+// The warp's four rows of those sums added up, by column: dst[0 .. 127].
+__device__ __forceinline__ void leave_lane_sums(const float (&sum)[16], float* dst, int lane) {
+    const int block = (lane & 7) >> 1 ^ (lane >> 3), low = lane & 1;  // of this lane's columns within a box: 8 block + 4 low
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v += __shfl_sync(0xffffffffu, sum[e], q * 8 + ((block ^ q) << 1 | low));
+        if (lane < 8) dst[(e >> 2) * 32 + block * 8 + low * 4 + (e & 3)] = v;
+    }
+}
+__device__ __forceinline__ void leave_lane_sums(const float (&)[1], float*, int) {}
 
 // One tile of work.
 struct GroupedTile {
@@ -1002,8 +1031,10 @@ struct GroupedPairCfg {
     static constexpr int kTotals = 128;
     static constexpr int kSmallOffset = kStages * kStageBytes;
     static constexpr int kTableOffset = kSmallOffset + kSmall * kStageBytes;
-    static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
-    static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;
+    static constexpr int kSumBuffers = 3;             // of the converter warps' sums for dbias
+    static constexpr int kSumsOffset = kTableOffset + kGroupedTableBytes;
+    static constexpr int kBarOffset = kSumsOffset + kSumBuffers * kConvWarps * 128 * 4;
+    static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1 + kSumBuffers;
     static constexpr int kSmemBytes = 1024 + kBarOffset + kNumBars * 8 + 16;
     static constexpr int kEpiRegs = 168, kConvRegs = 48, kIssueRegs = 48;
     static_assert(2 * kEpiRegs + 2 * kConvRegs + kIssueRegs <= 480, "more registers than the launch has");
@@ -1032,6 +1063,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     auto tfull_bar = [&](int a) { return bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + a); };
     auto tempty_bar = [&](int a) { return bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 2 + a); };
     const uint32_t drain_bar = bar0 + 8u * (2 * C::kStages + 2 * C::kSmall + 4);
+    auto sums_bar = [&](int b) { return drain_bar + 8u * (1 + b); };              // converter warps -> the first of them
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
@@ -1052,6 +1084,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
             mbar_init(tempty_bar(a), 2 * C::kEpiWarps);
         }
         mbar_init(drain_bar, 1);
+        for (int b = 0; b < C::kSumBuffers; ++b) mbar_init(sums_bar(b), C::kConvWarps);
         *abort_flag = 0;
         fence_barrier_init();
         tma_prefetch_desc(&tm_lane);
@@ -1207,14 +1240,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
         fewer_registers<C::kConvRegs>();
         const int t0 = threadIdx.x - 32 * kConvWarp;
         const uint32_t conv_leader = mapa_shared(conv_bar(0), 0);
-        int stage = 0, small = 0;
-        uint32_t phase = 0, small_phase = 0;
+        int stage = 0, small = 0, sum_buf = 0;
+        uint32_t phase = 0, small_phase = 0, sum_phase = 0;
         bool failed = false;
         for (int round = 0; !failed; ++round) {
                 const int t = grouped_turn(round, pair, num_pairs, total_tiles);
                 if (t == -2) break;
                 if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
+            const bool sums = MODE == kGradB && p.dbias && g.col0 == 0;  // the bias gradient, once for each lane tile
+            float sum[MODE == kGradB ? 16 : 1];
+#pragma unroll
+            for (int e = 0; e < (MODE == kGradB ? 16 : 1); ++e) sum[e] = 0.0f;
             const int col_boxes = (half_cols(g.cols) + 31) / 32;
             const int num_kb = (g.sum + kBK - 1) / kBK;
             for (int kb = 0; kb < num_kb; ++kb) {
@@ -1228,12 +1265,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
                 }
                 convert_tile<MODE, 32 * C::kConvWarps>(smem + stage * C::kStageBytes, smem + C::kSmallOffset + small * C::kStageBytes, t0,
                                         1024 + col_boxes * 256, g.sum - kb * kBK, p.split3);
+                if (sums) add_lane_columns(smem + stage * C::kStageBytes, t0, sum);
                 fence_proxy_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_peer(conv_leader + 8u * small);
                 if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
                 if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
             }
+            if (failed || !sums) continue;
+            float* out = p.dbias + static_cast<long long>(g.group) * p.lane_dim;
+            const int col = g.lane0 + static_cast<int>(rank) * 128 + t0;
+            if (num_kb == 0) {
+                if (t0 < 128 && col < p.lane_dim) out[col] = 0.0f;
+                continue;
+            }
+            // Each warp leaves its sums; the first four add them up in warp order.  No warp is three tiles ahead of
+            // another (the MMA of two k-blocks back needs all of them), so three buffers take turns.
+            float* part = reinterpret_cast<float*>(smem + C::kSumsOffset) + sum_buf * C::kConvWarps * 128;
+            leave_lane_sums(sum, part + (t0 >> 5) * 128, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sums_bar(sum_buf));
+            if (t0 < 128) {
+                const bool got = mbar_wait(sums_bar(sum_buf), sum_phase, p.timeout_ns);
+                if (!__all_sync(0xffffffffu, got)) {
+                    if (lane == 0) raise_grouped(p, abort_flag, kErrProducer);
+                    failed = true;
+                } else if (col < p.lane_dim) {
+                    float v = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < C::kConvWarps; ++w) v += part[w * 128 + t0];
+                    out[col] = v;
+                }
+            }
+            if (++sum_buf == C::kSumBuffers) { sum_buf = 0; sum_phase ^= 1u; }
         }
     } else {
         // ------------------------------------------------------------ epilogue (both CTAs, their own lanes)
@@ -1498,8 +1562,11 @@ cudaError_t run_grouped_mode(const GroupedCall& g, GroupedParams& p, bool split3
     // A pair's tile is four times a single CTA's, so it also has to have enough of them for all pairs.
     const int cols = MODE == kGradB ? g.K : (g.rows + g.groups - 1) / g.groups;
     const long long pair_tiles = most_col_tiles<MODE>(g, GroupedPairCfg::kCols) * ((p.lane_dim + 255) / 256);
-    if (cols > 80 && p.lane_dim > 128 && pair_tiles >= num_sms * 3 / 8)
+    if (cols > 80 && p.lane_dim > 128 && pair_tiles >= num_sms * 3 / 8) {
+        // (TF32 mode: the staged dY is rounded; the bias gradient is summed from memory.)
+        p.dbias = split3 ? g.dbias : nullptr;
         return run_grouped_pair<MODE>(g, p, split3, num_sms, stream);
+    }
     if constexpr (MODE != kGradB) {
         if (cols <= 32) return run_grouped_few<MODE>(g, p, split3, num_sms, stream);
     }
@@ -1556,7 +1623,7 @@ int grouped_gemm(const char* fn, GpuCtx* ctx, const GroupedCall& g, const mxb_ep
                           : g.mode == kGradA ? run_grouped_mode<kGradA>(g, p, p.split3, ctx->num_sms, st)
                                              : run_grouped_mode<kGradB>(g, p, p.split3, ctx->num_sms, st);
     if (!cuda_ok(e, "grouped product launch")) return MXB_E_CUDA;
-    if (g.dbias) {
+    if (g.dbias && !p.dbias) {
         grouped_column_sums<<<dim3((g.N + 31) / 32, g.groups), dim3(32, 32), 0, st>>>(g.w, g.ldw, g.offsets, g.rows, g.N,
                                                                                      g.dbias);
         note_launch();
