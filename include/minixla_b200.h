@@ -367,7 +367,7 @@ MXB_API int mxb_layer_norm(GpuCtx* ctx, const float* x, long long ldx, const flo
  *   dx = rstd * (v - mean(v) - xhat * mean(v * xhat))    (means over the row)
  *   dgamma = sum over rows of dy * xhat,  dbeta = sum over rows of dy.
  * Each of dx, dgamma, dbeta may be NULL (not wanted; not all three).  dx may
- * be dy or x itself.  The sums over rows are made in a fixed order: the same
+ * be dy or x itself (same pointer and pitch).  The sums over rows are made in a fixed order: the same
  * inputs give the same bits.  rows == 0 writes zeros to dgamma and dbeta.
  * Partial sums use pooled workspace of the context; on a stream that is being
  * captured the workspace is an allocation of the graph itself, so captured
@@ -385,7 +385,9 @@ MXB_API int mxb_layer_norm_backward(GpuCtx* ctx, const float* dy, long long lddy
  * column K is not used).  scales: MXB_SCALE_* values, row pitch lds elements;
  * zeros: one byte (its low four bits) per scale, same pitch, or NULL for 8
  * everywhere.  group is a multiple of 32.  A needs a 16-byte aligned base and
- * lda % 4 == 0.  Epilogue steps as mxb_fused_gemm.  Products and sums are
+ * lda % 4 == 0.  Epilogue steps as mxb_fused_gemm; an ADD_FULL operand may be
+ * out itself (same pointer and pitch), otherwise out overlaps no input.
+ * M, N, K <= 2^30.  Products and sums are
  * fp32-faithful (the activations enter as exact bf16 parts, every
  * weight value q - z is exact in bf16, and each group's sum is scaled in
  * fp32), independent of the context's precision mode.  Workspace as for
@@ -413,7 +415,9 @@ MXB_API int mxb_q4_gemm(GpuCtx* ctx, const float* A, long long lda, const unsign
  * multiples of 4, A and B 16-byte aligned.  Steps: ADD_FULL, RELU, SCALE and
  * RELU_GRAD as named above (i: the row of out), and ADD_ROW with
  * operand[e * ld_or_size + j] (ld_or_size 0: one row for all groups).
- * precision as mxb_fused_gemm.  rows == 0 does nothing. */
+ * An ADD_FULL operand may be out itself (same pointer and pitch), otherwise
+ * out overlaps no input.  precision as mxb_fused_gemm.  Needs no workspace.
+ * rows, N, K <= 2^30.  rows == 0 does nothing. */
 #define MXB_MAX_GROUPS 1024
 MXB_API int mxb_grouped_gemm(GpuCtx* ctx, const float* A, long long lda, const float* B, long long ldb,
                    long long b_stride, const int* offsets, int groups, float* out, long long ldo, int rows, int N,

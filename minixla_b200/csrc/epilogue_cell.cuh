@@ -26,13 +26,13 @@ __device__ __forceinline__ float apply_cell(float v, long long row, int col, int
         switch (st.kind) {
             case MXB_EP_RELU: v = v > 0.0f ? v : 0.0f; break;
             case MXB_EP_SCALE: v = v * st.scale; break;
-            case MXB_EP_ADD_FULL: v += __ldg(st.ptr + row * st.ld_or_size + col); break;
+            case MXB_EP_ADD_FULL: v += __ldcs(st.ptr + row * st.ld_or_size + col); break;
             case MXB_EP_ADD_ROW: v += __ldg(st.ptr + group * st.ld_or_size + col); break;
             case MXB_EP_ADD_MOD:
                 v += __ldg(st.ptr + (static_cast<unsigned long long>(row) * e.n_cols + col) %
                                         static_cast<unsigned long long>(st.ld_or_size));
                 break;
-            case MXB_EP_RELU_GRAD: v = __ldg(st.ptr + row * st.ld_or_size + col) > 0.0f ? v : 0.0f; break;
+            case MXB_EP_RELU_GRAD: v = __ldcs(st.ptr + row * st.ld_or_size + col) > 0.0f ? v : 0.0f; break;
             default: break;
         }
     }
@@ -60,11 +60,11 @@ __device__ __forceinline__ void apply_column(float (&v)[W], long long row, int n
 #pragma unroll
             for (int i = 0; i < W; ++i)
                 if (i < n) v[i] += __ldg(st.ptr + (static_cast<unsigned long long>(row + i) * e.n_cols + col) % size);
-        } else {  // ADD_FULL, RELU_GRAD
+        } else {  // ADD_FULL, RELU_GRAD (plain loads: the operand may be the output itself)
             const float* src = st.ptr + row * st.ld_or_size + col;
             float c[W];
 #pragma unroll
-            for (int i = 0; i < W; ++i) c[i] = i < n ? __ldg(src + i * st.ld_or_size) : 0.0f;
+            for (int i = 0; i < W; ++i) c[i] = i < n ? __ldcs(src + i * st.ld_or_size) : 0.0f;
             if (st.kind == MXB_EP_ADD_FULL) {
 #pragma unroll
                 for (int i = 0; i < W; ++i) v[i] += c[i];

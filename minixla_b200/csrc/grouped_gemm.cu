@@ -1593,6 +1593,10 @@ int grouped_gemm(const char* fn, GpuCtx* ctx, const GroupedCall& g, const mxb_ep
         set_error("%s: the operands need 16-byte aligned bases, pitches and group strides (multiples of 4)", fn);
         return MXB_E_ARG;
     }
+    if (g.rows > kMaxExtent || g.N > kMaxExtent || g.K > kMaxExtent) {
+        set_error("%s: rows, N and K are limited to 2^30", fn);
+        return MXB_E_UNSUPPORTED;
+    }
     GroupedParams p{};
     if (!take_cell_steps(fn, steps, n_steps, out_cols, true, p.epi)) return MXB_E_ARG;
     if (g.rows == 0 && !grad_b) return MXB_OK;

@@ -150,6 +150,10 @@ bool encode_tensor_map(struct CUtensorMap_st* map, int dtype, int rank, const vo
                        const unsigned long long* dims, const unsigned long long* strides, const unsigned* box,
                        int swizzle, int l2_promotion);
 
+// Largest extent that the norm, 4-bit and grouped kernels take: tile and column
+// indices, which run up to a tile past it, are 32-bit.
+constexpr int kMaxExtent = 1 << 30;
+
 // Process-wide count of kernel launches issued by this library.
 void note_launch(unsigned n = 1);
 

@@ -885,6 +885,10 @@ int layer_norm(GpuCtx* ctx, NormParams p, void* stream) {
         set_error("mxb_layer_norm: in place, x and y need the same pitch");
         return MXB_E_ARG;
     }
+    if (p.cols > kMaxExtent) {
+        set_error("mxb_layer_norm: cols is limited to 2^30");
+        return MXB_E_UNSUPPORTED;
+    }
     if (p.rows == 0) return MXB_OK;
     DeviceScope scope(ctx->device);
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
@@ -907,6 +911,10 @@ int layer_norm_backward(GpuCtx* ctx, NormGradParams p, float* dgamma, float* dbe
             set_error("mxb_layer_norm_backward: in place, dx needs the pitch of the matrix that it replaces");
             return MXB_E_ARG;
         }
+    }
+    if (p.cols > kMaxExtent) {
+        set_error("mxb_layer_norm_backward: cols is limited to 2^30");
+        return MXB_E_UNSUPPORTED;
     }
     DeviceScope scope(ctx->device);
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;

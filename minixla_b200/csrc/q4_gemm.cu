@@ -921,6 +921,10 @@ int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, voi
         set_error("mxb_q4_gemm: A and Q need 16-byte aligned bases and row pitches (lda %% 4 == 0, ldq %% 16 == 0)");
         return MXB_E_ARG;
     }
+    if (p.M > kMaxExtent || p.N > kMaxExtent || p.K > kMaxExtent) {
+        set_error("mxb_q4_gemm: M, N and K are limited to 2^30");
+        return MXB_E_UNSUPPORTED;
+    }
     if (!take_cell_steps("mxb_q4_gemm", steps, n_steps, p.N, false, p.epi)) return MXB_E_ARG;
     DeviceScope scope(ctx->device);
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;

@@ -278,6 +278,64 @@ def test_large_groups(lib, gpu_ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("precision", [X3, TF32], ids=["3xtf32", "tf32"])
+def test_large_groups_exactly(lib, gpu_ctx, precision):
+    """Enough tiles for every SM, small integers: each product lands where it belongs, and nothing behind the groups."""
+    c = make([700, 0, 33, 1300, 256, 1], 1024, 1500, seed=15, before=1, behind=2, ints=True)
+    out, da, (db, dbias) = (f(lib, gpu_ctx, c, precision) for f in (forward, grad_a, grad_b))
+    for e in range(c["groups"]):
+        r = slice(c["at"][e], c["at"][e + 1])
+        a, dy, b = (t.double() for t in (c["a"][r], c["dy"][r], c["b"][e]))
+        assert (out[r] == a @ b).all() and (da[r] == dy @ b.t()).all()
+        assert (db[e] == a.t() @ dy).all() and (dbias[e] == dy.sum(0)).all()
+    assert (out[:1] == 77).all() and (out[-2:] == 77).all() and (da[:1] == 77).all() and (da[-2:] == 77).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [[3, 2], [60, 90], [700, 900]], ids=["few", "some", "many"])
+def test_added_to_the_output_itself(lib, gpu_ctx, sizes):
+    import torch
+
+    c = make(sizes, 96, 1400, seed=3, ints=True)
+    out = torch.randint(-9, 10, (c["rows"], c["n"]), device="cuda").float()
+    want = out.double() + torch.cat([c["a"][:sizes[0]].double() @ c["b"][0].double(),
+                                     c["a"][sizes[0]:].double() @ c["b"][1].double()])
+    forward(lib, gpu_ctx, c, st=steps((mlib.MXB_EP_ADD_FULL, out, out.stride(0), 0)), out=out)
+    assert (out == want).all()
+
+
+@pytest.mark.gpu
+def test_two_threads_share_a_context(lib, gpu_ctx):
+    """Calls from two host threads on streams of their own give what one thread gives."""
+    import threading
+
+    import torch
+
+    cases = [make([40, 0, 70], 200, 300, seed=s) for s in (1, 2)]
+    want = [(forward(lib, gpu_ctx, c), grad_a(lib, gpu_ctx, c), *grad_b(lib, gpu_ctx, c)) for c in cases]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i] = (forward(lib, gpu_ctx, cases[i]), grad_a(lib, gpu_ctx, cases[i]), *grad_b(lib, gpu_ctx, cases[i]))
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001 - reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for w, g in zip(want, got):
+        assert all((a == b).all() for a, b in zip(w, g))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("sizes", [[2, 0, 1], [60, 0, 30], [400, 0, 300]], ids=["few", "some", "many"])
 def test_captured_and_on_other_streams(lib, gpu_ctx, sizes):
     import torch
@@ -371,6 +429,13 @@ def test_block_of_an_expert_mlp_trains_and_serves(lib, gpu_ctx):
                               (out, dx, dgamma, dbeta, dw1, db1, dw2, db2), (O, *want)):
         err = ((got.double() - ref).norm() / ref.norm()).item()
         assert err <= 1e-4, (name, err)
+
+
+@pytest.mark.parametrize("which", ["mxb_grouped_gemm", "mxb_grouped_gemm_grad_a"])
+def test_extents_past_the_limit(lib, which):
+    n = (1 << 30) + 4
+    rc = getattr(lib, which)(fake_context(), 4096, n, 8192, n, 0, 12288, 1, 16384, n, 4, n, n, None, 0, X3, None)
+    assert rc == mlib.MXB_E_UNSUPPORTED and "2^30" in mlib.last_error()
 
 
 A, B, OFF, OUT = 4096, 8192, 12288, 16384

@@ -274,6 +274,29 @@ def test_streams_and_the_contexts_own(lib, gpu_ctx):
         assert all((a == b).all() for a, b in zip(g, full))
 
 
+@pytest.mark.gpu
+def test_rows_at_the_ends_of_an_allocation(lib, gpu_ctx):
+    """The copies of unaligned rows reach past a row's ends, never past the matrix's: with NaN right before and behind
+    it, and rows of every alignment, nothing changes."""
+    import torch
+
+    for cols in (1029, 2050, 4099):
+        x, dy, gamma, beta = make(9, cols, cols)
+        buf = torch.full((3, 9 * cols + 8), float("nan"), device="cuda")
+        xv, dv = (buf[i][4:4 + 9 * cols].view(9, cols).copy_(t) for i, t in ((0, x), (1, dy)))
+        y, mean, rstd = forward(lib, gpu_ctx, xv, gamma, beta)
+        check_forward(x, gamma, beta, y, mean, rstd)
+        check_backward(dy, x, gamma, mean, rstd, *backward(lib, gpu_ctx, dv, xv, gamma, mean, rstd))
+
+
+def test_columns_past_the_limit(lib):
+    n = (1 << 30) + 4
+    assert lib.mxb_layer_norm(fake_context(), 4096, n, None, None, EPS, 8192, n, None, None, 1, n, None) == mlib.MXB_E_UNSUPPORTED
+    assert lib.mxb_layer_norm_backward(fake_context(), 4096, n, 8192, n, None, 64, 64, 16384, n, None, None, 1, n,
+                                       None) == mlib.MXB_E_UNSUPPORTED
+    assert "2^30" in mlib.last_error()
+
+
 REFUSED = [
     dict(ctx=None), dict(x=None), dict(y=None), dict(cols=0), dict(rows=-1), dict(ldx=15), dict(ldy=15),
     dict(y="x", ldy=20),

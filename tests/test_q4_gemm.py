@@ -182,6 +182,43 @@ def test_captured_and_on_other_streams(lib, gpu_ctx, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 8, 16, 200])
+def test_added_to_the_output_itself(lib, gpu_ctx, m):
+    import torch
+
+    c = make(m, 300, 512, 64, seed=m)
+    c["a"] = torch.randint(-9, 10, (m, 512), device="cuda").float()
+    c["s"].fill_(1.0)
+    out = torch.randint(-9, 10, (m, 300), device="cuda").float()
+    want = out.double() + c["a"].double() @ weight(c)
+    run(lib, gpu_ctx, c, steps((mlib.MXB_EP_ADD_FULL, out, 300, 0)), out)
+    assert (out == want).all()
+
+
+@pytest.mark.gpu
+def test_norm_then_two_products_serve_a_block(lib, gpu_ctx):
+    """norm -> 4-bit product (bias, relu) -> 4-bit product added to the block's input, for one row and for a prompt,
+    the calls one after the other on one stream: within 1e-5 of the norm of the float64 block (each call is within
+    about 1e-6 of its own norm, and the block's condition is about one)."""
+    import torch
+    from tests.test_layer_norm import forward as norm
+
+    d, h = 384, 1000
+    up, down = make(1, h, d, 64, "bf16", seed=1), make(1, d, h, 128, "f16", seed=2)
+    gamma, beta, bias = torch.randn(d, device="cuda"), torch.randn(d, device="cuda"), torch.randn(h, device="cuda")
+    for m in (1, 7, 150):
+        x = torch.randn(m, d, device="cuda")
+        y, _, _ = norm(lib, gpu_ctx, x, gamma, beta)
+        hid = run(lib, gpu_ctx, dict(up, a=y, m=m), steps((mlib.MXB_EP_ADD_ROW, bias, 0, 0), (mlib.MXB_EP_RELU, None, 0, 0)))
+        out = run(lib, gpu_ctx, dict(down, a=hid, m=m), steps((mlib.MXB_EP_ADD_FULL, x, d, 0)))
+        X = x.double()
+        c = X - X.mean(1, keepdim=True)
+        Y = c * (c.square().mean(1, keepdim=True) + 1e-5).rsqrt() * gamma.double() + beta.double()
+        want = torch.relu(Y @ weight(up) + bias.double()) @ weight(down) + X
+        assert ((out.double() - want).norm() / want.norm()).item() <= 1e-5
+
+
+@pytest.mark.gpu
 def test_weight_past_32_bit_offsets(lib, gpu_ctx):
     """A weight of more than 2^32 bytes: the last columns are read at their place."""
     import torch
