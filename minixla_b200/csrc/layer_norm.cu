@@ -180,23 +180,36 @@ __device__ __forceinline__ RowSpan row_span(const RowSource& m, long long row, l
 
 __host__ __device__ constexpr int row_slot_bytes(int cols) { return (cols * 4 + 12 + 15) / 16 * 16; }
 
+__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
 template <int MATS>
 struct RowRing {
     RowSource mats[MATS];
-    uint8_t* slots;
+    uint32_t slots;         // shared addresses
     uint32_t bar0;
+    int (*skip)[MATS];      // of each slot: floats before its row's first, or -1 where the row is read directly
     int n, cols;
     long long rows;
 
-    // Asks for `row` into `slot`; one thread.
+    // Asks for `row` into `slot`; one thread.  (What it leaves in `skip` is released by its arrival at the barrier.)
     __device__ __forceinline__ void ask(long long row, int slot) const {
-        const uint32_t bar = bar0 + 8 * slot, dst = smem_addr(slots) + slot * MATS * row_slot_bytes(cols);
+        const uint32_t bar = bar0 + 8 * slot, dst = slots + slot * MATS * row_slot_bytes(cols);
         RowSpan s[MATS];
         uint32_t bytes = 0;
 #pragma unroll
         for (int m = 0; m < MATS; ++m) {
             s[m] = row_span(mats[m], row, rows, cols);
             bytes += s[m].inside ? s[m].bytes : 0;
+            skip[slot][m] = s[m].inside ? static_cast<int>(s[m].skip) : -1;
         }
         mbar_arrive_expect_tx(bar, bytes);
 #pragma unroll
@@ -204,28 +217,35 @@ struct RowRing {
             if (s[m].inside)
                 bulk_load(dst + m * row_slot_bytes(cols), reinterpret_cast<const void*>(s[m].begin), s[m].bytes, bar);
     }
-    // Where a thread finds matrix m's row: in its slot or, at the matrix's ends, where it lies.
-    __device__ __forceinline__ const float* find(int m, long long row, int slot) const {
-        const RowSpan s = row_span(mats[m], row, rows, cols);
-        if (!s.inside) return mats[m].base + row * mats[m].ld;
-        return reinterpret_cast<const float*>(slots + (slot * MATS + m) * row_slot_bytes(cols)) + s.skip;
+
+    // This thread's units of matrix m's row: from its slot or, at the matrix's ends, from where it lies.
+    template <int W, int NV>
+    __device__ __forceinline__ void take(float (&v)[NV][W], int m, long long row, int slot, int t, int threads) const {
+        const int ahead = skip[slot][m];
+        if (ahead >= 0) {
+            const uint32_t at = slots + (slot * MATS + m) * row_slot_bytes(cols) + (ahead + t * W) * 4;
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
+                const int c = (u * threads + t) * W;
+                if (W == 4 && c + W <= cols) {
+                    const float4 x = ld_shared_v4(at + u * threads * W * 4);
+                    v[u][0] = x.x;
+                    v[u][W > 1 ? 1 : 0] = x.y;
+                    v[u][W > 2 ? 2 : 0] = x.z;
+                    v[u][W > 3 ? 3 : 0] = x.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+                        v[u][i] = c + i < cols ? ld_shared_f32(at + (u * threads * W + i) * 4) : 0.0f;
+                }
+            }
+        } else {
+            const float* p = mats[m].base + row * mats[m].ld;
+#pragma unroll
+            for (int u = 0; u < NV; ++u) load_unit<W>(v[u], p, (u * threads + t) * W, cols);
+        }
     }
 };
-
-// W consecutive floats at p + c of a row in a slot (generic address), zeros from column `cols` on.
-template <int W>
-__device__ __forceinline__ void take_unit(float (&v)[W], const float* p, int c, int cols) {
-    if (W == 4 && c + W <= cols) {
-        const float4 t = *reinterpret_cast<const float4*>(p + c);
-        v[0] = t.x;
-        v[W > 1 ? 1 : 0] = t.y;
-        v[W > 2 ? 2 : 0] = t.z;
-        v[W > 3 ? 3 : 0] = t.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = c + i < cols ? p[c + i] : 0.0f;
-    }
-}
 
 constexpr int kWarpRowThreads = 256;  // blocks of eight warps, a row each
 
@@ -319,7 +339,8 @@ __global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_block_kern
     __shared__ int failed;  // the first round whose copy did not arrive: every thread leaves in that round
     extern __shared__ __align__(16) uint8_t ring_smem[];
     RowSum<false> row_sum{buf};
-    const RowRing<1> ring{{{p.x, p.ldx}}, ring_smem, smem_addr(bars), slots, p.cols, p.rows};
+    __shared__ int skip[kMaxSlots][1];
+    const RowRing<1> ring{{{p.x, p.ldx}}, smem_addr(ring_smem), smem_addr(bars), skip, slots, p.cols, p.rows};
     const int threads = blockDim.x, t = threadIdx.x;
     const float inv = 1.0f / static_cast<float>(p.cols);
     if (t == 0) {
@@ -337,10 +358,8 @@ __global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_block_kern
     uint32_t phase = 0;
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, ++round) {
         if (!mbar_wait(ring.bar0 + 8 * slot, phase, p.timeout_ns)) atomicMin(&failed, round);
-        const float* x = ring.find(0, row, slot);
         float v[NV][W];
-#pragma unroll
-        for (int u = 0; u < NV; ++u) take_unit<W>(v[u], x, (u * threads + t) * W, p.cols);
+        ring.take(v, 0, row, slot, t, threads);
         // The first sum's barrier says that every thread has taken its part: the slot can be filled again.
         bool first = true;
         const NormStats st = norm_stats<W, NV>(v, t, threads, p, inv, [&](float s) {
@@ -495,7 +514,8 @@ __global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_grad_block
     __shared__ int failed;  // the first round whose copy did not arrive: every thread leaves in that round
     extern __shared__ __align__(16) uint8_t smem[];
     RowSum<false> row_sum{buf};
-    const RowRing<2> ring{{{p.x, p.ldx}, {p.dy, p.lddy}}, smem, smem_addr(bars), slots, p.cols, p.rows};
+    __shared__ int skip[kMaxSlots][2];
+    const RowRing<2> ring{{{p.x, p.ldx}, {p.dy, p.lddy}}, smem_addr(smem), smem_addr(bars), skip, slots, p.cols, p.rows};
     const int threads = blockDim.x, t = threadIdx.x;
     const float inv = 1.0f / static_cast<float>(p.cols);
     if (t == 0) {
@@ -518,14 +538,9 @@ __global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_grad_block
         const NormStats st = next;
         next = saved_stats(p, row + gridDim.x);
         if (!mbar_wait(ring.bar0 + 8 * slot, phase, p.timeout_ns)) atomicMin(&failed, round);
-        const float* x = ring.find(0, row, slot);
-        const float* dy = ring.find(1, row, slot);
         float xh[NV][W], d[NV][W];
-#pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            take_unit<W>(xh[u], x, (u * threads + t) * W, p.cols);
-            take_unit<W>(d[u], dy, (u * threads + t) * W, p.cols);
-        }
+        ring.take(xh, 0, row, slot, t, threads);
+        ring.take(d, 1, row, slot, t, threads);
         // The sum's barrier says that every thread has taken its part: the slot can be filled again.
         norm_grad_row<W, NV>(xh, d, dg, db, gamma, st, t, threads, row, p, inv, [&](float2 s) {
             s = row_sum(s);
