@@ -651,8 +651,12 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
 // as possible: by the MMA once for big, against big and small activations side
 // by side (columns 0 .. n and n .. 2n of one MMA), and once by the
 // converter, a thread to a weight column, which leaves the small parts in
-// tensor memory, from where the second MMA takes them as its A operand.
-// That is 72 KB a k-block (of 32) where the kernel above moves 120.
+// tensor memory, from where the second MMA takes them as its A operand (and
+// adds to the columns of the other small term: the main columns then see
+// a third of the sums that the tensor core cuts).  That is 72 KB a k-block (of
+// 32) where the kernel above moves 120.  Small parts as bf16 pairs, half the
+// tensor memory and MMAs, were no faster (92 us either way at 128 rows, 64 groups of
+// 1024 x 2048) and less exact.
 //
 // With fewer tiles than SMs, a cluster of `splits` CTAs shares a tile, each
 // summing its own stretch of the sum; the totals meet in distributed shared
@@ -669,7 +673,7 @@ struct GroupedFewCfg {
     static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 2);
     static constexpr int kSmallCol = 4 * kCols;       // first TMEM column behind the two accumulators of 64
     static constexpr int kTmemCols = 256;
-    static constexpr int kSegKb = 2;                  // k-blocks to an accumulator: 16 sums into each column
+    static constexpr int kSegKb = 4;                  // k-blocks to an accumulator: 16 sums into a main column
     static constexpr int kTableOffset = kStages * kStageBytes;
     static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
     static constexpr int kNumBars = 2 * kStages + 2 * kSmall + 4 + 1;
@@ -823,7 +827,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
                         if (kk >= steps) break;
                         const uint64_t db = smem_desc_of(kHiK, bc + kk * 2);
                         mma_tf32(d, smem_desc_of(kLaneHi, bl + kk * kLaneStep), db, both, kk ? 1u : begun);
-                        if (p.split3) mma_tf32_ts(d, a_small + kk * 8, db, one, 1u);
+                        if (p.split3) mma_tf32_ts(d + n, a_small + kk * 8, db, one, 1u);
                     }
                     mma_commit(empty_bar(stage));
                     mma_commit(sfree_bar(small));
