@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const uint32_t bar0 = smem_addr(bars);
-    auto full_bar = [&](int s) { return bar0 + 8u * s; };                         // TMA -> converter, MMA
+    auto full_bar = [&](int s) { return bar0 + 8u * s; };                         // TMA -> converter (whose arrival passes it on to the MMA)
     auto empty_bar = [&](int s) { return bar0 + 8u * (C::kStages + s); };         // MMA -> TMA
     auto conv_bar = [&](int s) { return bar0 + 8u * (2 * C::kStages + s); };      // converter -> MMA
     auto sfree_bar = [&](int s) { return bar0 + 8u * (2 * C::kStages + C::kSmall + s); };  // MMA -> converter
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
             constexpr uint32_t kLaneStep = kLaneMn ? 64 : 2, kColStep = kColMn ? 64 : 2;
             const bool leader = elect_one();
             int stage = 0, small = 0, acc = 0;
-            uint32_t phase = 0, small_phase = 0, acc_phase = 0;
+            uint32_t small_phase = 0, acc_phase = 0;
             bool ok = true;
             for (int round = 0; ok; ++round) {
                     const int t = grouped_turn(round, team, teams, total_tiles);
@@ -455,8 +455,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                 for (int kb = kb0; kb < kb1; ++kb) {
                     bool ready = *abort_flag == 0;
                     if (ready && in_seg == 0) ready = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
-                    if (!ready || !mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
-                        !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
+                    if (!ready || !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
                         ok = false;
                         break;
                     }
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                         mma_commit(sfree_bar(small));
                         if (end_seg) mma_commit(tfull_bar(acc));
                     }
-                    if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                    if (++stage == C::kStages) stage = 0;
                     if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
                     if (end_seg) {
                         in_seg = 0;
@@ -669,8 +668,11 @@ struct GroupedFewCfg {
     static constexpr int kStageBytes = kLaneBytes + kColBytes;
     static constexpr int kStages = 8;
     static constexpr int kSmall = 4;                  // small weights in tensor memory: 32 columns each
-    static constexpr int kEpiWarps = 4, kConvWarps = 8;
-    static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 2);
+    static constexpr int kEpiWarps = 4, kConvGroups = 3, kConvWarps = 4 * kConvGroups;
+    static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 4);  // and a warpgroup with TMA and MMA
+    // Registers a thread: the launch has 640 x 96, given out in shares of 128 threads.
+    static constexpr int kEpiRegs = 144, kConvRegs = 88, kIssueRegs = 72;
+    static_assert(kEpiRegs + kConvGroups * kConvRegs + kIssueRegs <= 480, "more registers than the launch has");
     static constexpr int kSmallCol = 4 * kCols;       // first TMEM column behind the two accumulators of 64
     static constexpr int kTmemCols = 256;
     static constexpr int kSegKb = 4;                  // k-blocks to an accumulator: 16 sums into a main column
@@ -714,7 +716,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
             mbar_init(empty_bar(s), 1);
         }
         for (int s = 0; s < C::kSmall; ++s) {
-            mbar_init(conv_bar(s), C::kConvWarps);
+            mbar_init(conv_bar(s), 4);  // a group of the converter
             mbar_init(sfree_bar(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -744,77 +746,77 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
     const int kb0 = static_cast<int>(static_cast<long long>(all_kb) * rank / splits);
     const int kb1 = static_cast<int>(static_cast<long long>(all_kb) * (rank + 1) / splits);
 
-    if (warp == kTmaWarp) {
-        // ------------------------------------------------------------ TMA producer
-        const bool leader = elect_one();
-        int stage = 0;
-        uint32_t phase = 0;
-        long long issued = 0;
-        bool ok = true;
-        for (int round = 0; ok; ++round) {
-            const int t = grouped_turn(round, team, teams, total_tiles);
-            if (t == -2) break;
-            if (t < 0) continue;
-            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
-                    ok = false;
-                    break;
-                }
-                if (leader) {
-                    const uint32_t st = smem_addr(smem + stage * C::kStageBytes), fb = full_bar(stage);
-                    mbar_arrive_expect_tx(fb, C::kLaneBytes + kBoxBytes);
-                    const int q0 = kb * kBK;
-                    if (MODE == kForward) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, q0, g.group);
-                    } else {
-                        tma_load_3d(st, &tm_lane, fb, q0, g.lane0, g.group);
+    if (warp >= kTmaWarp) {
+        fewer_registers<C::kIssueRegs>();
+        if (warp == kTmaWarp) {
+            // ------------------------------------------------------------ TMA producer
+            const bool leader = elect_one();
+            int stage = 0;
+            uint32_t phase = 0;
+            long long issued = 0;
+            bool ok = true;
+            for (int round = 0; ok; ++round) {
+                const int t = grouped_turn(round, team, teams, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
+                const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
+                        ok = false;
+                        break;
                     }
-                    tma_load_2d(st + C::kLaneBytes, &tm_col, fb, q0, g.row0 + g.col0);
+                    if (leader) {
+                        const uint32_t st = smem_addr(smem + stage * C::kStageBytes), fb = full_bar(stage);
+                        mbar_arrive_expect_tx(fb, C::kLaneBytes + kBoxBytes);
+                        const int q0 = kb * kBK;
+                        if (MODE == kForward) {
+    #pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, q0, g.group);
+                        } else {
+                            tma_load_3d(st, &tm_lane, fb, q0, g.lane0, g.group);
+                        }
+                        tma_load_2d(st + C::kLaneBytes, &tm_col, fb, q0, g.row0 + g.col0);
+                    }
+                    __syncwarp();
+                    ++issued;
+                    if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
                 }
-                __syncwarp();
-                ++issued;
-                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
             }
-        }
-        if (!ok && leader) {
-            raise_grouped(p, abort_flag, kErrProducer);
-            // Copies in flight land in this CTA's shared memory: wait for them before leaving.
-            for (long long i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
-                mbar_wait(full_bar(static_cast<int>(i % C::kStages)), static_cast<uint32_t>((i / C::kStages) & 1),
-                          p.timeout_ns);
-        }
-        __syncwarp();
-    } else if (warp == kMmaWarp) {
-        // ------------------------------------------------------------ MMA issuer
-        constexpr uint32_t kHiMn = smem_desc_hi(512, kLayoutSW128Base32B), kHiK = smem_desc_hi(1024, kLayoutSW128);
-        constexpr uint32_t kLaneHi = kLaneMn ? kHiMn : kHiK, kLaneStep = kLaneMn ? 64 : 2;
-        const bool leader = elect_one();
-        int stage = 0, small = 0, acc = 0;
-        uint32_t phase = 0, small_phase = 0, acc_phase = 0;
-        bool ok = true;
-        for (int round = 0; ok; ++round) {
-            const int t = grouped_turn(round, team, teams, total_tiles);
-            if (t == -2) break;
-            if (t < 0) continue;
-            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
-            const int n = (g.cols + 15) & ~15;
-            const uint32_t both = idesc_tf32_major(128, p.split3 ? 2 * n : n, kLaneMn, 0);
-            const uint32_t one = idesc_tf32_major(128, n, 0, 0);  // (A in tensor memory is K-major)
-            int in_seg = 0;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                bool ready = *abort_flag == 0;
-                if (ready && in_seg == 0) ready = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
-                if (!ready || !mbar_wait(full_bar(stage), phase, p.timeout_ns) ||
-                    !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const bool end_seg = ++in_seg == C::kSegKb || kb == kb1 - 1;
-                if (leader) {
+            if (!ok && leader) {
+                raise_grouped(p, abort_flag, kErrProducer);
+                // Copies in flight land in this CTA's shared memory: wait for them before leaving.
+                for (long long i = issued > C::kStages ? issued - C::kStages : 0; i < issued; ++i)
+                    mbar_wait(full_bar(static_cast<int>(i % C::kStages)), static_cast<uint32_t>((i / C::kStages) & 1),
+                              p.timeout_ns);
+            }
+            __syncwarp();
+        } else if (warp == kMmaWarp) {
+            // ------------------------------------------------------------ MMA issuer
+            constexpr uint32_t kHiMn = smem_desc_hi(512, kLayoutSW128Base32B), kHiK = smem_desc_hi(1024, kLayoutSW128);
+            constexpr uint32_t kLaneHi = kLaneMn ? kHiMn : kHiK, kLaneStep = kLaneMn ? 64 : 2;
+            const uint32_t leader = elect_one();
+            int stage = 0, small = 0, acc = 0;
+            uint32_t small_phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int round = 0; ok; ++round) {
+                const int t = grouped_turn(round, team, teams, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
+                const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+                const int n = (g.cols + 15) & ~15;
+                const uint32_t both = idesc_tf32_major(128, p.split3 ? 2 * n : n, kLaneMn, 0);
+                const uint32_t one = idesc_tf32_major(128, n, 0, 0);  // (A in tensor memory is K-major)
+                int in_seg = 0;
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    bool ready = *abort_flag == 0;
+                    if (ready && in_seg == 0) ready = mbar_wait(tempty_bar(acc), acc_phase ^ 1u, p.timeout_ns);
+                    if (!ready || !mbar_wait(conv_bar(small), small_phase, p.timeout_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const bool end_seg = ++in_seg == C::kSegKb || kb == kb1 - 1;
                     const uint32_t d = tmem_base + static_cast<uint32_t>(acc * 2 * BT);
                     const uint32_t a_small = tmem_base + static_cast<uint32_t>(C::kSmallCol + 32 * small);
                     const uint32_t big = smem_addr(smem + stage * C::kStageBytes);
@@ -822,39 +824,43 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
                     const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, 16);
                     const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
                     const uint32_t begun = in_seg > 1 ? 1u : 0u;
-#pragma unroll
+    #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         if (kk >= steps) break;
                         const uint64_t db = smem_desc_of(kHiK, bc + kk * 2);
-                        mma_tf32(d, smem_desc_of(kLaneHi, bl + kk * kLaneStep), db, both, kk ? 1u : begun);
-                        if (p.split3) mma_tf32_ts(d + n, a_small + kk * 8, db, one, 1u);
+                        mma_tf32_of(leader, d, smem_desc_of(kLaneHi, bl + kk * kLaneStep), db, both, kk ? 1u : begun);
+                        if (p.split3) mma_tf32_ts_of(leader, d + n, a_small + kk * 8, db, one, 1u);
                     }
-                    mma_commit(empty_bar(stage));
-                    mma_commit(sfree_bar(small));
-                    if (end_seg) mma_commit(tfull_bar(acc));
-                }
-                __syncwarp();
-                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
-                if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
-                if (end_seg) {
-                    in_seg = 0;
-                    acc ^= 1;
-                    if (acc == 0) acc_phase ^= 1u;
+                    if (leader) {
+                        mma_commit(empty_bar(stage));
+                        mma_commit(sfree_bar(small));
+                        if (end_seg) mma_commit(tfull_bar(acc));
+                    }
+                    __syncwarp();
+                    if (++stage == C::kStages) stage = 0;
+                    if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
+                    if (end_seg) {
+                        in_seg = 0;
+                        acc ^= 1;
+                        if (acc == 0) acc_phase ^= 1u;
+                    }
                 }
             }
+            if (leader) {
+                if (!ok) raise_grouped(p, abort_flag, kErrMma);
+                mma_commit(drain_bar);
+                if (!mbar_wait(drain_bar, 0, p.timeout_ns)) raise_grouped(p, abort_flag, kErrMma);
+            }
+            __syncwarp();
         }
-        if (leader) {
-            if (!ok) raise_grouped(p, abort_flag, kErrMma);
-            mma_commit(drain_bar);
-            if (!mbar_wait(drain_bar, 0, p.timeout_ns)) raise_grouped(p, abort_flag, kErrMma);
-        }
-        __syncwarp();
     } else if (warp >= kConvWarp) {
-        // ------------------------------------------------------------ converter: a weight column and 16 k a thread
-        const int t0 = threadIdx.x - 32 * kConvWarp, row = t0 & 127, half = t0 >> 7;
-        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(row & ~31) << 16) + C::kSmallCol + 16 * half;
-        int stage = 0, small = 0;
-        uint32_t phase = 0, small_phase = 0;
+        // ------------------------------------------------------------ converter: a weight column a thread
+        fewer_registers<C::kConvRegs>();
+        // Each group of four warps takes every kConvGroups-th k-block: what a k-block costs besides the work (three
+        // waits of about 130 clocks) is then paid once for 32 k a thread.
+        const int t0 = threadIdx.x - 32 * kConvWarp, row = t0 & 127, turn = t0 >> 7;
+        const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(row & ~31) << 16) + C::kSmallCol;
+        unsigned count = 0;  // k-blocks so far
         bool failed = false;
         for (int round = 0; !failed; ++round) {
             const int t = grouped_turn(round, team, teams, total_tiles);
@@ -862,10 +868,12 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
             if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
             const int n = (g.cols + 15) & ~15;
-            for (int kb = kb0; kb < kb1; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb, ++count) {
+                if (static_cast<int>(count % C::kConvGroups) != turn) continue;
+                const int stage = static_cast<int>(count % C::kStages), small = static_cast<int>(count % C::kSmall);
                 const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
-                const bool got = !stop && mbar_wait(full_bar(stage), phase, p.timeout_ns) &&
-                                 mbar_wait(sfree_bar(small), small_phase ^ 1u, p.timeout_ns);
+                const bool got = !stop && mbar_wait(full_bar(stage), (count / C::kStages) & 1u, p.timeout_ns) &&
+                                 mbar_wait(sfree_bar(small), ((count / C::kSmall) & 1u) ^ 1u, p.timeout_ns);
                 if (!__all_sync(0xffffffffu, got)) {
                     if (lane == 0 && !stop) raise_grouped(p, abort_flag, kErrProducer);
                     failed = true;
@@ -874,44 +882,47 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
                 if (p.split3) {
                     tc_fence_after();
                     const uint8_t* st = smem + stage * C::kStageBytes;
-                    uint32_t r[16];
-                    if (kLaneMn) {
-                        // [k][n]: box n / 32, 128 bytes a k, its 32-byte chunks swizzled by k % 4.
-                        const uint8_t* src = st + (row >> 5) * kBoxBytes + half * 16 * 128 + (row & 7) * 4;
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            r[k] = __float_as_uint(small_of(
-                                *reinterpret_cast<const float*>(src + k * 128 + ((((row >> 3) & 3) ^ (k & 3)) << 5))));
-                    } else {
-                        // [n][k]: 128 bytes a weight column, 16-byte chunks swizzled by n % 8.
-                        const uint8_t* src = st + row * 128;
+                    for (int half = 0; half < 2; ++half) {  // (16 k at a time: fewer registers)
+                        uint32_t r[16];
+                        if (kLaneMn) {
+                            // [k][n]: box n / 32, 128 bytes a k, its 32-byte chunks swizzled by k % 4.
+                            const uint8_t* src = st + (row >> 5) * kBoxBytes + half * 16 * 128 + (row & 7) * 4;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const float4 v = *reinterpret_cast<const float4*>(src + (((half * 4 + c) ^ (row & 7)) << 4));
-                            r[4 * c] = __float_as_uint(small_of(v.x));
-                            r[4 * c + 1] = __float_as_uint(small_of(v.y));
-                            r[4 * c + 2] = __float_as_uint(small_of(v.z));
-                            r[4 * c + 3] = __float_as_uint(small_of(v.w));
+                            for (int k = 0; k < 16; ++k)
+                                r[k] = __float_as_uint(small_of(
+                                    *reinterpret_cast<const float*>(src + k * 128 + ((((row >> 3) & 3) ^ (k & 3)) << 5))));
+                        } else {
+                            // [n][k]: 128 bytes a weight column, 16-byte chunks swizzled by n % 8.
+                            const uint8_t* src = st + row * 128;
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                const float4 v = *reinterpret_cast<const float4*>(src + (((4 * half + c) ^ (row & 7)) << 4));
+                                r[4 * c] = __float_as_uint(small_of(v.x));
+                                r[4 * c + 1] = __float_as_uint(small_of(v.y));
+                                r[4 * c + 2] = __float_as_uint(small_of(v.z));
+                                r[4 * c + 3] = __float_as_uint(small_of(v.w));
+                            }
                         }
+                        tmem_st_32x32b_x16(lane_base + static_cast<uint32_t>(32 * small + 16 * half), r);
                     }
-                    tmem_st_32x32b_x16(lane_base + static_cast<uint32_t>(32 * small), r);
                     // The activations' small parts go behind them, to rows n .. 2n of the same swizzled tile.
                     float4* x = reinterpret_cast<float4*>(smem + stage * C::kStageBytes + C::kLaneBytes);
-                    const float4 v = x[t0];
-                    __syncwarp();
-                    if (t0 < n * 8) x[t0 + n * 8] = make_float4(small_of(v.x), small_of(v.y), small_of(v.z), small_of(v.w));
+                    for (int i = row; i < n * 8; i += 128) {
+                        const float4 v = x[i];
+                        x[i + n * 8] = make_float4(small_of(v.x), small_of(v.y), small_of(v.z), small_of(v.w));
+                    }
                     tmem_st_wait();
                     fence_proxy_async_shared();
                     tc_fence_before();
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(conv_bar(small));
-                if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
-                if (++small == C::kSmall) { small = 0; small_phase ^= 1u; }
             }
         }
     } else {
         // ------------------------------------------------------------ epilogue: a result column and 32 rows a thread
+        more_registers<C::kEpiRegs>();
         constexpr int W = 16;
         const int quad = warp & 3;
         const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
