@@ -4,8 +4,11 @@
 //   grad_a   dA[r, k]    = epi(sum over n of dY[r, n] * B_e[k, n])
 //   grad_b   dB_e[k, n]  = sum over the group's rows r of A[r, k] * dY[r, n],  dbias[e, n] = sum over r of dY[r, n]
 //
-// All three run on one tcgen05 kernel.  The tile is turned around compared
-// with the dense GEMMs: the dimension along which the result is contiguous
+// Three tcgen05 kernels: pairs of CTAs with tiles of 256 x 256 where groups
+// have many rows (all three products), a CTA with at most 64 rows to a tile
+// where they have few (forward, grad_a), and a CTA with 128 x 128 for grad_b's
+// small matrices.  run_grouped_mode has the rule.  The tile is turned around
+// compared with the dense GEMMs: the dimension along which the result is contiguous
 // (n, or k in grad_a) lies along the tensor core's 128 rows and TMEM lanes,
 // the ragged dimension (the group's rows; k in grad_b) along its columns.
 // A group with few rows then costs an MMA of 16 columns instead of 128 rows,
@@ -20,12 +23,12 @@
 //
 // 3xTF32: x = big + small, three TF32 products.  The tensor core itself cuts
 // an fp32 operand to its upper 19 bits, so the tile that TMA loaded serves as
-// big, and four warps write small = x - big (rounded to the nearest TF32) to a
-// second tile: no pass over the weights beforehand, which would cost two to
+// big, and converter warps write small = x - big (rounded to the nearest TF32)
+// to a second tile or to tensor memory: no pass over the weights beforehand, which would cost two to
 // three times the bytes of the product where a group has few rows.  K is
-// summed in segments of 64, each in a fresh accumulator, because the tensor
-// core cuts its running sums toward zero; the epilogue warps add the segments
-// in fp32 registers.
+// summed in segments of 64 or 128, each in a fresh accumulator, because the
+// tensor core cuts its running sums toward zero; the epilogue warps add the
+// segments in fp32 registers.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -74,11 +77,10 @@ struct GroupedParams {
 
 constexpr int kGroupedTableBytes = 20 * MXB_MAX_GROUPS + 128 * 4 + 16;
 
-// BT: tile columns, the most rows of a group (grad_b: columns of A) that one tile takes.
-template <int BT>
-struct GroupedCfg {
+struct GroupedGradBCfg {
+    static constexpr int kCols = 128;                 // columns of A that a tile takes
     static constexpr int kLaneBytes = 128 * kBK * 4;
-    static constexpr int kColBytes = BT * kBK * 4;
+    static constexpr int kColBytes = kCols * kBK * 4;
     static constexpr int kStageBytes = kLaneBytes + kColBytes;
     static constexpr int kStages = 4;                 // tiles as loaded
     static constexpr int kSmall = 2;                  // their small parts
@@ -88,8 +90,8 @@ struct GroupedCfg {
     // Registers a thread: the launch has 640 x 96, given out in shares of 128 threads.
     static constexpr int kEpiRegs = 144, kConvRegs = 64, kIssueRegs = 64;
     static_assert(2 * kEpiRegs + 2 * kConvRegs + kIssueRegs <= 480, "more registers than the launch has");
-    static constexpr int kTmemCols = 2 * BT;          // two segment buffers
-    static constexpr int kTotals = BT * 4 / kEpiWarps;  // columns of one epilogue thread
+    static constexpr int kTmemCols = 2 * kCols;          // two segment buffers
+    static constexpr int kTotals = kCols * 4 / kEpiWarps;  // columns of one epilogue thread
     static constexpr int kSmallOffset = kStages * kStageBytes;
     static constexpr int kTableOffset = kSmallOffset + kSmall * kStageBytes;
     static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
@@ -310,12 +312,15 @@ __device__ __forceinline__ void raise_grouped(const GroupedParams& p, volatile i
 
 constexpr int kGroupedSegKb = 2;  // k-blocks (of 32) to an accumulator
 
-template <int MODE, int BT>
-__global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
-    grouped_gemm_kernel(const __grid_constant__ CUtensorMap tm_lane, const __grid_constant__ CUtensorMap tm_col,
+// grad_b with K too small for pairs, or too few tiles for all of them: 128 x
+// 128 of dB_e to a CTA, or to a cluster that splits the group's rows, both
+// operands MN-major as they lie.  Bound by shared memory (120 KB a k-block for
+// 3xTF32) where there are many rows.
+__global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
+    grouped_grad_b_kernel(const __grid_constant__ CUtensorMap tm_lane, const __grid_constant__ CUtensorMap tm_col,
                         const __grid_constant__ GroupedParams p, const int splits) {
-    using C = GroupedCfg<BT>;
-    constexpr bool kLaneMn = MODE != kGradA, kColMn = MODE == kGradB;
+    using C = GroupedGradBCfg;
+    constexpr int BT = C::kCols;
     extern __shared__ uint8_t smem_raw[];
     // (an offset, not a rounded pointer: the compiler then still knows that these are shared addresses)
     uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -359,7 +364,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
         tmem_relinquish();
     } else if (warp == kConvWarp) {
-        grouped_scan<MODE, BT>(tab, p, lane);
+        grouped_scan<kGradB, BT>(tab, p, lane);
     }
     tc_fence_before();
     __syncthreads();
@@ -386,7 +391,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                     const int t = grouped_turn(round, team, teams, total_tiles);
                     if (t == -2) break;
                     if (t < 0) continue;
-                    const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+                    const GroupedTile g = grouped_tile<kGradB, BT>(tab, t, p);
                     const int col_boxes = (g.cols + 31) / 32;
                     int kb0;
                 const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
@@ -400,25 +405,11 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                         const uint32_t fb = full_bar(stage);
                         mbar_arrive_expect_tx(fb, C::kLaneBytes + col_boxes * kBoxBytes);
                         const int q0 = kb * kBK;
-                        if (MODE == kForward) {
-    #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, q0, g.group);
-                        } else if (MODE == kGradA) {
-                            tma_load_3d(st, &tm_lane, fb, q0, g.lane0, g.group);
-                        } else {
-    #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                tma_load_2d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, g.row0 + q0);
-                        }
-                        for (int j = 0; j < col_boxes; ++j) {
-                            const uint32_t dst = st + C::kLaneBytes + j * kBoxBytes;
-                            if (MODE == kGradB) {
-                                tma_load_2d(dst, &tm_col, fb, g.col0 + 32 * j, g.row0 + q0);
-                            } else {
-                                tma_load_2d(dst, &tm_col, fb, q0, g.row0 + g.col0 + 32 * j);
-                            }
-                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            tma_load_2d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, g.row0 + q0);
+                        for (int j = 0; j < col_boxes; ++j)
+                            tma_load_2d(st + C::kLaneBytes + j * kBoxBytes, &tm_col, fb, g.col0 + 32 * j, g.row0 + q0);
                         ++issued;
                         if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
                     }
@@ -435,10 +426,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
             }
         } else if (warp == kMmaWarp) {
             // ------------------------------------------------------------ MMA issuer
-            // K-major operand: 32 bytes of a 128-byte row for each 8 of the sum; MN-major: 8 rows of 128 bytes.
-            constexpr uint32_t kHiMn = smem_desc_hi(512, kLayoutSW128Base32B), kHiK = smem_desc_hi(1024, kLayoutSW128);
-            constexpr uint32_t kLaneHi = kLaneMn ? kHiMn : kHiK, kColHi = kColMn ? kHiMn : kHiK;
-            constexpr uint32_t kLaneStep = kLaneMn ? 64 : 2, kColStep = kColMn ? 64 : 2;
+            constexpr uint32_t kHi = smem_desc_hi(512, kLayoutSW128Base32B), kStep = 64;  // 8 rows of 128 bytes
             const bool leader = elect_one();
             int stage = 0, small = 0, acc = 0;
             uint32_t small_phase = 0, acc_phase = 0;
@@ -447,8 +435,8 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                     const int t = grouped_turn(round, team, teams, total_tiles);
                     if (t == -2) break;
                     if (t < 0) continue;
-                const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
-                const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, kLaneMn, kColMn);
+                const GroupedTile g = grouped_tile<kGradB, BT>(tab, t, p);
+                const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, 1, 1);
                 int kb0;
                 const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
                 int in_seg = 0;
@@ -465,22 +453,22 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                         const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BT);
                         const uint32_t big = smem_addr(smem + stage * C::kStageBytes);
                         const uint32_t low = smem_addr(smem + C::kSmallOffset + small * C::kStageBytes);
-                        const uint32_t bl = smem_desc_lo(big, kLaneMn ? kBoxBytes : 16);
-                        const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, kColMn ? kBoxBytes : 16);
-                        const uint32_t sl = smem_desc_lo(low, kLaneMn ? kBoxBytes : 16);
-                        const uint32_t sc = smem_desc_lo(low + C::kLaneBytes, kColMn ? kBoxBytes : 16);
+                        const uint32_t bl = smem_desc_lo(big, kBoxBytes);
+                        const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, kBoxBytes);
+                        const uint32_t sl = smem_desc_lo(low, kBoxBytes);
+                        const uint32_t sc = smem_desc_lo(low + C::kLaneBytes, kBoxBytes);
                         // The last k-block ends with its own eighth: nothing past the sum is multiplied.
                         const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
                         const uint32_t begun = in_seg > 1 ? 1u : 0u;
     #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
                             if (kk >= steps) break;
-                            const uint64_t da = smem_desc_of(kLaneHi, bl + kk * kLaneStep);
-                            const uint64_t db = smem_desc_of(kColHi, bc + kk * kColStep);
+                            const uint64_t da = smem_desc_of(kHi, bl + kk * kStep);
+                            const uint64_t db = smem_desc_of(kHi, bc + kk * kStep);
                             if (p.split3) {
                                 // Small cross terms first, the dominant product last.
-                                mma_tf32(d, da, smem_desc_of(kColHi, sc + kk * kColStep), idesc, kk ? 1u : begun);
-                                mma_tf32(d, smem_desc_of(kLaneHi, sl + kk * kLaneStep), db, idesc, 1u);
+                                mma_tf32(d, da, smem_desc_of(kHi, sc + kk * kStep), idesc, kk ? 1u : begun);
+                                mma_tf32(d, smem_desc_of(kHi, sl + kk * kStep), db, idesc, 1u);
                                 mma_tf32(d, da, db, idesc, 1u);
                             } else {
                                 mma_tf32(d, da, db, idesc, kk ? 1u : begun);
@@ -517,7 +505,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                 const int t = grouped_turn(round, team, teams, total_tiles);
                 if (t == -2) break;
                 if (t < 0) continue;
-            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            const GroupedTile g = grouped_tile<kGradB, BT>(tab, t, p);
             const int col_boxes = (g.cols + 31) / 32;
             int kb0;
                 const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
@@ -530,8 +518,9 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                     failed = true;
                     break;
                 }
-                convert_tile<MODE, 32 * C::kConvWarps>(smem + stage * C::kStageBytes, smem + C::kSmallOffset + small * C::kStageBytes, t0,
-                                        1024 + col_boxes * 256, g.sum - kb * kBK, p.split3);
+                convert_tile<kGradB, 32 * C::kConvWarps>(smem + stage * C::kStageBytes,
+                                                         smem + C::kSmallOffset + small * C::kStageBytes, t0,
+                                                         1024 + col_boxes * 256, g.sum - kb * kBK, p.split3);
                 fence_proxy_async_shared();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(conv_bar(small));
@@ -553,7 +542,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                 const int t = grouped_turn(round, team, teams, total_tiles);
                 if (t == -2) break;
                 if (t < 0) continue;
-            const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+            const GroupedTile g = grouped_tile<kGradB, BT>(tab, t, p);
             int kb0;
                 const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
             float total[C::kTotals];
@@ -602,9 +591,8 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                     float v[W];
 #pragma unroll
                     for (int i = 0; i < W; ++i) v[i] = total[c + i];
-                    const long long row = g.col0 + first_col + c + (MODE == kGradB ? 0 : g.row0);
-                    if (MODE != kGradB) apply_column<W>(v, row, n, col, g.group, p.epi);
-                    float* dst = p.out + row * p.ldo + col + (MODE == kGradB ? g.group * p.out_stride : 0);
+                    const long long row = g.col0 + first_col + c;
+                    float* dst = p.out + row * p.ldo + col + g.group * p.out_stride;
 #pragma unroll
                     for (int i = 0; i < W; ++i)
                         if (i < n) __stcs(dst + i * p.ldo, v[i]);
@@ -617,7 +605,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
         __syncwarp();
         cluster_sync();  // the totals of every CTA of the tile are in place (or a CTA gave up)
         if (team < total_tiles && *abort_flag == 0) {
-            const GroupedTile g = grouped_tile<MODE, BT>(tab, team, p);
+            const GroupedTile g = grouped_tile<kGradB, BT>(tab, team, p);
             // Every thread an output, this CTA the tile columns rank, rank + splits, ...
             const int share = (g.cols - rank + splits - 1) / splits;
             for (int i = threadIdx.x; i < share * 128; i += C::kThreads) {
@@ -626,9 +614,7 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
                 const uint32_t at = smem_addr(smem) + static_cast<uint32_t>(c * 128 + (i & 127)) * 4;
                 float v = 0.0f;
                 for (int r = 0; r < splits; ++r) v += ld_shared_cluster_f32(mapa_shared(at, static_cast<uint32_t>(r)));
-                const long long row = g.col0 + c + (MODE == kGradB ? 0 : g.row0);
-                if (MODE != kGradB) v = apply_cell(v, row, col, g.group, p.epi);
-                p.out[row * p.ldo + col + (MODE == kGradB ? g.group * p.out_stride : 0)] = v;
+                p.out[(g.col0 + c) * p.ldo + col + g.group * p.out_stride] = v;
             }
         }
         __syncwarp();
@@ -653,28 +639,34 @@ __global__ void __launch_bounds__(GroupedCfg<BT>::kThreads, 1)
 // tensor memory, from where the second MMA takes them as its A operand (and
 // adds to the columns of the other small term: the main columns then see
 // a third of the sums that the tensor core cuts).  That is 72 KB a k-block (of
-// 32) where the kernel above moves 120.  Small parts as bf16 pairs, half the
-// tensor memory and MMAs, were no faster (92 us either way at 128 rows, 64 groups of
-// 1024 x 2048) and less exact.
+// 32) where small parts in shared memory would move 120.  Small parts as bf16
+// pairs, half the tensor memory and MMAs, were no faster (92 us either way at
+// 128 rows, 64 groups of 1024 x 2048) and less exact.  Tiles of 32 rows, with
+// two stages more, were within 2% at 16 and 32 rows a group and behind from
+// there (8 groups, 2048 x 4096: 24 rows 93 us against 70, 48 rows 108 against 100).
+//
+// Cold L2: 128 rows over 64 groups of 1024 x 2048 86 us (5.3 TB/s of the
+// weights that a group with a row has), 16 rows of one group x 16384 x 18944
+// 221 us (5.6 TB/s).
 //
 // With fewer tiles than SMs, a cluster of `splits` CTAs shares a tile, each
 // summing its own stretch of the sum; the totals meet in distributed shared
 // memory, added in CTA order.
 
 struct GroupedFewCfg {
-    static constexpr int kCols = 32;                  // rows of the group per tile
+    static constexpr int kCols = 64;  // rows of the group that a tile takes
     static constexpr int kLaneBytes = 128 * kBK * 4;
     static constexpr int kColBytes = 2 * kCols * kBK * 4;  // activations, then their small parts
     static constexpr int kStageBytes = kLaneBytes + kColBytes;
-    static constexpr int kStages = 8;
+    static constexpr int kStages = 6;
     static constexpr int kSmall = 4;                  // small weights in tensor memory: 32 columns each
     static constexpr int kEpiWarps = 4, kConvGroups = 3, kConvWarps = 4 * kConvGroups;
     static constexpr int kThreads = 32 * (kEpiWarps + kConvWarps + 4);  // and a warpgroup with TMA and MMA
     // Registers a thread: the launch has 640 x 96, given out in shares of 128 threads.
     static constexpr int kEpiRegs = 144, kConvRegs = 88, kIssueRegs = 72;
     static_assert(kEpiRegs + kConvGroups * kConvRegs + kIssueRegs <= 480, "more registers than the launch has");
-    static constexpr int kSmallCol = 4 * kCols;       // first TMEM column behind the two accumulators of 64
-    static constexpr int kTmemCols = 256;
+    static constexpr int kSmallCol = 4 * kCols;       // first TMEM column behind the two accumulators of 2 kCols
+    static constexpr int kTmemCols = 512;
     static constexpr int kSegKb = 4;                  // k-blocks to an accumulator: 16 sums into a main column
     static constexpr int kTableOffset = kStages * kStageBytes;
     static constexpr int kBarOffset = kTableOffset + kGroupedTableBytes;
@@ -689,8 +681,8 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
     grouped_few_kernel(const __grid_constant__ CUtensorMap tm_lane, const __grid_constant__ CUtensorMap tm_col,
                        const __grid_constant__ GroupedParams p, const int splits) {
     using C = GroupedFewCfg;
-    static_assert(MODE != kGradB, "the rows are the columns here");
     constexpr int BT = C::kCols;
+    static_assert(MODE != kGradB, "the rows are the columns here");
     constexpr bool kLaneMn = MODE == kForward;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
@@ -760,6 +752,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
                 if (t == -2) break;
                 if (t < 0) continue;
                 const GroupedTile g = grouped_tile<MODE, BT>(tab, t, p);
+                const int col_boxes = (g.cols + 31) / 32;
                 for (int kb = kb0; kb < kb1; ++kb) {
                     if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
                         ok = false;
@@ -767,7 +760,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
                     }
                     if (leader) {
                         const uint32_t st = smem_addr(smem + stage * C::kStageBytes), fb = full_bar(stage);
-                        mbar_arrive_expect_tx(fb, C::kLaneBytes + kBoxBytes);
+                        mbar_arrive_expect_tx(fb, C::kLaneBytes + col_boxes * kBoxBytes);
                         const int q0 = kb * kBK;
                         if (MODE == kForward) {
     #pragma unroll
@@ -776,7 +769,8 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
                         } else {
                             tma_load_3d(st, &tm_lane, fb, q0, g.lane0, g.group);
                         }
-                        tma_load_2d(st + C::kLaneBytes, &tm_col, fb, q0, g.row0 + g.col0);
+                        for (int j = 0; j < col_boxes; ++j)
+                            tma_load_2d(st + C::kLaneBytes + j * kBoxBytes, &tm_col, fb, q0, g.row0 + g.col0 + 32 * j);
                     }
                     __syncwarp();
                     ++issued;
@@ -921,7 +915,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
             }
         }
     } else {
-        // ------------------------------------------------------------ epilogue: a result column and 32 rows a thread
+        // ------------------------------------------------------------ epilogue: a result column and all rows a thread
         more_registers<C::kEpiRegs>();
         constexpr int W = 16;
         const int quad = warp & 3;
@@ -1033,6 +1027,13 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
 // The epilogue's 128 totals a thread need more registers than an even
 // split gives: the other warps hand some over (setmaxnreg; the shares add up
 // to the launch's 640 x 96).
+//
+// 8192 rows, 8 groups of 4096 x 4096: 1105 us in a burst, 249 TFLOP/s of fp32
+// products (three TF32 products each), and 1270 us once the power limit has the
+// clock at 1.57 GHz; 4096 rows of 4 groups keep the tensor cores 76% active.
+// 8191 rows, 8 groups, 1024 x 4096: grad_b with dbias 290 us.  4001 rows of 16
+// groups, 1024 x 4096: grad_a 240 us; of the 74 pairs 64 have a whole tile and
+// some a tile of the few rows behind one as well (balance, not rate).
 
 struct GroupedPairCfg {
     static constexpr int kCols = 256;
@@ -1468,10 +1469,9 @@ cudaError_t launch_clusters(Kernel kernel, int threads, int smem, long long tile
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <int MODE, int BT>
-cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
-    using C = GroupedCfg<BT>;
-    auto kernel = grouped_gemm_kernel<MODE, BT>;
+cudaError_t run_grouped_grad_b(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
+    using C = GroupedGradBCfg;
+    auto kernel = grouped_grad_b_kernel;
     static std::mutex mu;
     static uint64_t configured = 0;
     int dev = 0;
@@ -1486,11 +1486,11 @@ cudaError_t run_grouped(const GroupedCall& g, GroupedParams& p, bool split3, int
         }
     }
     CUtensorMap lane, col;
-    if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
+    if (!grouped_maps<kGradB>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
     p.lane_tiles = (p.lane_dim + 127) / 128;
-    const long long tiles = most_col_tiles<MODE>(g, BT) * p.lane_tiles;
-    // The k-blocks a tile has at most; in grad_b of an even split, which is only a guess.
-    const int all_kb = ((MODE == kGradB ? g.rows / g.groups : p.sum_dim) + kBK - 1) / kBK;
+    const long long tiles = most_col_tiles<kGradB>(g, C::kCols) * p.lane_tiles;
+    // The k-blocks of a tile if the rows are spread evenly, which is only a guess.
+    const int all_kb = (g.rows / g.groups + kBK - 1) / kBK;
     return launch_clusters(kernel, C::kThreads, C::kSmemBytes, tiles, all_kb, num_sms, stream, lane, col, p);
 }
 
@@ -1572,20 +1572,22 @@ cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3
 
 template <int MODE>
 cudaError_t run_grouped_mode(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
-    // By the columns that a group's tiles have on average (8 groups, 2048 x 4096, cold L2, few / single / pair in us):
-    // 16 rows 74 / - / 109, 48 rows - / 103 / 118, 64 rows - / 113 / 125, 96 rows - / 160 / 129, 256 rows - / 280 / 203.
-    // A pair's tile is four times a single CTA's, so it also has to have enough of them for all pairs.
+    // By the rows that a group has on average.  8 groups, 2048 x 4096, cold L2, a CTA with 64 rows to a tile / a pair
+    // with 256, in us: 80 rows 131 / -, 88 rows 131 / 127, 96 rows 133 / 129, 128 rows 166 / 135, 192 rows 228 / 191.
+    // A pair's tile is eight times the other's, so there also have to be enough of them for the pairs: 459 rows of 12
+    // groups, 811 x 1022, 32 us against the pairs' 42.  grad_b has its columns from K instead, and a CTA takes 128.
     const int cols = MODE == kGradB ? g.K : (g.rows + g.groups - 1) / g.groups;
     const long long pair_tiles = most_col_tiles<MODE>(g, GroupedPairCfg::kCols) * ((p.lane_dim + 255) / 256);
-    if (cols > 80 && p.lane_dim > 128 && pair_tiles >= num_sms * 3 / 8) {
+    if (cols > 84 && p.lane_dim > 128 && pair_tiles >= num_sms * 3 / 8) {
         // (TF32 mode: the staged dY is rounded; the bias gradient is summed from memory.)
         p.dbias = split3 ? g.dbias : nullptr;
         return run_grouped_pair<MODE>(g, p, split3, num_sms, stream);
     }
-    if constexpr (MODE != kGradB) {
-        if (cols <= 32) return run_grouped_few<MODE>(g, p, split3, num_sms, stream);
+    if constexpr (MODE == kGradB) {
+        return run_grouped_grad_b(g, p, split3, num_sms, stream);
+    } else {
+        return run_grouped_few<MODE>(g, p, split3, num_sms, stream);
     }
-    return run_grouped<MODE, 128>(g, p, split3, num_sms, stream);
 }
 
 int grouped_gemm(const char* fn, GpuCtx* ctx, const GroupedCall& g, const mxb_ep_step* steps, int n_steps,
