@@ -27,10 +27,10 @@ __device__ __forceinline__ float apply_cell(float v, long long row, int col, int
             case MXB_EP_RELU: v = v > 0.0f ? v : 0.0f; break;
             case MXB_EP_SCALE: v = v * st.scale; break;
             case MXB_EP_ADD_FULL: v += __ldcs(st.ptr + row * st.ld_or_size + col); break;
-            case MXB_EP_ADD_ROW: v += __ldg(st.ptr + group * st.ld_or_size + col); break;
+            case MXB_EP_ADD_ROW: v += ld_global(st.ptr + group * st.ld_or_size + col); break;
             case MXB_EP_ADD_MOD:
-                v += __ldg(st.ptr + (static_cast<unsigned long long>(row) * e.n_cols + col) %
-                                        static_cast<unsigned long long>(st.ld_or_size));
+                v += ld_global(st.ptr + (static_cast<unsigned long long>(row) * e.n_cols + col) %
+                                             static_cast<unsigned long long>(st.ld_or_size));
                 break;
             case MXB_EP_RELU_GRAD: v = __ldcs(st.ptr + row * st.ld_or_size + col) > 0.0f ? v : 0.0f; break;
             default: break;
@@ -52,14 +52,14 @@ __device__ __forceinline__ void apply_column(float (&v)[W], long long row, int n
 #pragma unroll
             for (int i = 0; i < W; ++i) v[i] = v[i] * st.scale;
         } else if (st.kind == MXB_EP_ADD_ROW) {
-            const float b = __ldg(st.ptr + group * st.ld_or_size + col);
+            const float b = ld_global(st.ptr + group * st.ld_or_size + col);
 #pragma unroll
             for (int i = 0; i < W; ++i) v[i] += b;
         } else if (st.kind == MXB_EP_ADD_MOD) {
             const unsigned long long size = static_cast<unsigned long long>(st.ld_or_size);
 #pragma unroll
             for (int i = 0; i < W; ++i)
-                if (i < n) v[i] += __ldg(st.ptr + (static_cast<unsigned long long>(row + i) * e.n_cols + col) % size);
+                if (i < n) v[i] += ld_global(st.ptr + (static_cast<unsigned long long>(row + i) * e.n_cols + col) % size);
         } else {  // ADD_FULL, RELU_GRAD (plain loads: the operand may be the output itself)
             const float* src = st.ptr + row * st.ld_or_size + col;
             float c[W];

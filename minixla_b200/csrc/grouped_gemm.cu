@@ -234,8 +234,8 @@ __device__ __forceinline__ void grouped_scan(GroupedTable& tab, const GroupedPar
         tiles = 0;
         const int e = i >> 1;
         if (e >= p.groups) return -1;
-        const int r0 = min(max(__ldg(p.offsets + e), 0), p.rows);
-        const int r1 = min(max(__ldg(p.offsets + e + 1), r0), p.rows);
+        const int r0 = min(max(ld_global(p.offsets + e), 0), p.rows);
+        const int r1 = min(max(ld_global(p.offsets + e + 1), r0), p.rows);
         if ((i & 1) == 0) {
             tab.row0[e] = r0;
             tab.row1[e] = r1;
@@ -363,9 +363,10 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
     if (warp == kMmaWarp) {
         tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
         tmem_relinquish();
-    } else if (warp == kConvWarp) {
-        grouped_scan<kGradB, BT>(tab, p, lane);
     }
+    wait_for_previous_kernel();
+    let_next_kernel_in();
+    if (warp == kConvWarp) grouped_scan<kGradB, BT>(tab, p, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -724,9 +725,10 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
     if (warp == kMmaWarp) {
         tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
         tmem_relinquish();
-    } else if (warp == kConvWarp) {
-        grouped_scan<MODE, BT>(tab, p, lane);
     }
+    wait_for_previous_kernel();
+    let_next_kernel_in();
+    if (warp == kConvWarp) grouped_scan<MODE, BT>(tab, p, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -1109,9 +1111,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
     if (warp == kMmaWarp) {
         tmem_alloc_pair(smem_addr(tmem_slot), C::kTmemCols);
         tmem_relinquish_pair();
-    } else if (warp == kConvWarp) {
-        grouped_scan<MODE, BT>(tab, p, lane);
     }
+    wait_for_previous_kernel();
+    let_next_kernel_in();
+    if (warp == kConvWarp) grouped_scan<MODE, BT>(tab, p, lane);
     __syncwarp();
     tc_fence_before();
     cluster_sync();  // barriers initialised, TMEM allocated and the tables written in both CTAs
@@ -1452,21 +1455,8 @@ cudaError_t launch_clusters(Kernel kernel, int threads, int smem, long long tile
                             cudaStream_t stream, const CUtensorMap& lane, const CUtensorMap& col, const GroupedParams& p) {
     int splits = 1;
     while (splits < kMaxSplits && 2 * splits * tiles <= num_sms && all_kb >= 4 * splits) splits *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = splits;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(splits > 1 ? tiles * splits : std::min<long long>(tiles, num_sms)), 1, 1);
-    cfg.blockDim = dim3(threads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, lane, col, p, splits);
-    note_launch();
-    return e != cudaSuccess ? e : cudaGetLastError();
+    const dim3 grid(static_cast<unsigned>(splits > 1 ? tiles * splits : std::min<long long>(tiles, num_sms)));
+    return launch_early(kernel, grid, dim3(threads), smem, stream, splits, lane, col, p, splits);
 }
 
 cudaError_t run_grouped_grad_b(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
@@ -1565,9 +1555,7 @@ cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3
     p.lane_tiles = (p.lane_dim + 255) / 256;
     const int pairs =
         static_cast<int>(std::min<long long>(most_col_tiles<MODE>(g, C::kCols) * p.lane_tiles, clusters));
-    kernel<<<2 * pairs, C::kThreads, C::kSmemBytes, stream>>>(lane, col, p);
-    note_launch();
-    return cudaGetLastError();
+    return launch_early(kernel, dim3(2 * pairs), dim3(C::kThreads), C::kSmemBytes, stream, 1, lane, col, p);
 }
 
 template <int MODE>

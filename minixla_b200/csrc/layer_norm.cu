@@ -14,7 +14,10 @@
 // hold are read again (from L2).  A block's rows arrive through a ring in shared
 // memory that bulk copies keep full: with loads by the threads themselves,
 // which can only be issued between a row's two barriers, the same kernels
-// reached 5.3 (forward) and 5.4 TB/s (backward).  The
+// reached 5.3 (forward) and 5.4 TB/s (backward); with the ring forward takes
+// 86 us at 16384 x 4096 (6.2 TB/s) and backward 130 us at 8192 x 8192 (6.2
+// TB/s), against 6.5 TB/s for a copy.  Short ones are latency: 27 us for the
+// backward pass of 5003 x 1027, of which its bytes need 9.  The
 // gradients of gamma and beta are summed per thread over the rows its block
 // walks through, then stored as one partial row per block and summed by a
 // second small kernel in block order, so the result does not depend on timing.
@@ -80,21 +83,24 @@ __device__ __forceinline__ void load_unit(float (&v)[W], const float* p, int c, 
     }
 }
 
-// The same for a vector that every row reads (gamma, beta): cached; `absent` where there is none.
-template <int W>
+// The same for a vector that every row reads (gamma, beta): cached; `absent` where there is none.  EARLY: in a kernel
+// that launch_early starts; elsewhere a read-only load, which the compiler may repeat for every row instead of keeping
+// its result in a register that the kernel needs more (the backward kernel at 5003 x 1027 27 us, else 34).
+template <int W, bool EARLY>
 __device__ __forceinline__ void load_param(float (&v)[W], const float* p, int c, int cols, float absent) {
     if (!p) {
 #pragma unroll
         for (int i = 0; i < W; ++i) v[i] = absent;
     } else if (W == 4 && c + W <= cols) {
-        const float4 t = __ldg(reinterpret_cast<const float4*>(p + c));
+        const float4* at = reinterpret_cast<const float4*>(p + c);
+        const float4 t = EARLY ? ld_global(at) : __ldg(at);
         v[0] = t.x;
         v[W > 1 ? 1 : 0] = t.y;
         v[W > 2 ? 2 : 0] = t.z;
         v[W > 3 ? 3 : 0] = t.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = c + i < cols ? __ldg(p + c + i) : 0.0f;
+        for (int i = 0; i < W; ++i) v[i] = c + i < cols ? (EARLY ? ld_global(p + c + i) : __ldg(p + c + i)) : 0.0f;
     }
 }
 
@@ -290,8 +296,8 @@ struct NormAffine {
         }
     }
     __device__ __forceinline__ void read(int into, int u, const NormParams& p, int t, int threads) {
-        load_param<W>(g[into], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
-        load_param<W>(b[into], p.beta, (u * threads + t) * W, p.cols, 0.0f);
+        load_param<W, true>(g[into], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
+        load_param<W, true>(b[into], p.beta, (u * threads + t) * W, p.cols, 0.0f);
     }
 };
 
@@ -319,6 +325,8 @@ __global__ void __launch_bounds__(kWarpRowThreads) layer_norm_warp_kernel(const 
     const int t = threadIdx.x & 31;
     const long long rows_at_once = static_cast<long long>(gridDim.x) * (kWarpRowThreads / 32);
     const float inv = 1.0f / static_cast<float>(p.cols);
+    wait_for_previous_kernel();
+    let_next_kernel_in();
     NormAffine<W, NV, W * NV <= 16> affine(p, t, 32);
     for (long long row = blockIdx.x * static_cast<long long>(kWarpRowThreads / 32) + (threadIdx.x >> 5); row < p.rows;
          row += rows_at_once) {
@@ -347,6 +355,10 @@ __global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_block_kern
         for (int s = 0; s < slots; ++s) mbar_init(ring.bar0 + 8 * s, 1);
         failed = INT_MAX;
         fence_barrier_init();
+    }
+    wait_for_previous_kernel();
+    let_next_kernel_in();
+    if (t == 0) {
         for (int s = 0; s < slots; ++s) {
             const long long row = blockIdx.x + static_cast<long long>(s) * gridDim.x;
             if (row < p.rows) ring.ask(row, s);
@@ -387,6 +399,8 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const NormParams 
     RowSum<false> row_sum{buf};
     const int step = blockDim.x * W;
     const float inv = 1.0f / static_cast<float>(p.cols);
+    wait_for_previous_kernel();
+    let_next_kernel_in();
     for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const float* x = p.x + row * p.ldx;
         float* y = p.y + row * p.ldy;
@@ -415,8 +429,8 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(const NormParams 
         for (long long c = threadIdx.x * W; c < p.cols; c += step) {
             float g[W], b[W];
             load_unit<W>(v, x, static_cast<int>(c), p.cols);
-            load_param<W>(g, p.gamma, static_cast<int>(c), p.cols, 1.0f);
-            load_param<W>(b, p.beta, static_cast<int>(c), p.cols, 0.0f);
+            load_param<W, true>(g, p.gamma, static_cast<int>(c), p.cols, 1.0f);
+            load_param<W, true>(b, p.beta, static_cast<int>(c), p.cols, 0.0f);
 #pragma unroll
             for (int i = 0; i < W; ++i) v[i] = (v[i] - mean) * rstd * g[i] + b[i];
             store_unit<W>(v, y, static_cast<int>(c), p.cols);
@@ -472,7 +486,7 @@ __global__ void __launch_bounds__(kWarpRowThreads) layer_norm_grad_warp_kernel(c
     const float inv = 1.0f / static_cast<float>(p.cols);
     float dg[NV][W] = {}, db[NV][W] = {}, gamma[NV][W];
 #pragma unroll
-    for (int u = 0; u < NV; ++u) load_param<W>(gamma[u], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
+    for (int u = 0; u < NV; ++u) load_param<W, false>(gamma[u], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
     long long row = blockIdx.x * static_cast<long long>(kWarpRowThreads / 32) + (threadIdx.x >> 5);
     NormStats next = saved_stats(p, row);  // a row ahead, so that no row waits for its two numbers
     for (; row < p.rows; row += rows_at_once) {
@@ -530,7 +544,7 @@ __global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_grad_block
     __syncthreads();
     float dg[NV][W] = {}, db[NV][W] = {}, gamma[NV][W];
 #pragma unroll
-    for (int u = 0; u < NV; ++u) load_param<W>(gamma[u], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
+    for (int u = 0; u < NV; ++u) load_param<W, false>(gamma[u], p.gamma, (u * threads + t) * W, p.cols, 1.0f);
     int slot = 0, round = 0;
     uint32_t phase = 0;
     NormStats next = saved_stats(p, blockIdx.x);  // a row ahead, so that no row waits for its two numbers
@@ -596,7 +610,7 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_wide_kernel(const NormGr
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
             float g[W];
-            load_param<W>(g, p.gamma, (u * 1024 + t) * W, p.cols, 1.0f);
+            load_param<W, false>(g, p.gamma, (u * 1024 + t) * W, p.cols, 1.0f);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 const int c = (u * 1024 + t) * W + i;
@@ -647,7 +661,7 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(const NormGr
             const int c = static_cast<int>(cc);
             load_unit<W>(xh, x, c, p.cols);
             load_unit<W>(d, dy, c, p.cols);
-            load_param<W>(g, p.gamma, c, p.cols, 1.0f);
+            load_param<W, false>(g, p.gamma, c, p.cols, 1.0f);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 xh[i] = (xh[i] - mean) * rstd;
@@ -668,7 +682,7 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(const NormGr
             const int c = static_cast<int>(cc);
             load_unit<W>(xh, x, c, p.cols);
             load_unit<W>(d, dy, c, p.cols);
-            load_param<W>(g, p.gamma, c, p.cols, 1.0f);
+            load_param<W, false>(g, p.gamma, c, p.cols, 1.0f);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
                 xh[i] = (xh[i] - mean) * rstd;
@@ -687,7 +701,7 @@ __global__ void __launch_bounds__(32 * ROWS) sum_partials_kernel(const float* pa
     __shared__ float part[ROWS][33];
     float* out = blockIdx.y ? dbeta : dgamma;
     const int c = blockIdx.x * 32 + threadIdx.x;
-    cudaGridDependencySynchronize();
+    wait_for_previous_kernel();
     if (!out) return;
     float s = 0.0f;
     if (c < cols) {
@@ -791,7 +805,7 @@ cudaError_t launch_norm(const NormParams& p, const RowPlan& plan, int num_sms, c
         const long long want = (p.rows + kWarpRowThreads / 32 - 1) / (kWarpRowThreads / 32);
         const int blocks = static_cast<int>(
             std::min<long long>(want, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_warp_kernel<W, NV>>(kWarpRowThreads, 0)));
-        layer_norm_warp_kernel<W, NV><<<blocks, kWarpRowThreads, 0, stream>>>(p);
+        return launch_early(layer_norm_warp_kernel<W, NV>, dim3(blocks), dim3(kWarpRowThreads), 0, stream, 1, p);
     } else {
         static uint64_t allowed = 0;
         const cudaError_t e = allow_ring(layer_norm_block_kernel<W, NV>, &allowed);
@@ -800,10 +814,8 @@ cudaError_t launch_norm(const NormParams& p, const RowPlan& plan, int num_sms, c
         const size_t smem = static_cast<size_t>(slots) * row_slot_bytes(p.cols);
         const int blocks = static_cast<int>(
             std::min<long long>(p.rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_block_kernel<W, NV>>(plan.threads, smem)));
-        layer_norm_block_kernel<W, NV><<<blocks, plan.threads, smem, stream>>>(p, slots);
+        return launch_early(layer_norm_block_kernel<W, NV>, dim3(blocks), dim3(plan.threads), smem, stream, 1, p, slots);
     }
-    note_launch();
-    return cudaGetLastError();
 }
 
 template <int W>
@@ -820,9 +832,7 @@ cudaError_t launch_norm_width(const NormParams& p, int num_sms, cudaStream_t str
     }
     const int blocks = static_cast<int>(
         std::min<long long>(p.rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_long_kernel<W>>(plan.threads, 0)));
-    layer_norm_long_kernel<W><<<blocks, plan.threads, 0, stream>>>(p);
-    note_launch();
-    return cudaGetLastError();
+    return launch_early(layer_norm_long_kernel<W>, dim3(blocks), dim3(plan.threads), 0, stream, 1, p);
 }
 
 // One launch of the backward kernel, or (p == nullptr) the number of blocks it takes.
@@ -956,20 +966,10 @@ int layer_norm_backward(GpuCtx* ctx, NormGradParams p, float* dgamma, float* dbe
     }
     if (!cuda_ok(run(&p, &blocks), "layer norm backward launch")) return MXB_E_CUDA;
     if (!p.partial) return MXB_OK;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((p.cols + 31) / 32, 2);
     // Many columns fill the SMs with small blocks; few columns need more threads for each.
     const bool tall = p.cols <= 32 * ctx->num_sms;
-    cfg.blockDim = dim3(32, tall ? 32 : 8);
-    cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, tall ? sum_partials_kernel<32> : sum_partials_kernel<8>,
-                                             static_cast<const float*>(p.partial), blocks, p.cols, dgamma, dbeta);
-    note_launch();
+    const cudaError_t e = launch_early(tall ? sum_partials_kernel<32> : sum_partials_kernel<8>, dim3((p.cols + 31) / 32, 2),
+                                       dim3(32, tall ? 32 : 8), 0, st, 1, p.partial, blocks, p.cols, dgamma, dbeta);
     return cuda_ok(e, "layer norm gradient sums launch") ? MXB_OK : MXB_E_CUDA;
 }
 

@@ -55,6 +55,12 @@ struct Q4Params {
 // Each warp has a ring of its own: one lane asks TMA for the next run's
 // weights and activations (zeros past their edges), so that no instruction
 // is spent on addresses and bounds.
+//
+// Calls one behind the other, weights past L2: 1 x 4096 x 4096 5.6 us, 1 x 8192 x
+// 8192 14 us (2.5 TB/s), 8 x 8192 x 8192 with groups of 32, fp32 scales and zero
+// points 27.5 us (1.6 TB/s).  What bounds it there are the
+// instructions that make bf16 pairs of nibbles and scale each group's sums:
+// 55% of the issue slots and 48% of the ALU's.
 
 constexpr int kFewWarps = 8;
 
@@ -132,6 +138,8 @@ __global__ void __launch_bounds__(32 * kFewWarps)
     }
     if (threadIdx.x == 0) *abort_flag = 0;
     __syncthreads();
+    wait_for_previous_kernel();
+    let_next_kernel_in();
 
     // Unit of run r into slot `slot`.  Weights: row i's 16-byte chunk c (piece c, 32 k) at c ^ (i & 7), or at
     // c ^ ((i >> 1) & 3) in a row of 64 bytes; activations: a box for each piece, row m's 128 bytes at 128 m,
@@ -159,9 +167,9 @@ __global__ void __launch_bounds__(32 * kFewWarps)
             z_raw[i] = 8;
             if (row < 16 * MT && n < p.N && k < p.K) {
                 const long long at = n * p.lds + piece;
-                s_raw[i] = p.scale_type == MXB_SCALE_F32 ? __ldg(static_cast<const uint32_t*>(p.scales) + at)
-                                                         : __ldg(static_cast<const unsigned short*>(p.scales) + at);
-                if (p.zeros) z_raw[i] = __ldg(p.zeros + at);
+                s_raw[i] = p.scale_type == MXB_SCALE_F32 ? ld_global(static_cast<const uint32_t*>(p.scales) + at)
+                                                         : ld_global(static_cast<const unsigned short*>(p.scales) + at);
+                if (p.zeros) z_raw[i] = ld_global(p.zeros + at);
             }
         }
     };
@@ -345,10 +353,8 @@ cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
                            PACK ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
         return cudaErrorInvalidValue;
-    kernel<<<dim3((p.N + 16 * MT - 1) / (16 * MT), (p.M + C::kRows - 1) / C::kRows), 32 * kFewWarps, C::kSmem, stream>>>(
-        mw, ma, p);
-    note_launch();
-    return cudaGetLastError();
+    return launch_early(kernel, dim3((p.N + 16 * MT - 1) / (16 * MT), (p.M + C::kRows - 1) / C::kRows),
+                        dim3(32 * kFewWarps), C::kSmem, stream, 1, mw, ma, p);
 }
 
 template <int PACK, int RT, int MT>
@@ -385,6 +391,10 @@ cudaError_t run_few_rows_width(const Q4Params& p, int num_sms, cudaStream_t stre
 // With fewer tiles than SMs, a cluster of `splits` CTAs shares a tile, each
 // summing its own stretch of K; the totals meet in distributed shared memory,
 // added in CTA order.
+//
+// 1000 x 8192 x 8192, groups of 128: 326 us in a burst (412 TFLOP/s, 1236 of the
+// tensor core's bf16 ones), 377 us once the power limit has the clock at 1.57
+// GHz; the tensor cores are then 65% active.
 
 constexpr int kManyCols = 128;  // rows of A per tile, at most
 constexpr int kManyK = 64;      // k per stage: 128 bytes of bf16
@@ -436,21 +446,23 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t leader, uint32_t d_tmem, uin
 __global__ void __launch_bounds__(256) q4_cut_kernel(const float* a, long long lda, int M, int K, long long kp,
                                                      uint4* parts) {
     const long long eights = kp / 8, total = M * eights;
+    wait_for_previous_kernel();
+    let_next_kernel_in();
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
         const long long m = i / eights;
         const int k = static_cast<int>(i - m * eights) * 8;
         const float* src = a + m * lda + k;
         float u[4], v[4];
         if (k + 8 <= K) {
-            const float4 lo = __ldg(reinterpret_cast<const float4*>(src));
-            const float4 hi = __ldg(reinterpret_cast<const float4*>(src) + 1);
+            const float4 lo = ld_global(reinterpret_cast<const float4*>(src));
+            const float4 hi = ld_global(reinterpret_cast<const float4*>(src) + 1);
             u[0] = lo.x, u[1] = lo.y, u[2] = lo.z, u[3] = lo.w;
             v[0] = hi.x, v[1] = hi.y, v[2] = hi.z, v[3] = hi.w;
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                u[j] = k + j < K ? __ldg(src + j) : 0.0f;
-                v[j] = k + 4 + j < K ? __ldg(src + 4 + j) : 0.0f;
+                u[j] = k + j < K ? ld_global(src + j) : 0.0f;
+                v[j] = k + 4 + j < K ? ld_global(src + 4 + j) : 0.0f;
             }
         }
 #pragma unroll
@@ -474,8 +486,8 @@ __device__ __forceinline__ void raise_q4(const Q4Params& p, volatile int* abort_
 
 // A scale as it lies in memory, and as a number: apart, so that a load can be under way while others are used.
 __device__ __forceinline__ uint32_t scale_raw(const Q4Params& p, long long at) {
-    return p.scale_type == MXB_SCALE_F32 ? __ldg(static_cast<const uint32_t*>(p.scales) + at)
-                                         : __ldg(static_cast<const unsigned short*>(p.scales) + at);
+    return p.scale_type == MXB_SCALE_F32 ? ld_global(static_cast<const uint32_t*>(p.scales) + at)
+                                         : ld_global(static_cast<const unsigned short*>(p.scales) + at);
 }
 __device__ __forceinline__ float scale_value(const Q4Params& p, uint32_t raw) {
     return p.scale_type == MXB_SCALE_F32   ? __uint_as_float(raw)
@@ -546,6 +558,8 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    wait_for_previous_kernel();
+    let_next_kernel_in();
 
     const int all_stages = (p.K + kManyK - 1) / kManyK;
     const int halves = (p.K + 31) / 32;                                     // of 32 k
@@ -677,7 +691,7 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
             GroupWalk at{p.group, 0, 0};
             at.step(kb0 * kManyK + 32 * half);
             auto zero_of = [&](int kb) -> uint32_t {
-                return p.zeros && kb * kManyK + 32 * half < p.K ? __ldg(p.zeros + n * p.lds + at.index) : 8u;
+                return p.zeros && kb * kManyK + 32 * half < p.K ? ld_global(p.zeros + n * p.lds + at.index) : 8u;
             };
             uint32_t z_next = zero_of(kb0);
             for (int kb = kb0; kb < kb1; ++kb) {
@@ -843,10 +857,10 @@ int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
     void* parts = scratch.alloc(static_cast<size_t>(3) * p.M * kp * 2);
     if (!parts) return MXB_E_NOMEM;
     const long long blocks = (p.M * (kp / 8) + 255) / 256;
-    q4_cut_kernel<<<static_cast<int>(std::min<long long>(blocks, 8ll * ctx->num_sms)), 256, 0, stream>>>(
-        p.a, p.lda, p.M, p.K, kp, static_cast<uint4*>(parts));
-    note_launch();
-    if (!cuda_ok(cudaGetLastError(), "4-bit product: cutting the rows")) return MXB_E_CUDA;
+    if (!cuda_ok(launch_early(q4_cut_kernel, dim3(static_cast<unsigned>(std::min<long long>(blocks, 8ll * ctx->num_sms))),
+                              dim3(256), 0, stream, 1, p.a, p.lda, p.M, p.K, kp, static_cast<uint4*>(parts)),
+                 "4-bit product: cutting the rows"))
+        return MXB_E_CUDA;
 
     // The tile width (a multiple of 16) that needs the least time in whole rounds of the SMs: a round costs its width (96
     // columns at least: a narrower MMA takes no less) and about 32 columns more.  1000 rows x 8192: 9 tiles of 112 in 4
@@ -887,20 +901,9 @@ int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
         set_error("mxb_q4_gemm: the tensor maps could not be made");
         return MXB_E_CUDA;
     }
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = mp.splits;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(mp.splits > 1 ? tiles * mp.splits : std::min<long long>(tiles, ctx->num_sms)));
-    cfg.blockDim = dim3(C::kThreads);
-    cfg.dynamicSmemBytes = C::kSmem;
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, q4_many_rows_kernel, mw, mx, mp);
-    note_launch();
+    const dim3 grid(static_cast<unsigned>(mp.splits > 1 ? tiles * mp.splits : std::min<long long>(tiles, ctx->num_sms)));
+    const cudaError_t e =
+        launch_early(q4_many_rows_kernel, grid, dim3(C::kThreads), C::kSmem, stream, mp.splits, mw, mx, mp);
     return cuda_ok(e, "4-bit product launch") ? MXB_OK : MXB_E_CUDA;
 }
 
@@ -930,6 +933,8 @@ int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, voi
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     p.timeout_ns = ctx->timeout_ns;
     p.err = ctx->d_err;
+    // 8192 x 8192, groups of 128, cold L2: 16 rows 35.8 us in the few-row kernel, whose time grows with every eight rows
+    // (8: 29.6); 17 rows 50 us in the other, whose time is that of 32.
     if (p.M > 16) return run_many_rows(ctx, p, st);
     const cudaError_t e = p.M == 1   ? run_few_rows_width<1, 1>(p, ctx->num_sms, st)
                           : p.M == 2 ? run_few_rows_width<2, 1>(p, ctx->num_sms, st)

@@ -355,6 +355,47 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// For kernels launched by launch_early: nothing before this wait may touch global memory, since the previous kernel of
+// the stream may still run; behind it that kernel has finished and its results are visible.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// The stream's next kernel, if it was launched by launch_early, may take its place on the SMs as this one's blocks leave
+// (and wait there in turn); without it, once they all have.
+__device__ __forceinline__ void let_next_kernel_in() { asm volatile("griddepcontrol.launch_dependents;"); }
+
+// Loads for such kernels: they stay behind the wait, which the compiler need not respect with read-only loads (__ldg),
+// and are known to be of global memory, which it cannot tell of pointers inside a parameter structure.
+__device__ __forceinline__ float ld_global(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float4 ld_global(const float4* p) {
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int ld_global(const int* p) {
+    int v;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_global(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_global(const unsigned short* p) {
+    unsigned short v;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_global(const unsigned char* p) {
+    uint32_t v;
+    asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+
 // The same for writes that the arriving thread has already published to the
 // async proxy (fence_proxy_async_shared): what the barrier guards is read by
 // the pair's MMA from the shared memory of the CTA that wrote it, so no release

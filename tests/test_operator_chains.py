@@ -1,0 +1,99 @@
+"""Norm, 4-bit and grouped products one behind the other, each reading what the last one wrote.
+
+Their kernels are placed while the previous kernel of the stream still runs and wait for it before they touch memory, so
+a chain without a pause has to give the bits of one that is synchronised after every call.
+"""
+import pytest
+
+from minixla_b200 import lib as mlib
+from tests.operator_calls import captured, current_stream, ok, ptr, steps
+
+D = 512        # width of every product
+GROUP = 64
+EXPERTS = 4
+TURNS = 10
+
+
+class Chain:
+    def __init__(self, lib, ctx, rows):
+        import torch
+
+        g = torch.Generator(device="cuda").manual_seed(rows)
+
+        def randn(*shape):
+            return torch.randn(*shape, generator=g, device="cuda")
+
+        self.lib, self.ctx, self.rows = lib, ctx, rows
+        self.q = torch.randint(0, 256, (D, D // 2), generator=g, device="cuda", dtype=torch.uint8)
+        self.scales = randn(D, D // GROUP) * (0.2 / D ** 0.5)
+        self.b = randn(EXPERTS, D, D) / D ** 0.5
+        cuts = torch.randint(0, rows + 1, (EXPERTS - 1,), generator=g, device="cuda").sort().values
+        self.offsets = torch.cat([cuts.new_zeros(1), cuts, cuts.new_full((1,), rows)]).int()
+        self.start = randn(rows, D), randn(1, D)
+        self.x, self.gamma = (t.clone() for t in self.start)
+        self.y, self.z, self.w = (torch.empty(rows, D, device="cuda") for _ in range(3))
+        self.statistics = torch.empty(2, rows, device="cuda")
+
+    def reset(self):
+        self.x.copy_(self.start[0])
+        self.gamma.copy_(self.start[1])
+
+    def run(self, after=lambda: None):
+        lib, ctx, rows, st = self.lib, self.ctx, self.rows, current_stream()
+        add = steps((mlib.MXB_EP_ADD_FULL, self.x, D, 1.0))
+        none = steps()
+        for _ in range(TURNS):
+            # gamma is what the last turn's product for one row left.
+            ok(lib.mxb_layer_norm(ctx, ptr(self.x), D, ptr(self.gamma), None, 1e-5, ptr(self.y), D,
+                                  ptr(self.statistics[0]), ptr(self.statistics[1]), rows, D, st))
+            after()
+            ok(lib.mxb_q4_gemm(ctx, ptr(self.y), D, ptr(self.q), D // 2, ptr(self.scales), mlib.MXB_SCALE_F32, None,
+                               D // GROUP, GROUP, ptr(self.z), D, rows, D, D, *none, st))
+            after()
+            ok(lib.mxb_grouped_gemm(ctx, ptr(self.z), D, ptr(self.b), D, D * D, ptr(self.offsets), EXPERTS, ptr(self.w),
+                                    D, rows, D, D, *add, mlib.GPU_PRECISION_3XTF32, st))
+            after()
+            ok(lib.mxb_q4_gemm(ctx, ptr(self.w), D, ptr(self.q), D // 2, ptr(self.scales), mlib.MXB_SCALE_F32, None,
+                               D // GROUP, GROUP, ptr(self.gamma), D, 1, D, D, *none, st))
+            after()
+            # The backward kernels read the norm's rows and write the next turn's.
+            ok(lib.mxb_layer_norm_backward(ctx, ptr(self.w), D, ptr(self.x), D, ptr(self.gamma),
+                                           ptr(self.statistics[0]), ptr(self.statistics[1]), ptr(self.x), D, None, None,
+                                           rows, D, st))
+            after()
+        return self.x, self.gamma
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 8, 16, 40, 700, 5000])
+def test_chain_without_a_pause(lib, gpu_ctx, rows):
+    import torch
+
+    chain = Chain(lib, gpu_ctx, rows)
+    chain.reset()
+    want = [t.clone() for t in chain.run(torch.cuda.synchronize)]
+    assert all(torch.isfinite(t).all() for t in want)
+    for _ in range(3):
+        chain.reset()
+        torch.cuda.synchronize()
+        got = chain.run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2, 40, 700])
+def test_captured_chain(lib, gpu_ctx, rows):
+    import torch
+
+    chain = Chain(lib, gpu_ctx, rows)
+    chain.reset()
+    want = [t.clone() for t in chain.run(torch.cuda.synchronize)]
+
+    def turn():
+        chain.reset()
+        chain.run()
+
+    graph = captured(turn, replays=3)
+    assert all(torch.equal(g, w) for g, w in zip((chain.x, chain.gamma), want))
+    del graph
