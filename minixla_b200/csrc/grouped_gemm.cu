@@ -646,9 +646,9 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
 // two stages more, were within 2% at 16 and 32 rows a group and behind from
 // there (8 groups, 2048 x 4096: 24 rows 93 us against 70, 48 rows 108 against 100).
 //
-// Cold L2: 128 rows over 64 groups of 1024 x 2048 86 us (5.3 TB/s of the
-// weights that a group with a row has), 16 rows of one group x 16384 x 18944
-// 221 us (5.6 TB/s).
+// Cold L2: 128 rows over 64 groups of 1024 x 2048, of which 45 have a row, 84 us
+// (4.5 TB/s; five rounds of tiles and a start of 5 us), 16 rows of one group x
+// 16384 x 18944 221 us (5.6 TB/s).
 //
 // With fewer tiles than SMs, a cluster of `splits` CTAs shares a tile, each
 // summing its own stretch of the sum; the totals meet in distributed shared
