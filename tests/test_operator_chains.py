@@ -97,3 +97,84 @@ def test_captured_chain(lib, gpu_ctx, rows):
     graph = captured(turn, replays=3)
     assert all(torch.equal(g, w) for g, w in zip((chain.x, chain.gamma), want))
     del graph
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 16, 300])
+def test_calls_behind_another_stream(lib, gpu_ctx, rows):
+    """A call whose stream waits for an event of another stream reads what that stream wrote."""
+    import torch
+
+    chain = Chain(lib, gpu_ctx, rows)
+    other, here = torch.cuda.Stream(), torch.cuda.Stream()
+    none = steps()
+    x = torch.empty_like(chain.x)
+
+    def product(src, out):
+        ok(lib.mxb_q4_gemm(gpu_ctx, ptr(src), D, ptr(chain.q), D // 2, ptr(chain.scales), mlib.MXB_SCALE_F32, None,
+                           D // GROUP, GROUP, ptr(out), D, rows, D, D, *none, current_stream()))
+
+    def normed(src, out):
+        ok(lib.mxb_layer_norm(gpu_ctx, ptr(src), D, None, None, 1e-5, ptr(out), D, None, None, rows, D, current_stream()))
+
+    normed(chain.start[0], x)
+    product(x, chain.w)
+    torch.cuda.synchronize()
+    want = chain.w.clone()
+    for _ in range(5):
+        x.zero_()
+        chain.w.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(2_000_000)
+            normed(chain.start[0], x)
+            written = other.record_event()
+        with torch.cuda.stream(here):
+            product(chain.start[0], chain.z)  # the kernel before, on this stream, has nothing to do with x
+            here.wait_event(written)
+            product(x, chain.w)
+        torch.cuda.synchronize()
+        assert torch.equal(chain.w, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 16, 300])
+def test_captured_fork(lib, gpu_ctx, rows):
+    """The same inside a graph: a branch on another stream writes what the call behind the join reads."""
+    import torch
+
+    chain = Chain(lib, gpu_ctx, rows)
+    other = torch.cuda.Stream()
+    none = steps()
+    x = torch.empty_like(chain.x)
+
+    def product(src, out):
+        ok(lib.mxb_q4_gemm(gpu_ctx, ptr(src), D, ptr(chain.q), D // 2, ptr(chain.scales), mlib.MXB_SCALE_F32, None,
+                           D // GROUP, GROUP, ptr(out), D, rows, D, D, *none, current_stream()))
+
+    def normed():
+        ok(lib.mxb_layer_norm(gpu_ctx, ptr(chain.x), D, None, None, 1e-5, ptr(x), D, None, None, rows, D,
+                              current_stream()))
+
+    def fork():
+        here = torch.cuda.current_stream()
+        other.wait_stream(here)
+        with torch.cuda.stream(other):
+            for _ in range(20):
+                normed()
+        product(chain.start[0], chain.z)
+        here.wait_stream(other)
+        product(x, chain.w)
+
+    graph = captured(fork)
+    for turn in range(3):
+        chain.x.copy_(chain.start[0] * (turn + 1) + turn)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = chain.w.clone()
+        normed()
+        torch.cuda.synchronize()
+        product(x, chain.w)
+        torch.cuda.synchronize()
+        assert torch.equal(got, chain.w)
+    del graph
