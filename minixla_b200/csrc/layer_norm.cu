@@ -16,8 +16,8 @@
 // which can only be issued between a row's two barriers, the same kernels
 // reached 5.3 (forward) and 5.4 TB/s (backward); with the ring forward takes
 // 86 us at 16384 x 4096 (6.2 TB/s) and backward 130 us at 8192 x 8192 (6.2
-// TB/s), against 6.5 TB/s for a copy.  Short ones are latency: 27 us for the
-// backward pass of 5003 x 1027, of which its bytes need 9.  The
+// TB/s), against 6.5 TB/s for a copy.  Short or odd rows are latency and
+// instructions: 25 us for the backward pass of 5003 x 1027, of which its bytes need 9.  The
 // gradients of gamma and beta are summed per thread over the rows its block
 // walks through, then stored as one partial row per block and summed by a
 // second small kernel in block order, so the result does not depend on timing.
@@ -68,6 +68,33 @@ struct NormGradParams {
     int* err;
 };
 
+// Accesses under a predicate, for rows of single floats (W = 1): the compiler puts a branch around a conditional asm
+// statement, one for every access there (backward 20003 x 1027 74 -> 64 us without them, 2000 x 5001 42 -> 35).  Rows of
+// four have few such accesses, and keep the branch.
+__device__ __forceinline__ float load_if(bool wanted, const float* p) {
+    float v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.global.cs.f32 %0, [%1];\n\t}"
+        : "=f"(v)
+        : "l"(p), "r"(static_cast<int>(wanted))
+        : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_if(bool wanted, float* p, float v) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p st.global.cs.f32 [%0], %1;\n\t}" ::"l"(p), "f"(v),
+                 "r"(static_cast<int>(wanted))
+                 : "memory");
+}
+__device__ __forceinline__ float load_shared_if(bool wanted, uint32_t addr) {
+    float v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.shared.f32 %0, [%1];\n\t}"
+        : "=f"(v)
+        : "r"(addr), "r"(static_cast<int>(wanted))
+        : "memory");
+    return v;
+}
+
 // W consecutive floats at p + c, zeros from column `cols` on.
 template <int W>
 __device__ __forceinline__ void load_unit(float (&v)[W], const float* p, int c, int cols) {
@@ -79,13 +106,13 @@ __device__ __forceinline__ void load_unit(float (&v)[W], const float* p, int c, 
         v[W > 3 ? 3 : 0] = t.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = c + i < cols ? __ldcs(p + c + i) : 0.0f;
+        for (int i = 0; i < W; ++i) v[i] = W == 1 ? load_if(c < cols, p + c) : c + i < cols ? __ldcs(p + c + i) : 0.0f;
     }
 }
 
 // The same for a vector that every row reads (gamma, beta): cached; `absent` where there is none.  EARLY: in a kernel
 // that launch_early starts; elsewhere a read-only load, which the compiler may repeat for every row instead of keeping
-// its result in a register that the kernel needs more (the backward kernel at 5003 x 1027 27 us, else 34).
+// its result in a register that the kernel needs more (the backward pass of 5003 x 1027 is 7 us slower with the result pinned).
 template <int W, bool EARLY>
 __device__ __forceinline__ void load_param(float (&v)[W], const float* p, int c, int cols, float absent) {
     if (!p) {
@@ -111,7 +138,11 @@ __device__ __forceinline__ void store_unit(const float (&v)[W], float* p, int c,
     } else {
 #pragma unroll
         for (int i = 0; i < W; ++i)
-            if (c + i < cols) __stcs(p + c + i, v[i]);
+            if (W == 1) {
+                store_if(c < cols, p + c, v[0]);
+            } else if (c + i < cols) {
+                __stcs(p + c + i, v[i]);
+            }
     }
 }
 
@@ -186,11 +217,6 @@ __device__ __forceinline__ RowSpan row_span(const RowSource& m, long long row, l
 
 __host__ __device__ constexpr int row_slot_bytes(int cols) { return (cols * 4 + 12 + 15) / 16 * 16; }
 
-__device__ __forceinline__ float ld_shared_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ float4 ld_shared_v4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -242,7 +268,7 @@ struct RowRing {
                 } else {
 #pragma unroll
                     for (int i = 0; i < W; ++i)
-                        v[u][i] = c + i < cols ? ld_shared_f32(at + (u * threads * W + i) * 4) : 0.0f;
+                        v[u][i] = W == 1 || c + i < cols ? load_shared_if(c + i < cols, at + (u * threads * W + i) * 4) : 0.0f;
                 }
             }
         } else {
