@@ -409,9 +409,11 @@ MXB_API int mxb_q4_gemm(GpuCtx* ctx, const float* A, long long lda, const unsign
  *   out[r, :] = epi(A[r, :] @ B_e),   B_e = B + e * b_stride  (K x N, pitch ldb).
  * offsets: groups + 1 non-decreasing values in 0 .. rows, in device memory
  * (never read on the host).  A group may be empty; rows of A and out that lie
- * in no group are neither used nor written.  Values outside 0 .. rows, or
- * decreasing ones, are taken as the nearest allowed value, so that no access
- * leaves the buffers.  groups <= MXB_MAX_GROUPS; lda, ldb and b_stride are
+ * in no group are neither used nor written.  No value can make an access leave
+ * the buffers: group e begins at offsets[e] clamped to 0 .. rows and ends at
+ * offsets[e+1] clamped to its begin .. rows.  Each value of a row that
+ * decreasing offsets give to several groups is one of their results (what the
+ * steps add to out itself may then be added more than once).  groups <= MXB_MAX_GROUPS; lda, ldb and b_stride are
  * multiples of 4, A and B 16-byte aligned.  Steps: ADD_FULL, RELU, SCALE and
  * RELU_GRAD as named above (i: the row of out), and ADD_ROW with
  * operand[e * ld_or_size + j] (ld_or_size 0: one row for all groups).

@@ -287,21 +287,24 @@ __device__ __forceinline__ void grouped_scan(GroupedTable& tab, const GroupedPar
         }
         __syncwarp();
     }
-    int base = 0;
+    // Sums end at 2^31 - 1 (an entry's own tiles are below 2^25, since the result has to be in memory): only groups that
+    // decreasing offsets make overlap can have more tiles together, and those beyond are left out.
+    auto add = [](unsigned a, unsigned b) { return min(a + b, 0x7FFFFFFFu); };
+    unsigned base = 0;
     for (int i0 = 0; i0 < entries; i0 += 32) {
-        const int tiles = i0 + lane < entries ? tab.first_tile[i0 + lane] : 0;
-        int inclusive = tiles;
+        unsigned upto_here = i0 + lane < entries ? tab.first_tile[i0 + lane] : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, inclusive, o);
-            if (lane >= o) inclusive += v;
+            const unsigned v = __shfl_up_sync(0xffffffffu, upto_here, o);
+            if (lane >= o) upto_here = add(upto_here, v);
         }
-        if (i0 + lane < entries) tab.first_tile[i0 + lane] = base + inclusive - tiles;
-        base += __shfl_sync(0xffffffffu, inclusive, 31);
+        const unsigned before = __shfl_up_sync(0xffffffffu, upto_here, 1);
+        if (i0 + lane < entries) tab.first_tile[i0 + lane] = static_cast<int>(lane ? add(base, before) : base);
+        base = add(base, __shfl_sync(0xffffffffu, upto_here, 31));
     }
     if (lane == 0) {
         tab.entries = entries;
-        tab.total = base;
+        tab.total = static_cast<int>(base);
     }
 }
 
@@ -652,7 +655,10 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
 //
 // With fewer tiles than SMs, a cluster of `splits` CTAs shares a tile, each
 // summing its own stretch of the sum; the totals meet in distributed shared
-// memory, added in CTA order.
+// memory, added in CTA order.  A cluster has room for one tile's totals, and
+// the grid has a cluster for every tile that non-decreasing offsets can give.
+// Decreasing ones can give more (groups then overlap): every CTA sees that in
+// its table and takes whole tiles for itself, in rounds.
 
 struct GroupedFewCfg {
     static constexpr int kCols = 64;  // rows of the group that a tile takes
@@ -680,7 +686,7 @@ struct GroupedFewCfg {
 template <int MODE>
 __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
     grouped_few_kernel(const __grid_constant__ CUtensorMap tm_lane, const __grid_constant__ CUtensorMap tm_col,
-                       const __grid_constant__ GroupedParams p, const int splits) {
+                       const __grid_constant__ GroupedParams p, const int cluster) {
     using C = GroupedFewCfg;
     constexpr int BT = C::kCols;
     static_assert(MODE != kGradB, "the rows are the columns here");
@@ -734,6 +740,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = tab.total;
+    const int splits = total_tiles > static_cast<int>(gridDim.x) / cluster ? 1 : cluster;
     const int team = blockIdx.x / splits, teams = gridDim.x / splits, rank = blockIdx.x - team * splits;
     // This CTA's k-blocks [kb0, kb1) of every tile (all sums are as long as sum_dim).
     const int all_kb = (p.sum_dim + kBK - 1) / kBK;

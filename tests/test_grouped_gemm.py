@@ -222,6 +222,29 @@ def test_offsets_out_of_range_are_clamped(lib, gpu_ctx, offsets, meant):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,length,groups,overlaps", [(130, 64, 512, 5, 3), (640, 128, 1024, 3, 2)])
+def test_decreasing_offsets_where_clusters_share_sums(lib, gpu_ctx, rows, width, length, groups, overlaps):
+    """Offsets 0, rows, 0, rows, ... make every other group all of the rows: more tiles (64 rows, 128 columns) than
+    non-decreasing offsets can give, from which the grid of clusters was sized."""
+    import torch
+
+    tiles, most = overlaps * -(-rows // 64), rows // 64 + groups
+    assert tiles > most and 2 * 4 * most <= 148 and length // 32 >= 16, "a shape for clusters of eight with a tile too many"
+    offsets = torch.tensor([e % 2 * rows for e in range(groups + 1)], dtype=torch.int32, device="cuda")
+    for f, k, n in ((forward, length, width), (grad_a, width, length)):
+        c = make([rows] + [0] * (groups - 1), k, n, seed=rows, ints=True)
+        c["off"] = offsets
+        got = f(lib, gpu_ctx, c)
+        x = (c["a"] if f is forward else c["dy"]).double()
+        meant = torch.stack([x @ (b if f is forward else b.t()) for b in c["b"][::2].double()])
+        assert (got == meant).any(0).all()
+        # Increasing ones again, of the same extents: clusters.
+        c["off"] = torch.tensor([0] + [rows] * groups, dtype=torch.int32, device="cuda")
+        assert (f(lib, gpu_ctx, c) == meant[0]).all()
+    assert lib.mxb_check_device_error(gpu_ctx) == 0
+
+
+@pytest.mark.gpu
 def test_no_rows(lib, gpu_ctx):
     import torch
 
