@@ -34,7 +34,10 @@ inline std::atomic<long long>& alloc_calls() {
 //
 // Size-class free lists.  A released block carries an event recorded on the
 // stream that last used it; handing it to a different stream makes that
-// stream wait on the event, so reuse is always stream-ordered.  A failed
+// stream wait on the event, so reuse is always stream-ordered.  Streams are
+// told apart by cudaStreamGetId: the handle cudaStreamPerThread names another
+// stream in every host thread, and a destroyed stream's handle may come back
+// while its work still runs.  A failed
 // cudaMalloc first returns every cached block to the driver and retries.
 // MINIXLA_FAIL_ALLOC_AT=n makes the n-th pool allocation of the process fail
 // (host-side fault injection for the out-of-memory path).  A mutex guards the
@@ -66,7 +69,7 @@ class DevicePool {
             Cached c = it->second.back();
             it->second.pop_back();
             cached_bytes_ -= cls;
-            if (c.stream != stream) cudaStreamWaitEvent(stream, c.ready, 0);
+            if (c.stream_id == 0 || c.stream_id != stream_id(stream)) cudaStreamWaitEvent(stream, c.ready, 0);
             spare_events_.push_back(c.ready);
             live_[c.ptr] = cls;
             return c.ptr;
@@ -94,7 +97,7 @@ class DevicePool {
         live_.erase(it);
         cudaEvent_t ev = take_event();
         if (ev) cudaEventRecord(ev, stream);
-        free_[cls].push_back(Cached{p, stream, ev});
+        free_[cls].push_back(Cached{p, stream_id(stream), ev});
         cached_bytes_ += cls;
         if (!ev) {  // could not make an event: fall back to a full sync before reuse
             cudaStreamSynchronize(stream);
@@ -134,9 +137,19 @@ class DevicePool {
 
     struct Cached {
         void* ptr;
-        cudaStream_t stream;
+        unsigned long long stream_id;
         cudaEvent_t ready;
     };
+
+    // Never given to another stream of the process; 0: could not be asked (no stream is the same as that one).
+    static unsigned long long stream_id(cudaStream_t stream) {
+        unsigned long long id = 0;
+        if (cudaStreamGetId(stream, &id) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        return id;
+    }
 
     static size_t size_class(size_t bytes) {
         if (bytes == 0) bytes = 1;

@@ -178,3 +178,60 @@ def test_captured_fork(lib, gpu_ctx, rows):
         torch.cuda.synchronize()
         assert torch.equal(got, chain.w)
     del graph
+
+
+@pytest.mark.gpu
+def test_two_threads_on_their_per_thread_streams(lib, gpu_ctx):
+    """cudaStreamPerThread is one handle and another stream in each thread: the calls' pooled workspaces stay apart."""
+    import threading
+
+    import torch
+
+    per_thread, turns, rows, cols, m = 2, 40, 2000, 1000, 64
+    none = steps()
+
+    def randn(*shape):
+        return torch.randn(*shape, device="cuda", generator=g)
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, dy, mean = randn(2, rows, cols), randn(2, rows, cols), randn(2, rows)
+    rstd = torch.ones(rows, device="cuda")
+    a, scales = randn(2, m, D), randn(D, D // GROUP)
+    q = torch.randint(0, 256, (D, D // 2), generator=g, device="cuda", dtype=torch.uint8)
+
+    def calls(i, dgamma, dbeta, out, stream):
+        ok(lib.mxb_layer_norm_backward(gpu_ctx, ptr(dy[i]), cols, ptr(x[i]), cols, None, ptr(mean[i]), ptr(rstd), None, 0,
+                                       ptr(dgamma), ptr(dbeta), rows, cols, stream))
+        ok(lib.mxb_q4_gemm(gpu_ctx, ptr(a[i]), D, ptr(q), D // 2, ptr(scales), mlib.MXB_SCALE_F32, None, D // GROUP, GROUP,
+                           ptr(out), D, m, D, D, *none, stream))
+
+    def outputs(n):
+        return [(torch.zeros(cols, device="cuda"), torch.zeros(cols, device="cuda"), torch.zeros(m, D, device="cuda"))
+                for _ in range(n)]
+
+    want, got = outputs(2), [outputs(turns) for _ in range(2)]
+    for i in range(2):
+        calls(i, *want[i], current_stream())
+        torch.cuda.synchronize()
+    errors, begin = [], threading.Barrier(2)
+
+    def work(i):
+        try:
+            torch.cuda.set_device(0)
+            begin.wait()
+            for o in got[i]:
+                calls(i, *o, per_thread)
+            torch.cuda.synchronize()
+        except BaseException as e:  # noqa: BLE001 - reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i in range(2):
+        for turn, o in enumerate(got[i]):
+            assert all(torch.equal(v, w) for v, w in zip(o, want[i])), (i, turn)
+    assert lib.mxb_check_device_error(gpu_ctx) == 0
