@@ -390,7 +390,9 @@ MXB_API int mxb_layer_norm_backward(GpuCtx* ctx, const float* dy, long long lddy
  * M, N, K <= 2^30.  Products and sums are
  * fp32-faithful (the activations enter as exact bf16 parts, every
  * weight value q - z is exact in bf16, and each group's sum is scaled in
- * fp32), independent of the context's precision mode.  Workspace as for
+ * fp32), independent of the context's precision mode.  Infinities and NaN in A
+ * give what fp32 arithmetic gives; finite values have to leave a group's sum of
+ * A (q - z), before its scale, inside fp32's range.  Workspace as for
  * mxb_layer_norm_backward. */
 enum {
     MXB_SCALE_F32 = 0,
@@ -418,7 +420,10 @@ MXB_API int mxb_q4_gemm(GpuCtx* ctx, const float* A, long long lda, const unsign
  * RELU_GRAD as named above (i: the row of out), and ADD_ROW with
  * operand[e * ld_or_size + j] (ld_or_size 0: one row for all groups).
  * An ADD_FULL operand may be out itself (same pointer and pitch), otherwise
- * out overlaps no input.  precision as mxb_fused_gemm.  Needs no workspace.
+ * out overlaps no input.  precision as mxb_fused_gemm (in 3xTF32 an infinite
+ * operand can give NaN where fp32 gives an infinity, as it does there: it also
+ * meets the other operand's small part, which may be 0; TF32 has no such
+ * product).  Needs no workspace.
  * rows, N, K <= 2^30.  rows == 0 does nothing. */
 #define MXB_MAX_GROUPS 1024
 MXB_API int mxb_grouped_gemm(GpuCtx* ctx, const float* A, long long lda, const float* B, long long ldb,

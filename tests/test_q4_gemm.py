@@ -141,6 +141,33 @@ def test_bad_rows_stay_alone(lib, gpu_ctx, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,k,group", [(70, 200, 32), (5000, 700, 128)])
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 16, 40, 200])
+def test_infinite_activations(lib, gpu_ctx, m, n, k, group):
+    """An infinity gives what fp32 gives: infinity with its weight's sign, NaN against a weight of zero or against another
+    infinity of the other sign; the relu that follows keeps the positive ones.  NaN stays NaN whatever its payload."""
+    import torch
+
+    c = make(m, n, k, group, seed=m)
+    good = run(lib, gpu_ctx, c)
+    inf = float("inf")
+    c["a"][0, 5] = inf
+    if m > 2:
+        c["a"][2, k - 1], c["a"][2, 40] = -inf, inf
+    if m > 7:
+        c["a"][6, 7] = torch.tensor([0x7F800001], dtype=torch.int32, device="cuda").view(torch.float32)[0]  # NaN
+    out = run(lib, gpu_ctx, c)
+    want = c["a"].double() @ weight(c)
+    bad = ~torch.isfinite(want)
+    assert bad[0].all() and (torch.isinf(want[0]).any() and torch.isnan(want[0]).any())
+    assert torch.equal(out[bad].nan_to_num(7.0), want[bad].float().nan_to_num(7.0))
+    assert torch.equal(out[~bad], good[~bad])
+    relu = run(lib, gpu_ctx, c, steps((mlib.MXB_EP_RELU, None, 0, 0)))
+    assert torch.equal(relu, torch.where(out > 0, out, 0.0))
+    assert torch.isinf(relu[0]).any()
+
+
+@pytest.mark.gpu
 def test_rows_do_not_depend_on_their_number(lib, gpu_ctx):
     """Every row of a larger product is within the bound of the same row alone."""
     c = make(40, 333, 1000, 128, seed=3)
