@@ -380,9 +380,9 @@ MXB_API int mxb_layer_norm_backward(GpuCtx* ctx, const float* dy, long long lddy
  * No counterpart in the reference.  out[M,N] = epi(A[M,K] @ W), with W held
  * in 4 bits and a scale for each `group` values along K:
  *   W[k, n] = (q[n, k] - z[n, k / group]) * scales[n * lds + k / group].
- * Q: N rows of ldq bytes, two values to a byte, the lower k in the low four
+ * Q: N rows ldq bytes apart, two values to a byte, the lower k in the low four
  * bits (ldq % 16 == 0, 16-byte aligned, ldq >= (K + 1) / 2; what lies behind
- * column K is not used).  scales: MXB_SCALE_* values, row pitch lds elements;
+ * column K is not used, so Q may be some columns of a wider matrix).  scales: MXB_SCALE_* values, row pitch lds elements;
  * zeros: one byte (its low four bits) per scale, same pitch, or NULL for 8
  * everywhere.  group is a multiple of 32.  A needs a 16-byte aligned base and
  * lda % 4 == 0.  Epilogue steps as mxb_fused_gemm; an ADD_FULL operand may be

@@ -362,6 +362,9 @@ __global__ void __launch_bounds__(32 * kFewWarps)
     }
 }
 
+// What the copies read of a weight row: not its pitch, behind whose last row the caller's memory may end.
+unsigned long long weight_row_bytes(const Q4Params& p) { return (static_cast<unsigned long long>(p.K) + 1) / 2; }
+
 template <int PACK, int RT, int MT, int SHIFT>
 cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
     using C = FewCfg<PACK, RT, MT, SHIFT>;
@@ -380,7 +383,7 @@ cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
         }
     }
     CUtensorMap mw, ma;
-    const unsigned long long w_dims[2] = {static_cast<unsigned long long>(p.ldq), static_cast<unsigned long long>(p.N)};
+    const unsigned long long w_dims[2] = {weight_row_bytes(p), static_cast<unsigned long long>(p.N)};
     const unsigned long long w_stride[1] = {static_cast<unsigned long long>(p.ldq)};
     const unsigned w_box[2] = {C::kRun / 2, 16 * MT};
     const unsigned long long a_dims[2] = {static_cast<unsigned long long>(p.K), static_cast<unsigned long long>(p.M)};
@@ -915,7 +918,7 @@ int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
     const int runs = (p.K + 127) / 128;
     while (mp.splits < C::kMaxSplits && 2 * mp.splits * tiles <= ctx->num_sms && runs >= 4 * mp.splits) mp.splits *= 2;
     CUtensorMap mw, mx;
-    const unsigned long long w_dims[2] = {static_cast<unsigned long long>(p.ldq), static_cast<unsigned long long>(p.N)};
+    const unsigned long long w_dims[2] = {weight_row_bytes(p), static_cast<unsigned long long>(p.N)};
     const unsigned long long w_stride[1] = {static_cast<unsigned long long>(p.ldq)};
     const unsigned w_box[2] = {64, 128};
     const unsigned long long x_dims[3] = {static_cast<unsigned long long>(kp), static_cast<unsigned long long>(p.M), 3};

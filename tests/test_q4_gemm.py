@@ -168,6 +168,21 @@ def test_infinite_activations(lib, gpu_ctx, m, n, k, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 5, 16, 40, 300])
+@pytest.mark.parametrize("k", [1, 33, 500])
+def test_columns_of_a_wider_weight(lib, gpu_ctx, m, k):
+    """The last columns of K of a wider matrix, whose last row ends where the memory does: the copies read K columns of
+    a row, not its pitch."""
+    import torch
+
+    c = make(m, 100, k, 32, seed=m + k)
+    keep = -(-k // 32) * 16
+    wide = torch.randint(0, 256, (100, 512 + keep), dtype=torch.uint8, device="cuda")
+    wide[:, 512:512 + (k + 1) // 2] = c["q"][:, :(k + 1) // 2]
+    assert torch.equal(run(lib, gpu_ctx, dict(c, q=wide[:, 512:])), run(lib, gpu_ctx, c))
+
+
+@pytest.mark.gpu
 def test_rows_do_not_depend_on_their_number(lib, gpu_ctx):
     """Every row of a larger product is within the bound of the same row alone."""
     c = make(40, 333, 1000, 128, seed=3)
