@@ -71,13 +71,12 @@ struct NormGradParams {
 // Accesses under a predicate, for rows of single floats (W = 1): the compiler puts a branch around a conditional asm
 // statement, one for every access there (backward 20003 x 1027 74 -> 64 us without them, 2000 x 5001 42 -> 35).  Rows of
 // four have few such accesses, and keep the branch.
-__device__ __forceinline__ float load_if(bool wanted, const float* p) {
-    float v;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.global.cs.f32 %0, [%1];\n\t}"
-        : "=f"(v)
-        : "l"(p), "r"(static_cast<int>(wanted))
-        : "memory");
+__device__ __forceinline__ float load_if(bool wanted, const float* p, float otherwise) {
+    float v = otherwise;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.global.cs.f32 %0, [%1];\n\t}"
+                 : "+f"(v)
+                 : "l"(p), "r"(static_cast<int>(wanted))
+                 : "memory");
     return v;
 }
 __device__ __forceinline__ void store_if(bool wanted, float* p, float v) {
@@ -85,19 +84,18 @@ __device__ __forceinline__ void store_if(bool wanted, float* p, float v) {
                  "r"(static_cast<int>(wanted))
                  : "memory");
 }
-__device__ __forceinline__ float load_shared_if(bool wanted, uint32_t addr) {
-    float v;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.f32 %0, 0f00000000;\n\t@p ld.shared.f32 %0, [%1];\n\t}"
-        : "=f"(v)
-        : "r"(addr), "r"(static_cast<int>(wanted))
-        : "memory");
+__device__ __forceinline__ float load_shared_if(bool wanted, uint32_t addr, float otherwise) {
+    float v = otherwise;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\t@p ld.shared.f32 %0, [%1];\n\t}"
+                 : "+f"(v)
+                 : "r"(addr), "r"(static_cast<int>(wanted))
+                 : "memory");
     return v;
 }
 
-// W consecutive floats at p + c, zeros from column `cols` on.
+// W consecutive floats at p + c, `past` from column `cols` on.
 template <int W>
-__device__ __forceinline__ void load_unit(float (&v)[W], const float* p, int c, int cols) {
+__device__ __forceinline__ void load_unit(float (&v)[W], const float* p, int c, int cols, float past = 0.0f) {
     if (W == 4 && c + W <= cols) {
         const float4 t = __ldcs(reinterpret_cast<const float4*>(p + c));
         v[0] = t.x;
@@ -106,7 +104,7 @@ __device__ __forceinline__ void load_unit(float (&v)[W], const float* p, int c, 
         v[W > 3 ? 3 : 0] = t.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = W == 1 ? load_if(c < cols, p + c) : c + i < cols ? __ldcs(p + c + i) : 0.0f;
+        for (int i = 0; i < W; ++i) v[i] = W == 1 ? load_if(c < cols, p + c, past) : c + i < cols ? __ldcs(p + c + i) : past;
     }
 }
 
@@ -250,9 +248,10 @@ struct RowRing {
                 bulk_load(dst + m * row_slot_bytes(cols), reinterpret_cast<const void*>(s[m].begin), s[m].bytes, bar);
     }
 
-    // This thread's units of matrix m's row: from its slot or, at the matrix's ends, from where it lies.
+    // This thread's units of matrix m's row: from its slot or, at the matrix's ends, from where it lies; `past` behind it.
     template <int W, int NV>
-    __device__ __forceinline__ void take(float (&v)[NV][W], int m, long long row, int slot, int t, int threads) const {
+    __device__ __forceinline__ void take(float (&v)[NV][W], int m, long long row, int slot, int t, int threads,
+                                         float past = 0.0f) const {
         const int ahead = skip[slot][m];
         if (ahead >= 0) {
             const uint32_t at = slots + (slot * MATS + m) * row_slot_bytes(cols) + (ahead + t * W) * 4;
@@ -268,13 +267,13 @@ struct RowRing {
                 } else {
 #pragma unroll
                     for (int i = 0; i < W; ++i)
-                        v[u][i] = W == 1 || c + i < cols ? load_shared_if(c + i < cols, at + (u * threads * W + i) * 4) : 0.0f;
+                        v[u][i] = W == 1 || c + i < cols ? load_shared_if(c + i < cols, at + (u * threads * W + i) * 4, past) : past;
                 }
             }
         } else {
             const float* p = mats[m].base + row * mats[m].ld;
 #pragma unroll
-            for (int u = 0; u < NV; ++u) load_unit<W>(v[u], p, (u * threads + t) * W, cols);
+            for (int u = 0; u < NV; ++u) load_unit<W>(v[u], p, (u * threads + t) * W, cols, past);
         }
     }
 };
@@ -470,8 +469,9 @@ __device__ __forceinline__ NormStats saved_stats(const NormGradParams& p, long l
     return {__ldg(p.mean + row), __ldg(p.rstd + row)};
 }
 
-// One row of the backward pass, held by `threads` threads: xh and d come in as x and dy; dx goes out, and the
-// thread's columns of dgamma and dbeta grow.
+// One row of the backward pass, held by `threads` threads: xh and d come in as x and dy, the mean and 0 past the row's end
+// (not 0 and 0: a mean times rstd past fp32's range would make the sums NaN there); dx goes out, and the thread's columns
+// of dgamma and dbeta grow.
 template <int W, int NV, typename Sum>
 __device__ __forceinline__ void norm_grad_row(float (&xh)[NV][W], float (&d)[NV][W], float (&dg)[NV][W], float (&db)[NV][W],
                                               const float (&gamma)[NV][W], NormStats st, int t, int threads, long long row, const NormGradParams& p, float inv, Sum sum) {
@@ -481,7 +481,7 @@ __device__ __forceinline__ void norm_grad_row(float (&xh)[NV][W], float (&d)[NV]
     for (int u = 0; u < NV; ++u) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            // Columns past the row have d = 0: they add nothing to any sum.
+            // Columns past the row have xh = d = 0: they add nothing to any sum.
             xh[u][i] = (xh[u][i] - mean) * rstd;
             dg[u][i] += d[u][i] * xh[u][i];
             db[u][i] += d[u][i];
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(kWarpRowThreads) layer_norm_grad_warp_kernel(c
         float xh[NV][W], d[NV][W];
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            load_unit<W>(xh[u], p.x + row * p.ldx, (u * 32 + t) * W, p.cols);
+            load_unit<W>(xh[u], p.x + row * p.ldx, (u * 32 + t) * W, p.cols, st.mean);
             load_unit<W>(d[u], p.dy + row * p.lddy, (u * 32 + t) * W, p.cols);
         }
         norm_grad_row<W, NV>(xh, d, dg, db, gamma, st, t, 32, row, p, inv, [](float2 s) { return warp_sum(s); });
@@ -579,8 +579,8 @@ __global__ void __launch_bounds__(W * NV > 8 ? 512 : 1024) layer_norm_grad_block
         next = saved_stats(p, row + gridDim.x);
         if (!mbar_wait(ring.bar0 + 8 * slot, phase, p.timeout_ns)) atomicMin(&failed, round);
         float xh[NV][W], d[NV][W];
-        ring.take(xh, 0, row, slot, t, threads);
         ring.take(d, 1, row, slot, t, threads);
+        ring.take(xh, 0, row, slot, t, threads, st.mean);
         // The sum's barrier says that every thread has taken its part: the slot can be filled again.
         norm_grad_row<W, NV>(xh, d, dg, db, gamma, st, t, threads, row, p, inv, [&](float2 s) {
             s = row_sum(s);
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_wide_kernel(const NormGr
         float xh[NV][W], d[NV][W];
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
-            load_unit<W>(xh[u], p.x + row * p.ldx, (u * 1024 + t) * W, p.cols);
+            load_unit<W>(xh[u], p.x + row * p.ldx, (u * 1024 + t) * W, p.cols, st.mean);
             load_unit<W>(d[u], p.dy + row * p.lddy, (u * 1024 + t) * W, p.cols);
         }
         float2 s = make_float2(0.0f, 0.0f);
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(const NormGr
         float2 s = make_float2(0.0f, 0.0f);
         for (long long cc = threadIdx.x * W; cc < p.cols; cc += step) {
             const int c = static_cast<int>(cc);
-            load_unit<W>(xh, x, c, p.cols);
+            load_unit<W>(xh, x, c, p.cols, mean);
             load_unit<W>(d, dy, c, p.cols);
             load_param<W, false>(g, p.gamma, c, p.cols, 1.0f);
 #pragma unroll
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(const NormGr
         float* dx = p.dx + row * p.lddx;
         for (long long cc = threadIdx.x * W; cc < p.cols; cc += step) {
             const int c = static_cast<int>(cc);
-            load_unit<W>(xh, x, c, p.cols);
+            load_unit<W>(xh, x, c, p.cols, mean);
             load_unit<W>(d, dy, c, p.cols);
             load_param<W, false>(g, p.gamma, c, p.cols, 1.0f);
 #pragma unroll

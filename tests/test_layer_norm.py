@@ -165,6 +165,22 @@ def test_constant_rows_and_far_offsets(lib, gpu_ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(3, 5), (900, 30), (900, 129), (400, 1030), (400, 1027), (2, 515), (400, 12001),
+                                       (400, 12002), (3, 40001), (3, 40002)])
+def test_mean_far_past_the_spread(lib, gpu_ctx, rows, cols):
+    """Rows of one value 1e37: xhat is 0 and dx what is left of dy, though mean times rstd is past fp32's range."""
+    import torch
+
+    _, dy, gamma, _ = make(rows, cols, cols)
+    x = torch.full((rows, cols), 2.0 ** 123, device="cuda")
+    mean, rstd = x[:, 0].contiguous(), torch.full((rows,), 316.0, device="cuda")
+    pitch = (cols + 3) // 4 * 4
+    for p in (cols, pitch):
+        check_backward(dy, x, gamma, mean, rstd, *backward(lib, gpu_ctx, pitched(dy, p), pitched(x, p), gamma, mean, rstd,
+                                                           dx=pitched(torch.zeros_like(x), p)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("cols", [200, 3000, 40000])
 def test_bad_values_stay_in_their_row(lib, gpu_ctx, cols):
     import torch
