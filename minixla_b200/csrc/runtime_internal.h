@@ -20,6 +20,7 @@ namespace mxb {
 
 inline bool cuda_ok(cudaError_t e, const char* what) {
     if (e == cudaSuccess) return true;
+    cudaGetLastError();  // reported here, not by the next launch's check
     set_error("%s: %s", what, cudaGetErrorString(e));
     return false;
 }
@@ -248,7 +249,7 @@ cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t sme
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
     note_launch();
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return e;
 }
 
 // Workspace of one call: pooled and given back, stream-ordered, when the call

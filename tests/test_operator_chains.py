@@ -235,3 +235,37 @@ def test_two_threads_on_their_per_thread_streams(lib, gpu_ctx):
         for turn, o in enumerate(got[i]):
             assert all(torch.equal(v, w) for v, w in zip(o, want[i])), (i, turn)
     assert lib.mxb_check_device_error(gpu_ctx) == 0
+
+
+@pytest.mark.gpu
+def test_a_failed_call_leaves_no_error_behind(lib, gpu_ctx):
+    """A call on the legacy stream while a blocking stream is being captured is an error of that call alone."""
+    import ctypes as C
+
+    import torch
+
+    driver = C.CDLL("libcuda.so.1")
+    x, gamma = torch.randn(40, D, device="cuda"), torch.ones(D, device="cuda")
+    dy, mean, rstd, grads = torch.randn_like(x), torch.zeros(40, device="cuda"), torch.ones(40, device="cuda"), torch.zeros(2, D, device="cuda")
+
+    def backward(stream):
+        return lib.mxb_layer_norm_backward(gpu_ctx, ptr(dy), D, ptr(x), D, ptr(gamma), ptr(mean), ptr(rstd), None, 0,
+                                           ptr(grads[0]), ptr(grads[1]), 40, D, stream)
+
+    ok(backward(mlib.CUDA_STREAM_LEGACY))
+    torch.cuda.synchronize()
+    want = grads.clone()
+    grads.zero_()
+    torch.cuda.synchronize()
+    stream, graph = C.c_void_p(), C.c_void_p()
+    assert driver.cuStreamCreate(C.byref(stream), 0) == 0
+    assert driver.cuStreamBeginCapture_v2(stream, 0) == 0
+    try:
+        assert backward(mlib.CUDA_STREAM_LEGACY) < 0 and "captur" in mlib.last_error()
+    finally:
+        if driver.cuStreamEndCapture(stream, C.byref(graph)) == 0 and graph:
+            driver.cuGraphDestroy(graph)
+        assert driver.cuStreamDestroy_v2(stream) == 0
+    ok(backward(mlib.CUDA_STREAM_LEGACY))
+    torch.cuda.synchronize()
+    assert torch.equal(grads, want)
