@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
         tmem_relinquish();
     }
     wait_for_previous_kernel();
-    let_next_kernel_in();
+    if (warp == kMmaWarp) let_next_kernel_in();  // behind this CTA's allocation
     if (warp == kConvWarp) grouped_scan<kGradB, BT>(tab, p, lane);
     tc_fence_before();
     __syncthreads();
@@ -733,7 +733,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
         tmem_relinquish();
     }
     wait_for_previous_kernel();
-    let_next_kernel_in();
+    if (warp == kMmaWarp) let_next_kernel_in();  // behind this CTA's allocation
     if (warp == kConvWarp) grouped_scan<MODE, BT>(tab, p, lane);
     tc_fence_before();
     __syncthreads();
@@ -1120,7 +1120,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
         tmem_relinquish_pair();
     }
     wait_for_previous_kernel();
-    let_next_kernel_in();
+    if (warp == kMmaWarp) let_next_kernel_in();  // behind this CTA's allocation
     if (warp == kConvWarp) grouped_scan<MODE, BT>(tab, p, lane);
     __syncwarp();
     tc_fence_before();

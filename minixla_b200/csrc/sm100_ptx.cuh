@@ -360,7 +360,8 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // The stream's next kernel, if it was launched by launch_early, may take its place on the SMs as this one's blocks leave
-// (and wait there in turn); without it, once they all have.
+// (and wait there in turn); without it, once they all have.  One thread of each block is enough: a block that takes tensor
+// memory lets it come behind its own allocation, so that it never waits for tensor memory of a block that waits for it.
 __device__ __forceinline__ void let_next_kernel_in() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 // Loads for such kernels: they stay behind the wait, which the compiler need not respect with read-only loads (__ldg),
