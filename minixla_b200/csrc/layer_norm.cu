@@ -1006,8 +1006,13 @@ extern "C" {
 
 int mxb_layer_norm(GpuCtx* ctx, const float* x, long long ldx, const float* gamma, const float* beta, float eps,
                    float* y, long long ldy, float* mean, float* rstd, long long rows, int cols, void* stream) {
-    return mxb::layer_norm(ctx, mxb::NormParams{x, ldx, gamma, beta, eps, y, ldy, mean, rstd, rows, cols, 0, nullptr},
-                           stream);
+    try {
+        return mxb::layer_norm(ctx, mxb::NormParams{x, ldx, gamma, beta, eps, y, ldy, mean, rstd, rows, cols, 0, nullptr},
+                               stream);
+    } catch (const std::exception& e) {  // a lock that cannot be taken
+        mxb::set_error("mxb_layer_norm: %s", e.what());
+        return MXB_E_CUDA;
+    }
 }
 
 int mxb_layer_norm_backward(GpuCtx* ctx, const float* dy, long long lddy, const float* x, long long ldx,
