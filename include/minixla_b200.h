@@ -445,6 +445,17 @@ MXB_API int mxb_grouped_gemm_grad_b(GpuCtx* ctx, const float* A, long long lda, 
                    const int* offsets, int groups, float* dB, long long lddb, long long db_stride, float* dbias,
                    int rows, int N, int K, int precision, void* stream);
 
+/* Which kernel runs one of the three products (host-only, as mxb_gemm_plan_for):
+ * kernel: MXB_KERNEL_CTA_PAIR or MXB_KERNEL_SINGLE_CTA; tile_rows, tile_cols:
+ * a tile's rows (GRAD_B: of dB_e) and columns of the result; k_splits: the CTAs
+ * that share a tile's sum; products: groups. */
+enum {
+    MXB_GROUPED_FORWARD = 0,  /* mxb_grouped_gemm         */
+    MXB_GROUPED_GRAD_A = 1,   /* mxb_grouped_gemm_grad_a  */
+    MXB_GROUPED_GRAD_B = 2    /* mxb_grouped_gemm_grad_b  */
+};
+MXB_API int mxb_grouped_plan_for(int product, int rows, int groups, int N, int K, int num_sms, mxb_gemm_plan* plan);
+
 /* Synchronises the context's device work and reports a device-side error
  * recorded by a kernel (MXB_E_TIMEOUT after a bounded wait ran out), then
  * clears it.  0 when clean. */

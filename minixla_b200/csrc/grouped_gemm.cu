@@ -7,7 +7,7 @@
 // Three tcgen05 kernels: pairs of CTAs with tiles of 256 x 256 where groups
 // have many rows (all three products), a CTA with at most 64 rows to a tile
 // where they have few (forward, grad_a), and a CTA with 128 x 128 for grad_b's
-// small matrices.  run_grouped_mode has the rule.  The tile is turned around
+// small matrices.  plan_grouped has the rule.  The tile is turned around
 // compared with the dense GEMMs: the dimension along which the result is contiguous
 // (n, or k in grad_a) lies along the tensor core's 128 rows and TMEM lanes,
 // the ragged dimension (the group's rows; k in grad_b) along its columns.
@@ -43,7 +43,7 @@ namespace mxb {
 
 namespace {
 
-enum GroupedMode : int { kForward, kGradA, kGradB };
+enum GroupedMode : int { kForward = MXB_GROUPED_FORWARD, kGradA = MXB_GROUPED_GRAD_A, kGradB = MXB_GROUPED_GRAD_B };
 
 struct GroupedCall {
     int mode;
@@ -1446,27 +1446,52 @@ bool grouped_maps(const GroupedCall& g, bool round, CUtensorMap* lane, CUtensorM
            grouped_map(col, g.x, 0, g.rows, MODE == kForward ? g.K : g.N, g.ldx, 0, 32, false, round);
 }
 
-// At most so many column tiles, whatever the offsets are: a part of a tile more for each group that has a row.
-template <int MODE>
-long long most_col_tiles(const GroupedCall& g, int cols) {
-    return MODE == kGradB ? static_cast<long long>((g.K + cols - 1) / cols) * g.groups
-                          : g.rows / cols + std::min(g.groups, g.rows);
-}
+// Which kernel runs a product, its tile and the CTAs that share one.
+struct GroupedPlan {
+    bool pair;
+    int lanes, cols;   // of a tile: result columns, and rows of a group (grad_b: columns of A)
+    long long tiles;   // at most, for non-decreasing offsets
+    int cluster;       // CTAs that share a tile's sum
+};
 
 constexpr int kMaxSplits = 8;
 
-// Launches `kernel` for at most `tiles` tiles of about all_kb k-blocks: persistent CTAs, or clusters that share a tile
-// while every cluster still has SMs of its own and every CTA two k-blocks.
-template <typename Kernel>
-cudaError_t launch_clusters(Kernel kernel, int threads, int smem, long long tiles, int all_kb, int num_sms,
-                            cudaStream_t stream, const CUtensorMap& lane, const CUtensorMap& col, const GroupedParams& p) {
-    int splits = 1;
-    while (splits < kMaxSplits && 2 * splits * tiles <= num_sms && all_kb >= 4 * splits) splits *= 2;
-    const dim3 grid(static_cast<unsigned>(splits > 1 ? tiles * splits : std::min<long long>(tiles, num_sms)));
-    return launch_early(kernel, grid, dim3(threads), smem, stream, splits, lane, col, p, splits);
+GroupedPlan plan_grouped(int mode, int rows, int groups, int N, int K, int num_sms) {
+    const int lane_dim = mode == kGradA ? K : N;
+    // At most so many tiles, whatever the offsets are: a part of a column tile more for each group that has a row.
+    auto most_tiles = [&](int lanes, int cols) {
+        const long long col_tiles =
+            mode == kGradB ? static_cast<long long>((K + cols - 1) / cols) * groups : rows / cols + std::min(groups, rows);
+        return col_tiles * ((lane_dim + lanes - 1) / lanes);
+    };
+    // By the rows that a group has on average.  8 groups, 2048 x 4096, cold L2, a CTA with 64 rows to a tile / a pair
+    // with 256, in us: 80 rows 131 / -, 88 rows 131 / 127, 96 rows 133 / 129, 128 rows 166 / 135, 192 rows 228 / 191.
+    // A pair's tile is eight times the other's, so there also have to be enough of them for the pairs: 459 rows of 12
+    // groups, 811 x 1022, 32 us against the pairs' 42.  grad_b has its columns from K instead, and a CTA takes 128.
+    const int cols = mode == kGradB ? K : (rows + groups - 1) / groups;
+    const long long pair_tiles = most_tiles(256, GroupedPairCfg::kCols);
+    if (cols > 84 && lane_dim > 128 && pair_tiles >= num_sms * 3 / 8)
+        return {true, 256, GroupedPairCfg::kCols, pair_tiles, 2};
+    GroupedPlan plan{false, 128, mode == kGradB ? GroupedGradBCfg::kCols : GroupedFewCfg::kCols, 0, 1};
+    plan.tiles = most_tiles(plan.lanes, plan.cols);
+    // Clusters while each still has SMs of its own and every CTA two k-blocks (of grad_b's rows, if they are spread
+    // evenly, which is only a guess).
+    const int sum = mode == kForward ? K : mode == kGradA ? N : rows / groups;
+    const int all_kb = (sum + kBK - 1) / kBK;
+    while (plan.cluster < kMaxSplits && 2 * plan.cluster * plan.tiles <= num_sms && all_kb >= 4 * plan.cluster) plan.cluster *= 2;
+    return plan;
 }
 
-cudaError_t run_grouped_grad_b(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
+// Launches `kernel` as persistent CTAs, or as clusters that share a tile each.
+template <typename Kernel>
+cudaError_t launch_clusters(Kernel kernel, int threads, int smem, const GroupedPlan& plan, int num_sms, cudaStream_t stream,
+                            const CUtensorMap& lane, const CUtensorMap& col, const GroupedParams& p) {
+    const dim3 grid(static_cast<unsigned>(plan.cluster > 1 ? plan.tiles * plan.cluster : std::min<long long>(plan.tiles, num_sms)));
+    return launch_early(kernel, grid, dim3(threads), smem, stream, plan.cluster, lane, col, p, plan.cluster);
+}
+
+cudaError_t run_grouped_grad_b(const GroupedCall& g, GroupedParams& p, bool split3, const GroupedPlan& plan, int num_sms,
+                               cudaStream_t stream) {
     using C = GroupedGradBCfg;
     auto kernel = grouped_grad_b_kernel;
     static std::mutex mu;
@@ -1484,15 +1509,12 @@ cudaError_t run_grouped_grad_b(const GroupedCall& g, GroupedParams& p, bool spli
     }
     CUtensorMap lane, col;
     if (!grouped_maps<kGradB>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
-    p.lane_tiles = (p.lane_dim + 127) / 128;
-    const long long tiles = most_col_tiles<kGradB>(g, C::kCols) * p.lane_tiles;
-    // The k-blocks of a tile if the rows are spread evenly, which is only a guess.
-    const int all_kb = (g.rows / g.groups + kBK - 1) / kBK;
-    return launch_clusters(kernel, C::kThreads, C::kSmemBytes, tiles, all_kb, num_sms, stream, lane, col, p);
+    return launch_clusters(kernel, C::kThreads, C::kSmemBytes, plan, num_sms, stream, lane, col, p);
 }
 
 template <int MODE>
-cudaError_t run_grouped_few(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
+cudaError_t run_grouped_few(const GroupedCall& g, GroupedParams& p, bool split3, const GroupedPlan& plan, int num_sms,
+                            cudaStream_t stream) {
     using C = GroupedFewCfg;
     auto kernel = grouped_few_kernel<MODE>;
     static std::mutex mu;
@@ -1510,14 +1532,12 @@ cudaError_t run_grouped_few(const GroupedCall& g, GroupedParams& p, bool split3,
     }
     CUtensorMap lane, col;
     if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
-    p.lane_tiles = (p.lane_dim + 127) / 128;
-    const long long tiles = most_col_tiles<MODE>(g, C::kCols) * p.lane_tiles;
-    return launch_clusters(kernel, C::kThreads, C::kSmemBytes, tiles, (p.sum_dim + kBK - 1) / kBK, num_sms, stream, lane,
-                           col, p);
+    return launch_clusters(kernel, C::kThreads, C::kSmemBytes, plan, num_sms, stream, lane, col, p);
 }
 
 template <int MODE>
-cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
+cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3, const GroupedPlan& plan, int num_sms,
+                             cudaStream_t stream) {
     using C = GroupedPairCfg;
     auto kernel = grouped_pair_kernel<MODE>;
     static std::mutex mu;
@@ -1559,29 +1579,23 @@ cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3
     }
     CUtensorMap lane, col;
     if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
-    p.lane_tiles = (p.lane_dim + 255) / 256;
-    const int pairs =
-        static_cast<int>(std::min<long long>(most_col_tiles<MODE>(g, C::kCols) * p.lane_tiles, clusters));
+    const int pairs = static_cast<int>(std::min<long long>(plan.tiles, clusters));
     return launch_early(kernel, dim3(2 * pairs), dim3(C::kThreads), C::kSmemBytes, stream, 1, lane, col, p);
 }
 
 template <int MODE>
 cudaError_t run_grouped_mode(const GroupedCall& g, GroupedParams& p, bool split3, int num_sms, cudaStream_t stream) {
-    // By the rows that a group has on average.  8 groups, 2048 x 4096, cold L2, a CTA with 64 rows to a tile / a pair
-    // with 256, in us: 80 rows 131 / -, 88 rows 131 / 127, 96 rows 133 / 129, 128 rows 166 / 135, 192 rows 228 / 191.
-    // A pair's tile is eight times the other's, so there also have to be enough of them for the pairs: 459 rows of 12
-    // groups, 811 x 1022, 32 us against the pairs' 42.  grad_b has its columns from K instead, and a CTA takes 128.
-    const int cols = MODE == kGradB ? g.K : (g.rows + g.groups - 1) / g.groups;
-    const long long pair_tiles = most_col_tiles<MODE>(g, GroupedPairCfg::kCols) * ((p.lane_dim + 255) / 256);
-    if (cols > 84 && p.lane_dim > 128 && pair_tiles >= num_sms * 3 / 8) {
+    const GroupedPlan plan = plan_grouped(MODE, g.rows, g.groups, g.N, g.K, num_sms);
+    p.lane_tiles = (p.lane_dim + plan.lanes - 1) / plan.lanes;
+    if (plan.pair) {
         // (TF32 mode: the staged dY is rounded; the bias gradient is summed from memory.)
         p.dbias = split3 ? g.dbias : nullptr;
-        return run_grouped_pair<MODE>(g, p, split3, num_sms, stream);
+        return run_grouped_pair<MODE>(g, p, split3, plan, num_sms, stream);
     }
     if constexpr (MODE == kGradB) {
-        return run_grouped_grad_b(g, p, split3, num_sms, stream);
+        return run_grouped_grad_b(g, p, split3, plan, num_sms, stream);
     } else {
-        return run_grouped_few<MODE>(g, p, split3, num_sms, stream);
+        return run_grouped_few<MODE>(g, p, split3, plan, num_sms, stream);
     }
 }
 
@@ -1652,6 +1666,23 @@ int grouped_gemm(const char* fn, GpuCtx* ctx, const GroupedCall& g, const mxb_ep
 }  // namespace mxb
 
 extern "C" {
+
+int mxb_grouped_plan_for(int product, int rows, int groups, int N, int K, int num_sms, mxb_gemm_plan* plan) {
+    if (!plan || product < MXB_GROUPED_FORWARD || product > MXB_GROUPED_GRAD_B || rows < 1 || groups < 1 ||
+        groups > MXB_MAX_GROUPS || N < 1 || K < 1 || rows > mxb::kMaxExtent || N > mxb::kMaxExtent || K > mxb::kMaxExtent ||
+        num_sms < 2) {
+        mxb::set_error("mxb_grouped_plan_for: invalid arguments");
+        return MXB_E_ARG;
+    }
+    const mxb::GroupedPlan p = mxb::plan_grouped(product, rows, groups, N, K, num_sms);
+    memset(plan, 0, sizeof(*plan));
+    plan->kernel = p.pair ? MXB_KERNEL_CTA_PAIR : MXB_KERNEL_SINGLE_CTA;
+    plan->tile_rows = p.cols;
+    plan->tile_cols = p.lanes;
+    plan->k_splits = p.pair ? 1 : p.cluster;
+    plan->products = groups;
+    return MXB_OK;
+}
 
 int mxb_grouped_gemm(GpuCtx* ctx, const float* A, long long lda, const float* B, long long ldb, long long b_stride,
                      const int* offsets, int groups, float* out, long long ldo, int rows, int N, int K,

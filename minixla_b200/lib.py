@@ -23,6 +23,7 @@ MXB_OK, MXB_E_ARG, MXB_E_CUDA, MXB_E_NOMEM, MXB_E_TIMEOUT, MXB_E_UNSUPPORTED = 0
 MXB_MAX_EPILOGUE = 16
 MXB_MAX_PEERS = 7
 MXB_MAX_GROUPS = 1024
+MXB_GROUPED_FORWARD, MXB_GROUPED_GRAD_A, MXB_GROUPED_GRAD_B = range(3)
 # cudaStreamLegacy: torch's default stream has handle 0, which the library
 # reads as "the context's own stream"; this handle names the default stream.
 CUDA_STREAM_LEGACY = 1
@@ -107,6 +108,7 @@ PROTOTYPES = {
         [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p, C.c_longlong, C.c_void_p, C.c_int, C.c_void_p,
          C.c_longlong, C.c_longlong, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p],
     ),
+    "mxb_grouped_plan_for": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "mxb_check_device_error": (C.c_int, [C.c_void_p]),
     "mxb_selftest_wait_timeout": (C.c_int, [C.c_void_p, C.c_ulonglong]),
     "mxb_launch_count": (C.c_ulonglong, []),
@@ -141,6 +143,14 @@ def gemm_plan(M: int, N: int, K: int, precision: int, num_sms: int = 148, batch:
         rc = load().mxb_gemm_plan_for(M, N, K, precision, num_sms, C.byref(plan))
     if rc != 0:
         raise ValueError(f"mxb_gemm_plan_for: {last_error()}")
+    return plan
+
+
+def grouped_plan(product: int, rows: int, groups: int, N: int, K: int, num_sms: int = 148) -> GemmPlan:
+    """What mxb_grouped_plan_for reports for a product of ``rows`` rows in ``groups`` groups (host-only)."""
+    plan = GemmPlan()
+    if load().mxb_grouped_plan_for(product, rows, groups, N, K, num_sms, C.byref(plan)) != 0:
+        raise ValueError(f"mxb_grouped_plan_for: {last_error()}")
     return plan
 
 

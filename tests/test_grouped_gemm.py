@@ -228,8 +228,9 @@ def test_decreasing_offsets_where_clusters_share_sums(lib, gpu_ctx, rows, width,
     non-decreasing offsets can give, from which the grid of clusters was sized."""
     import torch
 
-    tiles, most = overlaps * -(-rows // 64), rows // 64 + groups
-    assert tiles > most and 2 * 4 * most <= 148 and length // 32 >= 16, "a shape for clusters of eight with a tile too many"
+    assert overlaps * -(-rows // 64) > rows // 64 + groups, "a tile more than clusters"
+    assert mlib.grouped_plan(mlib.MXB_GROUPED_FORWARD, rows, groups, width, length).k_splits == 8
+    assert mlib.grouped_plan(mlib.MXB_GROUPED_GRAD_A, rows, groups, length, width).k_splits == 8
     offsets = torch.tensor([e % 2 * rows for e in range(groups + 1)], dtype=torch.int32, device="cuda")
     for f, k, n in ((forward, length, width), (grad_a, width, length)):
         c = make([rows] + [0] * (groups - 1), k, n, seed=rows, ints=True)
@@ -452,6 +453,151 @@ def test_block_of_an_expert_mlp_trains_and_serves(lib, gpu_ctx):
                               (out, dx, dgamma, dbeta, dw1, db1, dw2, db2), (O, *want)):
         err = ((got.double() - ref).norm() / ref.norm()).item()
         assert err <= 1e-4, (name, err)
+
+
+# ---- the CTA-pair kernel, which takes groups of more than 84 rows where there are enough tiles
+
+PAIR_SIZES, PAIR_K, PAIR_N = [300, 0, 190, 257, 1, 256, 400, 196], 1030, 1100
+
+
+def make_for_pairs(**kw):
+    """A case whose three products all run there (of this or of the full GPU's SMs)."""
+    c = make(PAIR_SIZES, PAIR_K, PAIR_N, **kw)
+    for product in (mlib.MXB_GROUPED_FORWARD, mlib.MXB_GROUPED_GRAD_A, mlib.MXB_GROUPED_GRAD_B):
+        assert mlib.grouped_plan(product, c["rows"], c["groups"], PAIR_N, PAIR_K).kernel == mlib.MXB_KERNEL_CTA_PAIR
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", [X3, TF32], ids=["3xtf32", "tf32"])
+def test_pairs_against_definition(lib, gpu_ctx, precision):
+    c = make_for_pairs(seed=21, before=3, behind=5)
+    check_all(c, forward(lib, gpu_ctx, c, precision), grad_a(lib, gpu_ctx, c, precision),
+              *grad_b(lib, gpu_ctx, c, precision), precision)
+    assert lib.mxb_check_device_error(gpu_ctx) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", [X3, TF32], ids=["3xtf32", "tf32"])
+def test_pairs_steps_pitches_and_gaps(lib, gpu_ctx, precision):
+    import torch
+
+    c = make_for_pairs(seed=22, before=2, behind=3, pad=8)
+    groups, rows = c["groups"], c["rows"]
+    for f, x, width, length in ((forward, c["a"], PAIR_N, PAIR_K), (grad_a, c["dy"], PAIR_K, PAIR_N)):
+        bias = pitched(torch.randn(groups, width, device="cuda"), width + 5)
+        one = torch.randn(width, device="cuda")
+        full = pitched(torch.randn(rows, width, device="cuda"), width + 7)
+        gate = pitched(torch.randn(rows, width, device="cuda"), width + 3)
+        out = pitched(torch.full((rows, width), 77.0, device="cuda"), width + 9, 5.0)
+        st = steps((mlib.MXB_EP_ADD_ROW, bias, width + 5, 0), (mlib.MXB_EP_ADD_ROW, one, 0, 0),
+                   (mlib.MXB_EP_ADD_FULL, full, width + 7, 0), (mlib.MXB_EP_RELU, None, 0, 0),
+                   (mlib.MXB_EP_SCALE, None, 0, -0.5), (mlib.MXB_EP_RELU_GRAD, gate, width + 3, 0))
+        f(lib, gpu_ctx, c, precision, st, out)
+        for e in range(groups):
+            r = slice(c["at"][e], c["at"][e + 1])
+            if c["at"][e] == c["at"][e + 1]:
+                continue
+            a, b = x[r].double(), c["b"][e].double() if f is forward else c["b"][e].double().t()
+            pre = a @ b
+            added = bias[e].double() + one.double() + full[r].double()
+            want = torch.where(gate[r] > 0, (pre + added).clamp(min=0) * -0.5, 0.0)
+            tol = bound(a.abs() @ b.abs(), length, precision) + 8 * U * (
+                pre.abs() + bias[e].double().abs() + one.double().abs() + full[r].double().abs())
+            within(out[r], want, tol)
+        assert (out.as_strided((rows, width + 9), (width + 9, 1))[:, width:] == 5.0).all()
+        assert (out[:2] == 77.0).all() and (out[rows - 3:] == 77.0).all()
+    db = pitched(torch.full((groups, PAIR_K, PAIR_N), 77.0, device="cuda"), PAIR_N + 3, 5.0)
+    _, dbias = grad_b(lib, gpu_ctx, c, precision, db=db)
+    check_all(c, None, None, db, dbias, precision)
+    assert (db.as_strided((groups * PAIR_K, PAIR_N + 3), (PAIR_N + 3, 1))[:, PAIR_N:] == 5.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", [X3, TF32], ids=["3xtf32", "tf32"])
+def test_pairs_bad_values_stay_in_their_group(lib, gpu_ctx, precision):
+    import torch
+
+    c = make_for_pairs(seed=23, before=2, behind=4)
+    at = c["at"]
+    good = [forward(lib, gpu_ctx, c, precision), grad_a(lib, gpu_ctx, c, precision), *grad_b(lib, gpu_ctx, c, precision)]
+    nan = float("nan")
+    for t in (c["a"], c["dy"]):
+        t[:2], t[-4:] = nan, float("inf")
+        t[at[3]] = nan  # the first row of the group behind two others in its tiles' boxes
+    c["b"][1] = nan     # of an empty group
+    out, da = forward(lib, gpu_ctx, c, precision), grad_a(lib, gpu_ctx, c, precision)
+    db, dbias = grad_b(lib, gpu_ctx, c, precision)
+    r = torch.arange(c["rows"], device="cuda")
+    keep = (r >= at[0]) & (r < at[-1]) & (r != at[3])
+    assert (out[keep] == good[0][keep]).all() and (da[keep] == good[1][keep]).all()
+    assert torch.isnan(out[at[3]]).all() and torch.isnan(da[at[3]]).all()
+    others = [0, 1, 2, 4, 5, 6, 7]
+    assert (db[others] == good[2][others]).all() and (dbias[others] == good[3][others]).all()
+    assert torch.isnan(db[3]).all() and torch.isnan(dbias[3]).all() and (db[1] == 0).all() and (dbias[1] == 0).all()
+
+
+@pytest.mark.gpu
+def test_pairs_added_to_the_output_itself(lib, gpu_ctx):
+    import torch
+
+    c = make_for_pairs(seed=24, ints=True)
+    for f, x, width in ((forward, c["a"], PAIR_N), (grad_a, c["dy"], PAIR_K)):
+        out = torch.randint(-9, 10, (c["rows"], width), device="cuda").float()
+        want = out.double()
+        for e in range(c["groups"]):
+            r = slice(c["at"][e], c["at"][e + 1])
+            b = c["b"][e].double()
+            want[r] += x[r].double() @ (b if f is forward else b.t())
+        f(lib, gpu_ctx, c, st=steps((mlib.MXB_EP_ADD_FULL, out, out.stride(0), 0)), out=out)
+        assert (out == want).all()
+
+
+@pytest.mark.gpu
+def test_pairs_with_decreasing_offsets(lib, gpu_ctx):
+    """Four groups of all the rows: more tiles than the grid was sized for."""
+    import torch
+
+    c = make_for_pairs(seed=25, ints=True)
+    c["off"] = torch.tensor([e % 2 * c["rows"] for e in range(9)], dtype=torch.int32, device="cuda")
+    for f, x in ((forward, c["a"]), (grad_a, c["dy"])):
+        got = f(lib, gpu_ctx, c)
+        found = torch.zeros_like(got, dtype=torch.bool)
+        for b in c["b"][::2].double():
+            found |= got == x.double() @ (b if f is forward else b.t())
+        assert found.all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("precision", [X3, TF32], ids=["3xtf32", "tf32"])
+def test_pairs_captured_and_on_other_streams(lib, gpu_ctx, precision):
+    import torch
+
+    c = make_for_pairs(seed=26)
+    calls = lambda: (forward(lib, gpu_ctx, c, precision), grad_a(lib, gpu_ctx, c, precision),  # noqa: E731
+                     *grad_b(lib, gpu_ctx, c, precision))
+    want, again = calls(), calls()
+    assert all((a == b).all() for a, b in zip(want, again)), "the same inputs gave other bits"
+    got = {}
+    graph = captured(lambda: got.update(r=calls()))
+    at = [0]
+    for size in PAIR_SIZES[::-1]:
+        at.append(at[-1] + size)
+    c["off"].copy_(torch.tensor(at, dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    moved = calls()
+    assert all((a == b).all() for a, b in zip(got["r"], moved))
+    c["off"].copy_(torch.tensor(c["at"], dtype=torch.int32))
+    torch.cuda.synchronize()
+    outs = []
+    for s in (torch.cuda.Stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(s):
+            outs.append(calls())
+    torch.cuda.synchronize()
+    assert all((a == b).all() for o in outs for a, b in zip(o, want))
+    assert lib.mxb_check_device_error(gpu_ctx) == 0
+    del graph
 
 
 @pytest.mark.parametrize("which", ["mxb_grouped_gemm", "mxb_grouped_gemm_grad_a"])

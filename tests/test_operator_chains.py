@@ -100,6 +100,33 @@ def test_captured_chain(lib, gpu_ctx, rows):
 
 
 @pytest.mark.gpu
+def test_chain_with_cta_pairs(lib, gpu_ctx):
+    """A chain whose grouped product runs on CTA pairs: without a pause, and captured."""
+    import torch
+
+    rows = 8000
+    assert mlib.grouped_plan(mlib.MXB_GROUPED_FORWARD, rows, EXPERTS, D, D).kernel == mlib.MXB_KERNEL_CTA_PAIR
+    chain = Chain(lib, gpu_ctx, rows)
+    chain.reset()
+    want = [t.clone() for t in chain.run(torch.cuda.synchronize)]
+    assert all(torch.isfinite(t).all() for t in want)
+    for _ in range(3):
+        chain.reset()
+        torch.cuda.synchronize()
+        got = chain.run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+    def turn():
+        chain.reset()
+        chain.run()
+
+    graph = captured(turn, replays=3)
+    assert all(torch.equal(g, w) for g, w in zip((chain.x, chain.gamma), want))
+    del graph
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 16, 300])
 def test_calls_behind_another_stream(lib, gpu_ctx, rows):
     """A call whose stream waits for an event of another stream reads what that stream wrote."""
