@@ -104,6 +104,26 @@ def test_forward_and_backward(lib, gpu_ctx, rows, cols):
     check_backward(dy, x, gamma, mean, rstd, *backward(lib, gpu_ctx, dy, x, gamma, mean, rstd))
 
 
+# Rows for which every block of the ring kernels refills each slot at least once: a block of t threads has at most
+# 2048 / t neighbours on one of 148 SMs, and a ring at most eight slots.
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols,threads", [(1027, 64), (1028, 64), (2051, 128), (2052, 128), (4099, 256), (4100, 256),
+                                          (8191, 512), (8192, 512)])
+def test_ring_refills_its_slots(lib, gpu_ctx, cols, threads):
+    """Widths of a block's rows, odd ones (a refilled slot then has another skip) and multiples of four."""
+    rows = 2 * 8 * 148 * (2048 // threads) + 5
+    x, dy, gamma, beta = make(rows, cols, cols)
+    y, mean, rstd = forward(lib, gpu_ctx, x, gamma, beta)
+    got = backward(lib, gpu_ctx, dy, x, gamma, mean, rstd)
+    part = 4096
+    for r in range(0, rows, part):
+        s = slice(r, min(rows, r + part))
+        check_forward(x[s], gamma, beta, y[s], mean[s], rstd[s])
+        check_backward(dy[s], x[s], gamma, mean[s], rstd[s], got[0][s], None, None)
+    check_backward(dy, x, gamma, mean, rstd, None, *got[1:])
+    assert lib.mxb_check_device_error(gpu_ctx) == 0
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("cols,pitch", [(96, 100), (96, 97), (1023, 1024), (1030, 1031), (5000, 5004)])
 def test_pitches_and_unaligned_bases(lib, gpu_ctx, cols, pitch):
