@@ -78,6 +78,45 @@ def test_against_definition(lib, gpu_ctx, m, n, k, group):
             check(c, run(lib, gpu_ctx, c))
 
 
+# Weights wide enough for the wider tiles of the few-row kernel (32 columns a warp tile from 24 columns an SM, 64 for more than
+# eight rows from 32) and long enough that each warp's ring goes round more than once; widths that end inside a tile.
+WIDE = [(1, 3555, 8200, 128), (1, 5000, 8200, 96), (2, 4100, 8200, 128), (2, 4100, 8200, 32), (2, 1000, 16500, 64),
+        (4, 3601, 4200, 256), (8, 4097, 8192, 32), (8, 4097, 8192, 128), (12, 3600, 4200, 64), (12, 3600, 4200, 128),
+        (9, 4800, 2049, 32), (16, 5000, 8200, 32), (16, 5000, 8200, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,group", WIDE)
+def test_wide_weights_for_few_rows(lib, gpu_ctx, m, n, k, group):
+    for scale, zeros in (("f32", True), ("f16", False), ("bf16", True)):
+        c = make(m, n, k, group, scale, zeros, seed=m + n + k)
+        check(c, run(lib, gpu_ctx, c))
+    assert lib.mxb_check_device_error(gpu_ctx) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(1, 4000), (2, 150), (2, 4000), (8, 4000), (13, 4000), (16, 5000)])
+def test_wide_weights_exactly(lib, gpu_ctx, m, n):
+    """Integer activations of very different sizes in the rows, scales of one: every sum is exact."""
+    import torch
+
+    k = 3000
+    c = make(m, n, k, 96 if n == 150 else 128, seed=m)
+    big = 2.0 ** (torch.arange(m, device="cuda") % 5 * 20 - 40)
+    c["a"] = torch.randint(-9, 10, (m, k), device="cuda").float() * big[:, None]
+    c["s"].fill_(1.0)
+    assert (run(lib, gpu_ctx, c).double() == c["a"].double() @ weight(c)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("size", [1e-20, 1e-3, 1e20])
+def test_large_and_tiny_activations_of_one_or_two_rows(lib, gpu_ctx, m, size):
+    c = make(m, 4000, 3000, 128, seed=m)
+    c["a"] = c["a"] * size
+    check(c, run(lib, gpu_ctx, c))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 3, 8, 16, 40, 200])
 def test_exact_small_integers(lib, gpu_ctx, m):
