@@ -32,6 +32,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <exception>
 
 #include "gemm_common.cuh"
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
                     const GroupedTile g = grouped_tile<kGradB, BT>(tab, t, p);
                     const int col_boxes = (g.cols + 31) / 32;
                     int kb0;
-                const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
+                    const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
                     for (int kb = kb0; kb < kb1; ++kb) {
                         if (*abort_flag || !mbar_wait(empty_bar(stage), phase ^ 1u, p.timeout_ns)) {
                             raise_grouped(p, abort_flag, kErrProducer);
@@ -436,9 +437,9 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
             uint32_t small_phase = 0, acc_phase = 0;
             bool ok = true;
             for (int round = 0; ok; ++round) {
-                    const int t = grouped_turn(round, team, teams, total_tiles);
-                    if (t == -2) break;
-                    if (t < 0) continue;
+                const int t = grouped_turn(round, team, teams, total_tiles);
+                if (t == -2) break;
+                if (t < 0) continue;
                 const GroupedTile g = grouped_tile<kGradB, BT>(tab, t, p);
                 const uint32_t idesc = idesc_tf32_major(128, (g.cols + 15) & ~15, 1, 1);
                 int kb0;
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
                         // The last k-block ends with its own eighth: nothing past the sum is multiplied.
                         const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
                         const uint32_t begun = in_seg > 1 ? 1u : 0u;
-    #pragma unroll
+#pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
                             if (kk >= steps) break;
                             const uint64_t da = smem_desc_of(kHi, bl + kk * kStep);
@@ -506,13 +507,13 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
         uint32_t phase = 0, small_phase = 0;
         bool failed = false;
         for (int round = 0; !failed; ++round) {
-                const int t = grouped_turn(round, team, teams, total_tiles);
-                if (t == -2) break;
-                if (t < 0) continue;
+            const int t = grouped_turn(round, team, teams, total_tiles);
+            if (t == -2) break;
+            if (t < 0) continue;
             const GroupedTile g = grouped_tile<kGradB, BT>(tab, t, p);
             const int col_boxes = (g.cols + 31) / 32;
             int kb0;
-                const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
+            const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
             for (int kb = kb0; kb < kb1; ++kb) {
                 const bool stop = __any_sync(0xffffffffu, *abort_flag != 0);
                 const bool got = !stop && mbar_wait(full_bar(stage), phase, p.timeout_ns) &&
@@ -543,12 +544,12 @@ __global__ void __launch_bounds__(GroupedGradBCfg::kThreads, 1)
         uint32_t acc_phase = 0;
         bool failed = false;
         for (int round = 0; !failed; ++round) {
-                const int t = grouped_turn(round, team, teams, total_tiles);
-                if (t == -2) break;
-                if (t < 0) continue;
+            const int t = grouped_turn(round, team, teams, total_tiles);
+            if (t == -2) break;
+            if (t < 0) continue;
             const GroupedTile g = grouped_tile<kGradB, BT>(tab, t, p);
             int kb0;
-                const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
+            const int kb1 = my_part((g.sum + kBK - 1) / kBK, kb0);
             float total[C::kTotals];
 #pragma unroll
             for (int i = 0; i < C::kTotals; ++i) total[i] = 0.0f;
@@ -772,7 +773,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
                         mbar_arrive_expect_tx(fb, C::kLaneBytes + col_boxes * kBoxBytes);
                         const int q0 = kb * kBK;
                         if (MODE == kForward) {
-    #pragma unroll
+#pragma unroll
                             for (int j = 0; j < 4; ++j)
                                 tma_load_3d(st + j * kBoxBytes, &tm_lane, fb, g.lane0 + 32 * j, q0, g.group);
                         } else {
@@ -827,7 +828,7 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
                     const uint32_t bc = smem_desc_lo(big + C::kLaneBytes, 16);
                     const int steps = min(4, (g.sum - kb * kBK + 7) / 8);
                     const uint32_t begun = in_seg > 1 ? 1u : 0u;
-    #pragma unroll
+#pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
                         if (kk >= steps) break;
                         const uint64_t db = smem_desc_of(kHiK, bc + kk * 2);
@@ -1270,9 +1271,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
         uint32_t phase = 0, small_phase = 0, sum_phase = 0;
         bool failed = false;
         for (int round = 0; !failed; ++round) {
-                const int t = grouped_turn(round, pair, num_pairs, total_tiles);
-                if (t == -2) break;
-                if (t < 0) continue;
+            const int t = grouped_turn(round, pair, num_pairs, total_tiles);
+            if (t == -2) break;
+            if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
             const bool sums = MODE == kGradB && p.dbias && g.col0 == 0;  // the bias gradient, once for each lane tile
             float sum[MODE == kGradB ? 16 : 1];
@@ -1336,9 +1337,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedPairCfg::kThr
         uint32_t acc_phase = 0;
         bool failed = false;
         for (int round = 0; !failed; ++round) {
-                const int t = grouped_turn(round, pair, num_pairs, total_tiles);
-                if (t == -2) break;
-                if (t < 0) continue;
+            const int t = grouped_turn(round, pair, num_pairs, total_tiles);
+            if (t == -2) break;
+            if (t < 0) continue;
             const GroupedTile g = grouped_tile<MODE, BT, 256>(tab, t, p);
             const int num_kb = (g.sum + kBK - 1) / kBK;
             float total[C::kTotals];
@@ -1418,8 +1419,6 @@ __global__ void __launch_bounds__(1024) grouped_column_sums(const float* dy, lon
     if (threadIdx.x == 0 && cc < N) dbias[static_cast<long long>(e) * N + cc] = s;
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 // Row-major [groups][rows][cols] (groups 0: a plain [rows][cols]) read in boxes of box_rows x 32 floats,
 // rounded to TF32 by the copy or (3xTF32) as it is.
 bool grouped_map(CUtensorMap* map, const float* base, int groups, long long rows, long long cols, long long ld,
@@ -1493,46 +1492,22 @@ cudaError_t launch_clusters(Kernel kernel, int threads, int smem, const GroupedP
 cudaError_t run_grouped_grad_b(const GroupedCall& g, GroupedParams& p, bool split3, const GroupedPlan& plan, int num_sms,
                                cudaStream_t stream) {
     using C = GroupedGradBCfg;
-    auto kernel = grouped_grad_b_kernel;
-    static std::mutex mu;
-    static uint64_t configured = 0;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    const cudaError_t e = allow_shared<grouped_grad_b_kernel>(C::kSmemBytes);
     if (e != cudaSuccess) return e;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (dev >= 64 || !(configured & (1ull << dev))) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
-            if (e != cudaSuccess) return e;
-            if (dev < 64) configured |= 1ull << dev;
-        }
-    }
     CUtensorMap lane, col;
     if (!grouped_maps<kGradB>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
-    return launch_clusters(kernel, C::kThreads, C::kSmemBytes, plan, num_sms, stream, lane, col, p);
+    return launch_clusters(grouped_grad_b_kernel, C::kThreads, C::kSmemBytes, plan, num_sms, stream, lane, col, p);
 }
 
 template <int MODE>
 cudaError_t run_grouped_few(const GroupedCall& g, GroupedParams& p, bool split3, const GroupedPlan& plan, int num_sms,
                             cudaStream_t stream) {
     using C = GroupedFewCfg;
-    auto kernel = grouped_few_kernel<MODE>;
-    static std::mutex mu;
-    static uint64_t configured = 0;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    const cudaError_t e = allow_shared<grouped_few_kernel<MODE>>(C::kSmemBytes);
     if (e != cudaSuccess) return e;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (dev >= 64 || !(configured & (1ull << dev))) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
-            if (e != cudaSuccess) return e;
-            if (dev < 64) configured |= 1ull << dev;
-        }
-    }
     CUtensorMap lane, col;
     if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;
-    return launch_clusters(kernel, C::kThreads, C::kSmemBytes, plan, num_sms, stream, lane, col, p);
+    return launch_clusters(grouped_few_kernel<MODE>, C::kThreads, C::kSmemBytes, plan, num_sms, stream, lane, col, p);
 }
 
 template <int MODE>
@@ -1540,42 +1515,29 @@ cudaError_t run_grouped_pair(const GroupedCall& g, GroupedParams& p, bool split3
                              cudaStream_t stream) {
     using C = GroupedPairCfg;
     auto kernel = grouped_pair_kernel<MODE>;
-    static std::mutex mu;
-    static uint64_t configured = 0;
-    static int max_clusters[64] = {0};
+    cudaError_t e = allow_shared<grouped_pair_kernel<MODE>>(C::kSmemBytes);
     int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    int clusters = num_sms / 2;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (dev >= 64 || !(configured & (1ull << dev))) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
-            if (e != cudaSuccess) return e;
-            cudaLaunchConfig_t cfg = {};
-            cudaLaunchAttribute attr;
-            attr.id = cudaLaunchAttributeClusterDimension;
-            attr.val.clusterDim.x = 2;
-            attr.val.clusterDim.y = 1;
-            attr.val.clusterDim.z = 1;
-            cfg.gridDim = dim3(2 * clusters, 1, 1);
-            cfg.blockDim = dim3(C::kThreads, 1, 1);
-            cfg.dynamicSmemBytes = C::kSmemBytes;
-            cfg.attrs = &attr;
-            cfg.numAttrs = 1;
-            int n = 0;
-            if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
-                cudaGetLastError();
-                n = clusters;
-            }
-            clusters = n;
-            if (dev < 64) {
-                max_clusters[dev] = n;
-                configured |= 1ull << dev;
-            }
-        } else {
-            clusters = max_clusters[dev];
+    static std::atomic<int> max_clusters[64];  // by device; 0: not asked yet
+    int clusters = dev < 64 ? max_clusters[dev].load() : 0;
+    if (!clusters) {
+        cudaLaunchConfig_t cfg = {};
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.gridDim = dim3(num_sms / 2 * 2, 1, 1);
+        cfg.blockDim = dim3(C::kThreads, 1, 1);
+        cfg.dynamicSmemBytes = C::kSmemBytes;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+            cudaGetLastError();
+            clusters = num_sms / 2;
         }
+        if (dev < 64) max_clusters[dev].store(clusters);
     }
     CUtensorMap lane, col;
     if (!grouped_maps<MODE>(g, !split3, &lane, &col)) return cudaErrorInvalidValue;

@@ -744,8 +744,6 @@ __global__ void __launch_bounds__(32 * ROWS) sum_partials_kernel(const float* pa
     }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 constexpr int kBlockThreads = 512;                      // of a block that holds more than kWideFloats of a row a thread
 constexpr int kWideThreads = 1024, kWideFloats = 8;
 
@@ -808,19 +806,7 @@ int ring_slots(int blocks, int cols, int mats) {
     return std::max(2, std::min(kMaxSlots, 216 * 1024 / std::min(blocks, 16) / (mats * row_slot_bytes(cols))));
 }
 
-// Allows `kernel` the shared memory that a ring may take, once per device.
-template <typename Kernel>
-cudaError_t allow_ring(Kernel kernel, uint64_t* done) {
-    static std::mutex mu;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    std::lock_guard<std::mutex> lock(mu);
-    if (dev < 64 && (*done & (1ull << dev))) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
-    if (e == cudaSuccess && dev < 64) *done |= 1ull << dev;
-    return e;
-}
+constexpr int kRingBytes = 224 * 1024;  // of shared memory that a ring may take, or the wide kernel's sums
 
 constexpr int kNormFloats = 32;      // of a row per thread: 1024 columns per warp, 16384 per block
 constexpr int kNormGradFloats = 16;  // x, dy and two sums for each: 512 columns per warp, 8192 per block
@@ -833,8 +819,7 @@ cudaError_t launch_norm(const NormParams& p, const RowPlan& plan, int num_sms, c
             std::min<long long>(want, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_warp_kernel<W, NV>>(kWarpRowThreads, 0)));
         return launch_early(layer_norm_warp_kernel<W, NV>, dim3(blocks), dim3(kWarpRowThreads), 0, stream, 1, p);
     } else {
-        static uint64_t allowed = 0;
-        const cudaError_t e = allow_ring(layer_norm_block_kernel<W, NV>, &allowed);
+        const cudaError_t e = allow_shared<layer_norm_block_kernel<W, NV>>(kRingBytes);
         if (e != cudaSuccess) return e;
         const int slots = ring_slots(blocks_per_sm<layer_norm_block_kernel<W, NV>>(plan.threads, 0), p.cols, 1);
         const size_t smem = static_cast<size_t>(slots) * row_slot_bytes(p.cols);
@@ -878,8 +863,7 @@ cudaError_t launch_norm_grad(const NormGradParams* p, const RowPlan& plan, long 
         const int slots = ring_slots(blocks_per_sm<layer_norm_grad_block_kernel<W, NV>>(plan.threads, 0), cols, 2);
         const size_t smem = static_cast<size_t>(slots) * 2 * row_slot_bytes(cols);
         if (!p) {
-            static uint64_t allowed = 0;
-            const cudaError_t e = allow_ring(layer_norm_grad_block_kernel<W, NV>, &allowed);
+            const cudaError_t e = allow_shared<layer_norm_grad_block_kernel<W, NV>>(kRingBytes);
             if (e != cudaSuccess) return e;
             *blocks = static_cast<int>(
                 std::min<long long>(rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_grad_block_kernel<W, NV>>(plan.threads, smem)));
@@ -906,8 +890,7 @@ cudaError_t launch_norm_grad_width(const NormGradParams* p, long long rows, int 
     if (cols <= 16 * 1024) {
         const size_t smem = 2 * sizeof(float) * cols;
         if (!p) {
-            static uint64_t allowed = 0;
-            const cudaError_t e = allow_ring(layer_norm_grad_wide_kernel<W>, &allowed);
+            const cudaError_t e = allow_shared<layer_norm_grad_wide_kernel<W>>(kRingBytes);
             if (e != cudaSuccess) return e;
             *blocks = static_cast<int>(
                 std::min<long long>(rows, static_cast<long long>(num_sms) * blocks_per_sm<layer_norm_grad_wide_kernel<W>>(kWideThreads, smem)));

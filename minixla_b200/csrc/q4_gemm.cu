@@ -8,7 +8,6 @@
 
 #include <algorithm>
 #include <exception>
-#include <mutex>
 
 #include "epilogue_cell.cuh"
 #include "runtime_internal.h"
@@ -368,20 +367,8 @@ unsigned long long weight_row_bytes(const Q4Params& p) { return (static_cast<uns
 template <int PACK, int RT, int MT, int SHIFT>
 cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
     using C = FewCfg<PACK, RT, MT, SHIFT>;
-    auto kernel = q4_few_rows_kernel<PACK, RT, MT, SHIFT>;
-    static std::mutex mu;
-    static uint64_t configured = 0;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    const cudaError_t e = allow_shared<q4_few_rows_kernel<PACK, RT, MT, SHIFT>>(C::kSmem);
     if (e != cudaSuccess) return e;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (dev >= 64 || !(configured & (1ull << dev))) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-            if (e != cudaSuccess) return e;
-            if (dev < 64) configured |= 1ull << dev;
-        }
-    }
     CUtensorMap mw, ma;
     const unsigned long long w_dims[2] = {weight_row_bytes(p), static_cast<unsigned long long>(p.N)};
     const unsigned long long w_stride[1] = {static_cast<unsigned long long>(p.ldq)};
@@ -396,8 +383,9 @@ cudaError_t run_few_rows(const Q4Params& p, cudaStream_t stream) {
                            PACK ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B))
         return cudaErrorInvalidValue;
-    return launch_early(kernel, dim3((p.N + 16 * MT - 1) / (16 * MT), (p.M + C::kRows - 1) / C::kRows),
-                        dim3(32 * kFewWarps), C::kSmem, stream, 1, mw, ma, p);
+    return launch_early(q4_few_rows_kernel<PACK, RT, MT, SHIFT>,
+                        dim3((p.N + 16 * MT - 1) / (16 * MT), (p.M + C::kRows - 1) / C::kRows), dim3(32 * kFewWarps), C::kSmem,
+                        stream, 1, mw, ma, p);
 }
 
 template <int PACK, int RT, int MT>
@@ -872,17 +860,7 @@ __global__ void __launch_bounds__(ManyCfg::kThreads, 1)
 
 int run_many_rows(GpuCtx* ctx, const Q4Params& p, cudaStream_t stream) {
     using C = ManyCfg;
-    static std::mutex mu;
-    static uint64_t configured = 0;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (ctx->device >= 64 || !(configured & (1ull << ctx->device))) {
-            if (!cuda_ok(cudaFuncSetAttribute(q4_many_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem),
-                         "4-bit product set-up"))
-                return MXB_E_CUDA;
-            if (ctx->device < 64) configured |= 1ull << ctx->device;
-        }
-    }
+    if (!cuda_ok(allow_shared<q4_many_rows_kernel>(C::kSmem), "4-bit product set-up")) return MXB_E_CUDA;
     const long long kp = (static_cast<long long>(p.K) + kManyK - 1) / kManyK * kManyK;
     Scratch scratch(ctx, stream);
     void* parts = scratch.alloc(static_cast<size_t>(3) * p.M * kp * 2);

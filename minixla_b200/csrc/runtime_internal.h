@@ -9,6 +9,7 @@
 
 #include <atomic>
 #include <cstddef>
+#include <cstdint>
 #include <mutex>
 #include <unordered_map>
 #include <utility>
@@ -225,6 +226,23 @@ struct GpuCtx {
 };
 
 namespace mxb {
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Allows `kernel` launches with up to `bytes` of dynamic shared memory, once per device.
+template <auto kernel>
+cudaError_t allow_shared(int bytes) {
+    static std::mutex mu;
+    static uint64_t done = 0;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev < 64 && (done >> dev & 1)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done |= 1ull << dev;
+    return e;
+}
 
 // Launches a kernel that begins with wait_for_previous_kernel: its blocks may be placed, and set up their barriers and
 // tensor memory, while the stream's previous kernel drains.  Calls one behind the other, before / with it: layer norm
