@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <type_traits>
 
 #include "epilogue_cell.cuh"
 #include "runtime_internal.h"
@@ -109,28 +110,6 @@ __device__ __forceinline__ float scale_value(const Q4Params& p, uint32_t raw) {
                                            : __uint_as_float(raw << 16);
 }
 
-// One sum in fp32, value by value, up to a group after which it is NaN: for the sums that the parts of an infinite
-// activation made NaN.  The few-row kernel asks for it there, because keeping inf - inf out of its cuts costs every call:
-// 8 x 8192 x 8192 with groups of 32 28.6 us instead of 26.5 by a choice for each value, 27.7 by a branch for every eight
-// (16 rows 35.2 and 39.6 instead of 34.2).
-__device__ __forceinline__ float sum_one_by_one(const Q4Params& p, long long m, long long n) {
-    const float* a = p.a + m * p.lda;
-    const unsigned char* q = p.q + n * p.ldq;
-    float total = 0.0f, sum = 0.0f;
-#pragma unroll 1
-    for (int k = 0; k < p.K; ++k) {
-        const long long at = n * p.lds + k / p.group;
-        const uint32_t w = ld_global(q + k / 2) >> 4 * (k & 1) & 15u, z = p.zeros ? ld_global(p.zeros + at) & 15u : 8u;
-        sum += ld_global(a + k) * static_cast<float>(static_cast<int>(w) - static_cast<int>(z));
-        if (k + 1 == p.K || (k + 1) % p.group == 0) {
-            total += scale_value(p, scale_raw(p, at)) * sum;
-            sum = 0.0f;
-            if (total != total) break;
-        }
-    }
-    return total;
-}
-
 template <int PACK, int RT, int MT, int SHIFT>
 struct FewCfg {
     static constexpr int kRows = PACK ? PACK : 8 * RT;
@@ -222,142 +201,172 @@ __global__ void __launch_bounds__(32 * kFewWarps)
     const uint2* scale_at = reinterpret_cast<const uint2*>(extra) + g;
 
     const int part_at = min(g, 3 * PACK - 1) * 4 + t;  // (columns without a part repeat the last: not stored)
-    float tot[MT][RT][4] = {};
-    int r = warp;
-    if (lane == 0) {
-#pragma unroll
-        for (int d = 0; d < C::kDepth - 1; ++d)
-            if (r + d * kFewWarps < runs) issue(r + d * kFewWarps, d);
-    }
-    if (r < runs) load_group(r);
+    int slot = 0;
     uint32_t phase = 0;
     bool failed = false;
-    for (int slot = 0; r < runs; r += kFewWarps) {
-        __syncwarp();  // the unit, scales and parts before these are read by every lane
+    // This warp's sums of its runs; INF: with parts made so that an infinity stays one.
+    auto sum_runs = [&](auto inf, float (&tot)[MT][RT][4]) {
+        constexpr bool INF = decltype(inf)::value;
+        int r = warp;
+        if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i < kOwn; ++i) {
-            const int e = 32 * i + lane;
-            const uint32_t raw = s_raw[i], z = z_raw[i] & 15u;
-            const uint32_t sc = p.scale_type == MXB_SCALE_F32   ? raw
-                                : p.scale_type == MXB_SCALE_F16 ? __float_as_uint(__half2float(
-                                                                      __ushort_as_half(static_cast<unsigned short>(raw))))
-                                                                : raw << 16;
-            if (e < kEntries)
-                reinterpret_cast<uint2*>(extra)[e % C::kStretches * (16 * MT + 8) + e / C::kStretches] =
-                    make_uint2(sc, 0x43004300u | z | (z << 16));
+            for (int d = 0; d < C::kDepth - 1; ++d)
+                if (r + d * kFewWarps < runs) issue(r + d * kFewWarps, INF ? (slot + d) % C::kDepth : d);
         }
-        if (r + kFewWarps < runs) load_group(r + kFewWarps);
-        const int ahead = r + (C::kDepth - 1) * kFewWarps;
-        if (lane == 0 && ahead < runs) issue(ahead, slot == 0 ? C::kDepth - 1 : slot - 1);
-        if (!mbar_wait(bar0 + 8 * slot, phase, p.timeout_ns)) failed = true;
-        if (__any_sync(0xffffffffu, failed)) {
-            failed = true;
-            break;
-        }
-        const uint8_t* unit = ring + slot * C::kUnit;
-        if constexpr (PACK) {
-            // Each lane cuts eight of a row's values, once for the run: piece lane / 4, word t = lane % 4.
+        if (r < runs) load_group(r);
+        for (; r < runs; r += kFewWarps) {
+            __syncwarp();  // the unit, scales and parts before these are read by every lane
 #pragma unroll
-            for (int m = 0; m < PACK; ++m) {
-                const float4* x = reinterpret_cast<const float4*>(unit + C::kWeightBytes + m * kRun * 4) + 2 * lane;
-                const float4 lo = x[0], hi = x[1];
-                float u[4] = {lo.x, lo.y, lo.z, lo.w}, v[4] = {hi.x, hi.y, hi.z, hi.w};
-                uint4* parts = reinterpret_cast<uint4*>(extra + C::kScaleBytes) + (g * 3 * PACK + 3 * m) * 4 + t;
-#pragma unroll
-                for (int q = 0; q < 3; ++q) parts[q * 4] = cut_pairs<false>(u, v);
+            for (int i = 0; i < kOwn; ++i) {
+                const int e = 32 * i + lane;
+                const uint32_t raw = s_raw[i], z = z_raw[i] & 15u;
+                const uint32_t sc = p.scale_type == MXB_SCALE_F32   ? raw
+                                    : p.scale_type == MXB_SCALE_F16 ? __float_as_uint(__half2float(
+                                                                          __ushort_as_half(static_cast<unsigned short>(raw))))
+                                                                    : raw << 16;
+                if (e < kEntries)
+                    reinterpret_cast<uint2*>(extra)[e % C::kStretches * (16 * MT + 8) + e / C::kStretches] =
+                        make_uint2(sc, 0x43004300u | z | (z << 16));
             }
-            __syncwarp();
-        }
-        float acc[MT][RT][4] = {};
+            if (r + kFewWarps < runs) load_group(r + kFewWarps);
+            const int ahead = r + (C::kDepth - 1) * kFewWarps;
+            if (lane == 0 && ahead < runs) issue(ahead, slot == 0 ? C::kDepth - 1 : slot - 1);
+            if (!mbar_wait(bar0 + 8 * slot, phase, p.timeout_ns)) failed = true;
+            if (__any_sync(0xffffffffu, failed)) {
+                failed = true;
+                break;
+            }
+            const uint8_t* unit = ring + slot * C::kUnit;
+            if constexpr (PACK) {
+                // Each lane cuts eight of a row's values, once for the run: piece lane / 4, word t = lane % 4.
 #pragma unroll
-        for (int c = 0; c < kPieces; ++c) {
-            // Parts of this lane's eight activations: pairs (k, k + 4) as the nibbles of a word pair up.
-            uint32_t b[RT][PACK ? 1 : 3][4];
-            if (PACK) {
-                const uint4 v = reinterpret_cast<const uint4*>(extra + C::kScaleBytes)[part_at + c * 3 * PACK * 4];
-                b[0][0][0] = v.x;
-                b[0][0][1] = v.y;
-                b[0][0][2] = v.z;
-                b[0][0][3] = v.w;
-            } else {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const uint8_t* x = unit + C::kWeightBytes + c * C::kPieceBytes + (rt * 8 + g) * 128;
-                    const float4 lo = *reinterpret_cast<const float4*>(x + (((2 * t) ^ g) << 4));
-                    const float4 hi = *reinterpret_cast<const float4*>(x + (((2 * t + 1) ^ g) << 4));
+                for (int m = 0; m < PACK; ++m) {
+                    const float4* x = reinterpret_cast<const float4*>(unit + C::kWeightBytes + m * kRun * 4) + 2 * lane;
+                    const float4 lo = x[0], hi = x[1];
                     float u[4] = {lo.x, lo.y, lo.z, lo.w}, v[4] = {hi.x, hi.y, hi.z, hi.w};
+                    uint4* parts = reinterpret_cast<uint4*>(extra + C::kScaleBytes) + (g * 3 * PACK + 3 * m) * 4 + t;
 #pragma unroll
-                    for (int q = 2; q >= 0; --q)  // (small parts first below)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) b[rt][PACK ? 0 : q][i] = cut_pair<false>(u[i], v[i]);
+                    for (int q = 0; q < 3; ++q) parts[q * 4] = cut_pairs<INF>(u, v);
                 }
+                __syncwarp();
             }
-            const int stretch = c >> SHIFT;
-            const bool flush = ((c + 1) >> SHIFT) != stretch;
+            float acc[MT][RT][4] = {};
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                uint32_t w[2];
-                uint2 sz[2];
+            for (int c = 0; c < kPieces; ++c) {
+                // Parts of this lane's eight activations: pairs (k, k + 4) as the nibbles of a word pair up.
+                uint32_t b[RT][PACK ? 1 : 3][4];
+                if (PACK) {
+                    const uint4 v = reinterpret_cast<const uint4*>(extra + C::kScaleBytes)[part_at + c * 3 * PACK * 4];
+                    b[0][0][0] = v.x;
+                    b[0][0][1] = v.y;
+                    b[0][0][2] = v.z;
+                    b[0][0][3] = v.w;
+                } else {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    w[h] = *reinterpret_cast<const uint32_t*>(unit + w_at[c] + (mt * 16 + h * 8) * (kRun / 2));
-                    sz[h] = scale_at[stretch * (16 * MT + 8) + mt * 16 + h * 8];
-                }
-                const uint32_t a1[4] = {weight_pair(w[0], sz[0].y), weight_pair(w[1], sz[1].y),
-                                        weight_pair(w[0] >> 4, sz[0].y), weight_pair(w[1] >> 4, sz[1].y)};
-                const uint32_t a2[4] = {weight_pair(w[0] >> 8, sz[0].y), weight_pair(w[1] >> 8, sz[1].y),
-                                        weight_pair(w[0] >> 12, sz[0].y), weight_pair(w[1] >> 12, sz[1].y)};
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const uint8_t* x = unit + C::kWeightBytes + c * C::kPieceBytes + (rt * 8 + g) * 128;
+                        const float4 lo = *reinterpret_cast<const float4*>(x + (((2 * t) ^ g) << 4));
+                        const float4 hi = *reinterpret_cast<const float4*>(x + (((2 * t + 1) ^ g) << 4));
+                        float u[4] = {lo.x, lo.y, lo.z, lo.w}, v[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
+                        for (int q = 2; q >= 0; --q)  // (small parts first below)
 #pragma unroll
-                    for (int q = 0; q < (PACK ? 1 : 3); ++q) {
-                        mma_bf16(acc[mt][rt], a1, b[rt][q][0], b[rt][q][1]);
-                        mma_bf16(acc[mt][rt], a2, b[rt][q][2], b[rt][q][3]);
+                            for (int i = 0; i < 4; ++i) b[rt][PACK ? 0 : q][i] = cut_pair<INF>(u[i], v[i]);
                     }
-                    if (flush) {
+                }
+                const int stretch = c >> SHIFT;
+                const bool flush = ((c + 1) >> SHIFT) != stretch;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            tot[mt][rt][i] += __uint_as_float(sz[i >> 1].x) * acc[mt][rt][i];
-                            acc[mt][rt][i] = 0.0f;
+                for (int mt = 0; mt < MT; ++mt) {
+                    uint32_t w[2];
+                    uint2 sz[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        w[h] = *reinterpret_cast<const uint32_t*>(unit + w_at[c] + (mt * 16 + h * 8) * (kRun / 2));
+                        sz[h] = scale_at[stretch * (16 * MT + 8) + mt * 16 + h * 8];
+                    }
+                    const uint32_t a1[4] = {weight_pair(w[0], sz[0].y), weight_pair(w[1], sz[1].y),
+                                            weight_pair(w[0] >> 4, sz[0].y), weight_pair(w[1] >> 4, sz[1].y)};
+                    const uint32_t a2[4] = {weight_pair(w[0] >> 8, sz[0].y), weight_pair(w[1] >> 8, sz[1].y),
+                                            weight_pair(w[0] >> 12, sz[0].y), weight_pair(w[1] >> 12, sz[1].y)};
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                        for (int q = 0; q < (PACK ? 1 : 3); ++q) {
+                            mma_bf16(acc[mt][rt], a1, b[rt][q][0], b[rt][q][1]);
+                            mma_bf16(acc[mt][rt], a2, b[rt][q][2], b[rt][q][3]);
+                        }
+                        if (flush) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                tot[mt][rt][i] += __uint_as_float(sz[i >> 1].x) * acc[mt][rt][i];
+                                acc[mt][rt][i] = 0.0f;
+                            }
                         }
                     }
                 }
             }
+            if (++slot == C::kDepth) { slot = 0; phase ^= 1u; }
         }
-        if (++slot == C::kDepth) { slot = 0; phase ^= 1u; }
-    }
-    if (failed && lane == 0) {
-        // Record it, and wait (again with a limit) for the copies still on their way to this CTA.
-        atomicOr(p.err, kErrProducer);
-        *abort_flag = 1;
-        for (int d = 0; d < C::kDepth; ++d) {
-            mbar_wait(bar0 + 8 * d, 0, p.timeout_ns);
-            mbar_wait(bar0 + 8 * d, 1, p.timeout_ns);
+    };
+    // The warps' sums added in warp order (PACK: small parts first), each for `store`: its thread's j-th, row m and column n.
+    float* red = reinterpret_cast<float*>(smem);  // [warp][MMA column][weight column]
+    auto finish = [&](const float (&tot)[MT][RT][4], auto store) {
+        if (failed && lane == 0) {
+            // Record it, and wait (again with a limit) for the copies still on their way to this CTA.
+            atomicOr(p.err, kErrProducer);
+            *abort_flag = 1;
+            for (int d = 0; d < C::kDepth; ++d) {
+                mbar_wait(bar0 + 8 * d, 0, p.timeout_ns);
+                mbar_wait(bar0 + 8 * d, 1, p.timeout_ns);
+            }
         }
+        __syncthreads();  // every warp is done with the ring
+        if (*abort_flag) return;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    red[(warp * 8 * RT + rt * 8 + 2 * t + (i & 1)) * 16 * MT + mt * 16 + (i >> 1) * 8 + g] = tot[mt][rt][i];
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * 16 * MT; i += 32 * kFewWarps) {
+            const int m = i / (16 * MT), n = i % (16 * MT);
+            if (n0 + n >= p.N) continue;
+            float v = 0.0f;
+#pragma unroll
+            for (int q = PACK ? 2 : 0; q >= 0; --q)
+#pragma unroll
+                for (int w = 0; w < kFewWarps; ++w)
+                    v += red[(w * 8 * RT + (PACK ? 3 * m + q : m)) * 16 * MT + n];
+            store(i / (32 * kFewWarps), m, n, v);
+        }
+    };
+    auto put = [&](int m, int n, float v) { p.out[(m0 + m) * p.ldo + n0 + n] = apply_cell(v, m0 + m, n0 + n, 0, p.epi); };
+    uint32_t again = 0;  // this thread's outputs that are NaN
+    {
+        float tot[MT][RT][4] = {};
+        sum_runs(std::false_type{}, tot);
+        finish(tot, [&](int j, int m, int n, float v) {
+            if (v != v) {
+                again |= 1u << j;
+            } else {
+                put(m, n, v);
+            }
+        });
     }
-    __syncthreads();  // every warp is done with the ring
-    if (*abort_flag) return;
-    // The warps' sums: [warp][MMA column][weight column], added in warp order (PACK: small parts first).
-    float* red = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                red[(warp * 8 * RT + rt * 8 + 2 * t + (i & 1)) * 16 * MT + mt * 16 + (i >> 1) * 8 + g] = tot[mt][rt][i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * 16 * MT; i += 32 * kFewWarps) {
-        const int m = i / (16 * MT), n = i % (16 * MT);
-        if (n0 + n >= p.N) continue;
-        float v = 0.0f;
-#pragma unroll
-        for (int q = PACK ? 2 : 0; q >= 0; --q)
-#pragma unroll
-            for (int w = 0; w < kFewWarps; ++w)
-                v += red[(w * 8 * RT + (PACK ? 3 * m + q : m)) * 16 * MT + n];
-        if (v != v) v = sum_one_by_one(p, m0 + m, n0 + n);
-        p.out[(m0 + m) * p.ldo + n0 + n] = apply_cell(v, m0 + m, n0 + n, 0, p.epi);
+    // NaN may be the parts inf and inf - inf of an infinite activation: those sums are made once more, with cuts that ask for
+    // infinities.  Asking in every call costs 8 x 8192 x 8192 with groups of 32 28.6 us instead of 26.5 by a choice for each
+    // value, 27.7 by a branch for every eight (16 rows 35.2 and 39.6 instead of 34.2).
+    if (__syncthreads_or(again != 0)) {
+        fence_proxy_async_shared();  // the sums in the ring, before copies are written over them
+        __syncthreads();
+        float tot[MT][RT][4] = {};
+        sum_runs(std::true_type{}, tot);
+        finish(tot, [&](int j, int m, int n, float v) {
+            if (again >> j & 1) put(m, n, v);
+        });
     }
 }
 

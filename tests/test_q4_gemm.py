@@ -180,7 +180,7 @@ def test_bad_rows_stay_alone(lib, gpu_ctx, m):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n,k,group", [(70, 200, 32), (5000, 700, 128)])
+@pytest.mark.parametrize("n,k,group", [(70, 200, 32), (5000, 700, 128), (4100, 8200, 32)])
 @pytest.mark.parametrize("m", [1, 2, 3, 8, 16, 40, 200])
 def test_infinite_activations(lib, gpu_ctx, m, n, k, group):
     """An infinity gives what fp32 gives: infinity with its weight's sign, NaN against a weight of zero or against another
@@ -204,6 +204,10 @@ def test_infinite_activations(lib, gpu_ctx, m, n, k, group):
     relu = run(lib, gpu_ctx, c, steps((mlib.MXB_EP_RELU, None, 0, 0)))
     assert torch.equal(relu, torch.where(out > 0, out, 0.0))
     assert torch.isinf(relu[0]).any()
+    # Added to the output itself: once, though some sums are made a second time.
+    added = torch.ones_like(out)
+    run(lib, gpu_ctx, c, steps((mlib.MXB_EP_ADD_FULL, added, n, 0)), added)
+    assert torch.equal(added.nan_to_num(7.0), (out + 1).nan_to_num(7.0))
 
 
 @pytest.mark.gpu
