@@ -1038,11 +1038,11 @@ __global__ void __launch_bounds__(GroupedFewCfg::kThreads, 1)
 // split gives: the other warps hand some over (setmaxnreg; the shares add up
 // to the launch's 640 x 96).
 //
-// 8192 rows, 8 groups of 4096 x 4096: 1105 us in a burst, 249 TFLOP/s of fp32
+// 8192 rows, 8 groups of 4096 x 4096: 1103 us in a burst, 249 TFLOP/s of fp32
 // products (three TF32 products each), and 1270 us once the power limit has the
 // clock at 1.57 GHz; 4096 rows of 4 groups keep the tensor cores 76% active.
-// 8191 rows, 8 groups, 1024 x 4096: grad_b with dbias 290 us.  4001 rows of 16
-// groups, 1024 x 4096: grad_a 240 us; of the 74 pairs 64 have a whole tile and
+// 8191 rows, 8 groups, 1024 x 4096: grad_b with dbias 305 us.  4001 rows of 16
+// groups, 1024 x 4096: grad_a 220-235 us; of the 74 pairs 64 have a whole tile and
 // some a tile of the few rows behind one as well (balance, not rate).
 
 struct GroupedPairCfg {
@@ -1463,8 +1463,8 @@ GroupedPlan plan_grouped(int mode, int rows, int groups, int N, int K, int num_s
             mode == kGradB ? static_cast<long long>((K + cols - 1) / cols) * groups : rows / cols + std::min(groups, rows);
         return col_tiles * ((lane_dim + lanes - 1) / lanes);
     };
-    // By the rows that a group has on average.  8 groups, 2048 x 4096, cold L2, a CTA with 64 rows to a tile / a pair
-    // with 256, in us: 80 rows 131 / -, 88 rows 131 / 127, 96 rows 133 / 129, 128 rows 166 / 135, 192 rows 228 / 191.
+    // By the rows that a group has on average.  8 groups of uneven sizes, 2048 x 4096, cold L2, a CTA with 64 rows to a
+    // tile / a pair with 256, in us: 80 rows 131 / -, 88 rows 131 / 127, 96 rows 133 / 129, 128 rows 166 / 135, 192 rows 228 / 191.
     // A pair's tile is eight times the other's, so there also have to be enough of them for the pairs: 459 rows of 12
     // groups, 811 x 1022, 32 us against the pairs' 42.  grad_b has its columns from K instead, and a CTA takes 128.
     const int cols = mode == kGradB ? K : (rows + groups - 1) / groups;

@@ -15,7 +15,7 @@
 // memory that bulk copies keep full: with loads by the threads themselves,
 // which can only be issued between a row's two barriers, the same kernels
 // reached 5.3 (forward) and 5.4 TB/s (backward); with the ring forward takes
-// 86 us at 16384 x 4096 (6.2 TB/s) and backward 130 us at 8192 x 8192 (6.2
+// 86 us at 16384 x 4096 (6.2 TB/s) and backward 131 us at 8192 x 8192 (6.1
 // TB/s), against 6.5 TB/s for a copy.  Short or odd rows are latency and
 // instructions: 25 us for the backward pass of 5003 x 1027, of which its bytes need 9.  The
 // gradients of gamma and beta are summed per thread over the rows its block

@@ -57,8 +57,8 @@ struct Q4Params {
 // is spent on addresses and bounds.
 //
 // Calls one behind the other, weights past L2: 1 x 4096 x 4096 5.6 us, 1 x 8192 x
-// 8192 14 us (2.5 TB/s), 8 x 8192 x 8192 with groups of 32, fp32 scales and zero
-// points 27.5 us (1.6 TB/s).  What bounds it there are the
+// 8192 13.7 us (2.6 TB/s), 8 x 8192 x 8192 with groups of 32, fp32 scales and zero
+// points 26.3 us (1.7 TB/s).  What bounds it there are the
 // instructions that make bf16 pairs of nibbles and scale each group's sums:
 // 55% of the issue slots and 48% of the ALU's.
 
@@ -432,8 +432,8 @@ cudaError_t run_few_rows_width(const Q4Params& p, int num_sms, cudaStream_t stre
 // summing its own stretch of K; the totals meet in distributed shared memory,
 // added in CTA order.
 //
-// 1000 x 8192 x 8192, groups of 128: 326 us in a burst (412 TFLOP/s, 1236 of the
-// tensor core's bf16 ones), 377 us once the power limit has the clock at 1.57
+// 1000 x 8192 x 8192, groups of 128: 324 us in a burst (414 TFLOP/s, 1243 of the
+// tensor core's bf16 ones), 346-380 us once the power limit has the clock at 1.57
 // GHz; the tensor cores are then 65% active.
 
 constexpr int kManyCols = 128;  // rows of A per tile, at most
@@ -951,8 +951,8 @@ int q4_gemm(GpuCtx* ctx, Q4Params& p, const mxb_ep_step* steps, int n_steps, voi
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     p.timeout_ns = ctx->timeout_ns;
     p.err = ctx->d_err;
-    // 8192 x 8192, groups of 128, cold L2: 16 rows 35.8 us in the few-row kernel, whose time grows with every eight rows
-    // (8: 29.6); 17 rows 50 us in the other, whose time is that of 32.
+    // 8192 x 8192, groups of 128, calls one behind the other: 16 rows 30 us in the few-row kernel, whose time grows with
+    // every eight rows (8: 23); 17 rows 41 us in the other, whose time is nearly that of 96 (49).
     if (p.M > 16) return run_many_rows(ctx, p, st);
     const cudaError_t e = p.M == 1   ? run_few_rows_width<1, 1>(p, ctx->num_sms, st)
                           : p.M == 2 ? run_few_rows_width<2, 1>(p, ctx->num_sms, st)

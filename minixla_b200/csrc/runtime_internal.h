@@ -246,8 +246,8 @@ cudaError_t allow_shared(int bytes) {
 
 // Launches a kernel that begins with wait_for_previous_kernel: its blocks may be placed, and set up their barriers and
 // tensor memory, while the stream's previous kernel drains.  Calls one behind the other, before / with it: layer norm
-// 8 x 4096 5.7 / 3.1 us, 4-bit product 1 x 4096 x 4096 8.2 / 5.6 us and 17 x 8192 x 8192 43 / 39 us, grouped product of two
-// rows 17 / 15.8 us; calls of 200 us and more are the same either way.  cluster: blocks to a cluster.
+// 8 x 4096 5.7 / 3.1 us, 4-bit product 1 x 4096 x 4096 8.2 / 5.6 us and 17 x 8192 x 8192 43 / 41 us, grouped product of two
+// rows 17 / 14.8 us; calls of 200 us and more are the same either way.  cluster: blocks to a cluster.
 template <typename... P, typename... A>
 cudaError_t launch_early(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, int cluster,
                          A&&... args) {
