@@ -60,7 +60,7 @@ struct Q4Params {
 // 8192 13.7 us (2.6 TB/s), 8 x 8192 x 8192 with groups of 32, fp32 scales and zero
 // points 26.3 us (1.7 TB/s).  What bounds it there are the
 // instructions that make bf16 pairs of nibbles and scale each group's sums:
-// 55% of the issue slots and 48% of the ALU's.
+// 54% of the issue slots and 48% of the ALU's.
 
 constexpr int kFewWarps = 8;
 
