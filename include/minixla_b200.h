@@ -382,9 +382,9 @@ MXB_API int mxb_layer_norm_backward(GpuCtx* ctx, const float* dy, long long lddy
  *   W[k, n] = (q[n, k] - z[n, k / group]) * scales[n * lds + k / group].
  * Q: N rows ldq bytes apart, two values to a byte, the lower k in the low four
  * bits (ldq % 16 == 0, 16-byte aligned, ldq >= (K + 1) / 2; what lies behind
- * column K is not used, so Q may be some columns of a wider matrix).  scales: MXB_SCALE_* values, row pitch lds elements;
- * zeros: one byte (its low four bits) per scale, same pitch, or NULL for 8
- * everywhere.  group is a multiple of 32.  A needs a 16-byte aligned base and
+ * column K is not used, so Q may be some columns of a wider matrix).  scales:
+ * MXB_SCALE_* values, row pitch lds elements; zeros: one byte (its low four
+ * bits) per scale, same pitch, or NULL for 8 everywhere.  group is a multiple of 32.  A needs a 16-byte aligned base and
  * lda % 4 == 0.  Epilogue steps as mxb_fused_gemm; an ADD_FULL operand may be
  * out itself (same pointer and pitch), otherwise out overlaps no input.
  * M, N, K <= 2^30.  Products and sums are
@@ -415,8 +415,8 @@ MXB_API int mxb_q4_gemm(GpuCtx* ctx, const float* A, long long lda, const unsign
  * the buffers: group e begins at offsets[e] clamped to 0 .. rows and ends at
  * offsets[e+1] clamped to its begin .. rows.  Each value of a row that
  * decreasing offsets give to several groups is one of their results (what the
- * steps add to out itself may then be added more than once).  groups <= MXB_MAX_GROUPS; lda, ldb and b_stride are
- * multiples of 4, A and B 16-byte aligned.  Steps: ADD_FULL, RELU, SCALE and
+ * steps add to out itself may then be added more than once).
+ * groups <= MXB_MAX_GROUPS; lda, ldb and b_stride are multiples of 4, A and B 16-byte aligned.  Steps: ADD_FULL, RELU, SCALE and
  * RELU_GRAD as named above (i: the row of out), and ADD_ROW with
  * operand[e * ld_or_size + j] (ld_or_size 0: one row for all groups).
  * An ADD_FULL operand may be out itself (same pointer and pitch), otherwise

@@ -1457,7 +1457,7 @@ constexpr int kMaxSplits = 8;
 
 GroupedPlan plan_grouped(int mode, int rows, int groups, int N, int K, int num_sms) {
     const int lane_dim = mode == kGradA ? K : N;
-    // At most so many tiles, whatever the offsets are: a part of a column tile more for each group that has a row.
+    // At most so many tiles for non-decreasing offsets: a part of a column tile more for each group that has a row.
     auto most_tiles = [&](int lanes, int cols) {
         const long long col_tiles =
             mode == kGradB ? static_cast<long long>((K + cols - 1) / cols) * groups : rows / cols + std::min(groups, rows);
